@@ -38,6 +38,16 @@ class Sampling(C.Structure):
                 ("repeat_penalty", C.c_float)]
 
 
+class KvShape(C.Structure):
+    _fields_ = [("format", C.c_uint32), ("n_kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("page_size", C.c_uint32), ("n_pages", C.c_uint32)]
+
+
+class LogitRules(C.Structure):
+    _fields_ = [("rows", View), ("history", View), ("bias_tokens", View), ("bias_values", View), ("masks", View),
+                ("n_history", C.c_uint32), ("n_bias", C.c_uint32), ("n_masks", C.c_uint32)]
+
+
 class DeltaShape(C.Structure):
     _fields_ = [("n_k_heads", C.c_uint32), ("n_v_heads", C.c_uint32), ("k_dim", C.c_uint32), ("v_dim", C.c_uint32)]
 
@@ -195,6 +205,15 @@ PROTOTYPES = {
     "bch_matmul_experts": (_int, [_vp, _u32, View, C.POINTER(View), _u32, _u32, _u32, View, C.c_int, View, View,
                                   _u32, View, _u32]),
     "bch_moe_combine": (_int, [_vp, View, View, View, _u32, _u32, _u32]),
+    "bch_kv_page_bytes": (_u64, [C.POINTER(KvShape)]),
+    "bch_kv_plan_check": (_int, [C.POINTER(KvShape), _u32, _u32, _vp, _vp, _vp, _u64]),
+    "bch_kv_plan_new": (_int, [_vp, C.POINTER(KvShape), _u32, C.POINTER(_vp)]),
+    "bch_kv_plan_free": (None, [_vp]),
+    "bch_kv_plan_set": (_int, [_vp, _u32, _vp, _vp, _vp, _u64]),
+    "bch_kv_store": (_int, [_vp, _vp, View, View, _u32, View, _u32]),
+    "bch_kv_load": (_int, [_vp, _vp, View, _u32, _u32, _u32, View, View]),
+    "bch_attention_paged": (_int, [_vp, _vp, View, View, _u32, View, _u32]),
+    "bch_logits_edit": (_int, [_vp, View, View, _u32, _u32, C.POINTER(LogitRules)]),
     "bch_lfm2_new": (_int, [_vp, C.POINTER(Lfm2Model), _u32, _int, C.POINTER(_vp)]),
     "bch_lfm2_free": (None, [_vp]),
     "bch_lfm2_n_past": (_u32, [_vp]),

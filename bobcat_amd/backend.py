@@ -15,7 +15,7 @@ from enum import IntEnum
 
 import numpy as np
 
-from ._lib import BobcatError, Norm as _Norm, ProfileEntry, View as _View, check, lib
+from ._lib import BobcatError, KvShape, LogitRules, Norm as _Norm, ProfileEntry, View as _View, check, lib
 
 
 class Format(IntEnum):
@@ -89,6 +89,70 @@ class NormSpec:
 
 def _view(v: ViewRef) -> _View:
     return v.c()
+
+
+class KvFormat(IntEnum):
+    """What a paged cache keeps a row as (bch_kv_format)."""
+    F16 = 0
+    I8 = 1
+    F8 = 2
+
+
+# One row's rules (bch_logit_row), as an array's type; NO_MASK in `mask` is no mask.
+LOGIT_ROW = np.dtype([("history_at", "<u4"), ("history_len", "<u4"), ("bias_at", "<u4"), ("bias_len", "<u4"),
+                      ("mask", "<u4"), ("repeat", "<f4"), ("presence", "<f4"), ("frequency", "<f4")])
+NO_MASK = 0xFFFFFFFF
+
+
+def kv_shape(fmt, n_kv_heads: int, head_dim: int, page_size: int, n_pages: int) -> KvShape:
+    """A paged cache's shape; `fmt` a KvFormat or its name in lower case."""
+    return KvShape(KvFormat[fmt.upper()] if isinstance(fmt, str) else int(fmt), n_kv_heads, head_dim, page_size, n_pages)
+
+
+def kv_page_bytes(shape: KvShape) -> int:
+    """Bytes of one page; 0 for a shape that is not supported."""
+    return lib().bch_kv_page_bytes(C.byref(shape))
+
+
+def _batch(n_past, n_new, pages):
+    """A batch's arguments: lengths, and each sequence's pages one list after the other."""
+    past, new = np.ascontiguousarray(n_past, np.uint32), np.ascontiguousarray(n_new, np.uint32)
+    if past.shape != new.shape or past.ndim != 1:
+        raise ValueError("n_past and n_new hold one number for each sequence")
+    flat = np.ascontiguousarray([p for seq in pages for p in seq], np.uint32)
+    return past, new, flat, (past.size, past.ctypes.data, new.ctypes.data, flat.ctypes.data, flat.size)
+
+
+def kv_plan_check(shape: KvShape, n_heads: int, n_past, n_new, pages) -> None:
+    """Raise what KvPlan and its set() would, without a device."""
+    *_keep, args = _batch(n_past, n_new, pages)
+    check(lib().bch_kv_plan_check(C.byref(shape), n_heads, *args))
+
+
+class KvPlan:
+    """A batch of sequences over a paged cache (bch_kv_plan)."""
+
+    def __init__(self, hip: "Hip", shape: KvShape, n_heads: int):
+        h = C.c_void_p()
+        check(lib().bch_kv_plan_new(hip.handle, C.byref(shape), n_heads, C.byref(h)))
+        self.handle, self.shape, self.n_heads = h.value, shape, n_heads
+        hip._dependents.add(self)
+
+    def set(self, n_past, n_new, pages) -> None:
+        """The batch: past positions and new tokens of each sequence, and each sequence's list of pages."""
+        *_keep, args = _batch(n_past, n_new, pages)
+        check(lib().bch_kv_plan_set(self.handle, *args))
+
+    def close(self) -> None:
+        if self.handle:
+            lib().bch_kv_plan_free(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 class Hip:
@@ -250,6 +314,27 @@ class Hip:
                                          eps, rope_theta, n_rot, _view(k_cache), _view(v_cache), int(kv_half),
                                          _view(scratch), _view(out), n_heads, n_kv_heads, head_dim, pos, n_ctx))
 
+    def kv_plan(self, fmt, n_kv_heads, head_dim, page_size, n_pages, n_heads) -> KvPlan:
+        return KvPlan(self, kv_shape(fmt, n_kv_heads, head_dim, page_size, n_pages), n_heads)
+
+    def kv_store(self, plan: KvPlan, cache, k, k_stride, v, v_stride):
+        check(lib().bch_kv_store(self.handle, plan.handle, _view(cache), _view(k), k_stride, _view(v), v_stride))
+
+    def kv_load(self, plan: KvPlan, cache, seq, first, n, k, v):
+        check(lib().bch_kv_load(self.handle, plan.handle, _view(cache), seq, first, n, _view(k), _view(v)))
+
+    def attention_paged(self, plan: KvPlan, cache, q, q_stride, out, out_stride):
+        check(lib().bch_attention_paged(self.handle, plan.handle, _view(cache), _view(q), q_stride, _view(out),
+                                        out_stride))
+
+    def logits_edit(self, logits, out, n_rows, n_vocab, rows, *, history=None, n_history=0, bias_tokens=None,
+                    bias_values=None, n_bias=0, masks=None, n_masks=0):
+        """`rows` holds n_rows LOGIT_ROW; a list of no entries needs no view."""
+        view = lambda v: _View() if v is None else _view(v)  # noqa: E731
+        rules = LogitRules(view(rows), view(history), view(bias_tokens), view(bias_values), view(masks), n_history,
+                           n_bias, n_masks)
+        check(lib().bch_logits_edit(self.handle, _view(logits), _view(out), n_rows, n_vocab, C.byref(rules)))
+
     def matmul(self, fmt, weights, n_rows, n_cols, x, y, n_tokens, store: Store):
         check(lib().bch_matmul(self.handle, int(fmt), _view(weights), n_rows, n_cols, _view(x),
                                _view(y), n_tokens, int(store)))
@@ -309,5 +394,6 @@ def row_bytes(fmt: int, n_cols: int) -> int:
     return lib().bch_row_bytes(int(fmt), n_cols)
 
 
-__all__ = ["Hip", "Buffer", "ViewRef", "NormSpec", "Format", "Store", "BobcatError",
-           "attention_scratch_floats", "attention_decode_scratch_floats", "row_bytes"]
+__all__ = ["Hip", "Buffer", "KvFormat", "KvPlan", "LOGIT_ROW", "NO_MASK", "ViewRef", "NormSpec", "Format", "Store",
+           "BobcatError", "attention_scratch_floats", "attention_decode_scratch_floats", "kv_page_bytes",
+           "kv_plan_check", "kv_shape", "row_bytes"]

@@ -1,0 +1,143 @@
+// The rules of a batch's rows on their logits, before the sampler: penalties
+// for the tokens of the row's history, biases, and a grammar's mask.
+//
+// With c the times that a token occurs in the history,
+//   y = (x > 0 ? x / repeat : x·repeat) − (presence + frequency·c)  for c > 0, else x,
+// then y + b for every bias (token, b) of the row in list order, then −inf
+// where the mask's bit is 0.
+//
+// One launch and one pass: a workgroup owns a slice of one row's vocabulary,
+// counts the whole history's tokens that fall into it in LDS (integers: the
+// order of the atomics changes nothing), and reads and writes its logits once.
+// That a row's history is read by each of its slices costs less than counters
+// in memory would: 4 bytes a token out of the L2 against 8 bytes a logit.
+#include <cmath>
+
+#include "device.h"
+#include "kernels.h"
+#include "runtime.h"
+
+namespace bch {
+
+constexpr uint32_t kEditThreads = 256;
+
+struct EditArgs {
+  const float *logits;
+  float *out;
+  const bch_logit_row *rows;
+  const uint32_t *history, *bias_tokens, *masks;
+  const float *bias_values;
+  uint32_t n_vocab, n_history, n_bias, n_masks, slices;
+};
+
+// PER logits per thread: slices of 256·PER tokens.
+template <uint32_t PER>
+__global__ __launch_bounds__(kEditThreads) void k_logits_edit(EditArgs a) {
+  constexpr uint32_t SLICE = kEditThreads * PER;
+  __shared__ uint32_t count_s[SLICE];  // then the logits as the biases change them
+  __shared__ uint32_t owner_s[SLICE];
+  const uint32_t row = blockIdx.x / a.slices, base = blockIdx.x % a.slices * SLICE, tid = threadIdx.x;
+  const uint32_t len = min(SLICE, a.n_vocab - base);
+  const bch_logit_row r = a.rows[row];
+  const uint64_t at = (uint64_t)row * a.n_vocab + base;
+  float x[PER];
+#pragma unroll
+  for (uint32_t j = 0; j < PER; j++) {
+    const uint32_t i = tid + kEditThreads * j;
+    x[j] = i < len ? a.logits[at + i] : 0.f;
+  }
+  // Lists never leave the buffers, whatever the row says.
+  const uint32_t h0 = min(r.history_at, a.n_history), hn = min(r.history_len, a.n_history - h0);
+  const uint32_t b0 = min(r.bias_at, a.n_bias), bn = min(r.bias_len, a.n_bias - b0);
+  if (hn) {
+    for (uint32_t i = tid; i < SLICE; i += kEditThreads) count_s[i] = 0;
+    __syncthreads();
+    for (uint32_t i = tid; i < hn; i += kEditThreads) {
+      const uint32_t t = a.history[h0 + i] - base;  // (below base: wraps past the slice)
+      if (t < len) atomicAdd(&count_s[t], 1u);
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t j = 0; j < PER; j++) {
+      const uint32_t c = count_s[tid + kEditThreads * j];
+      if (c) x[j] = (x[j] > 0.f ? x[j] / r.repeat : x[j] * r.repeat) - (r.presence + r.frequency * (float)c);
+    }
+  }
+  if (bn) {
+    float *y_s = reinterpret_cast<float *>(count_s);
+#pragma unroll
+    for (uint32_t j = 0; j < PER; j++) {
+      y_s[tid + kEditThreads * j] = x[j];  // (each thread's own counters)
+      owner_s[tid + kEditThreads * j] = ~0u;
+    }
+    __syncthreads();
+    // 256 biases at a time, each in turn added by the lowest thread that has
+    // one for its token: one round, or as many as a token is named.
+    for (uint32_t i0 = 0; i0 < bn; i0 += kEditThreads) {
+      const uint32_t i = i0 + tid;
+      const uint32_t t = i < bn ? a.bias_tokens[b0 + i] - base : ~0u;
+      bool waiting = t < len;
+      while (__syncthreads_or(waiting)) {
+        if (waiting) atomicMin(&owner_s[t], tid);
+        __syncthreads();
+        const bool mine = waiting && owner_s[t] == tid;
+        __syncthreads();
+        if (mine) {
+          y_s[t] += a.bias_values[b0 + i];
+          owner_s[t] = ~0u;
+          waiting = false;
+        }
+      }
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < PER; j++) x[j] = y_s[tid + kEditThreads * j];
+  }
+  const bool masked = r.mask != BCH_NO_MASK, known = r.mask < a.n_masks;
+  const uint32_t *mask = known ? a.masks + (uint64_t)r.mask * ((a.n_vocab + 31) / 32) : nullptr;
+#pragma unroll
+  for (uint32_t j = 0; j < PER; j++) {
+    const uint32_t i = tid + kEditThreads * j;
+    if (i >= len) continue;
+    const uint32_t t = base + i;
+    const bool allowed = !masked || (known && (mask[t / 32] >> (t % 32) & 1));
+    a.out[at + i] = allowed ? x[j] : -INFINITY;
+  }
+}
+
+}  // namespace bch
+
+using namespace bch;
+
+extern "C" int bch_logits_edit(bch_ctx *ctx, bch_view logits, bch_view out, uint32_t n_rows, uint32_t n_vocab,
+                               const bch_logit_rules *rules) {
+  if (!rules) return fail(BCH_ERR_ARGUMENT, "logits_edit: no rules");
+  if (!n_vocab || n_vocab > 1u << 30) return fail(BCH_ERR_ARGUMENT, "logits_edit: rows of %u logits", n_vocab);
+  EditArgs a{};
+  const uint64_t bytes = (uint64_t)n_rows * n_vocab * 4;
+  BCH_TRY(view_ptr(ctx, "logits_edit", logits, bytes, &a.logits));
+  BCH_TRY(view_ptr(ctx, "logits_edit", out, bytes, &a.out));
+  BCH_TRY(view_ptr(ctx, "logits_edit", rules->rows, (uint64_t)n_rows * sizeof(bch_logit_row), &a.rows));
+  if (rules->n_history) BCH_TRY(view_ptr(ctx, "logits_edit", rules->history, (uint64_t)rules->n_history * 4, &a.history));
+  if (rules->n_bias) {
+    BCH_TRY(view_ptr(ctx, "logits_edit", rules->bias_tokens, (uint64_t)rules->n_bias * 4, &a.bias_tokens));
+    BCH_TRY(view_ptr(ctx, "logits_edit", rules->bias_values, (uint64_t)rules->n_bias * 4, &a.bias_values));
+  }
+  if (rules->n_masks)
+    BCH_TRY(view_ptr(ctx, "logits_edit", rules->masks, (uint64_t)rules->n_masks * ((n_vocab + 31) / 32) * 4, &a.masks));
+  for (const void *p : {(const void *)a.logits, (const void *)a.out, (const void *)a.rows, (const void *)a.history,
+                        (const void *)a.bias_tokens, (const void *)a.bias_values, (const void *)a.masks})
+    if (reinterpret_cast<uintptr_t>(p) % 4) return fail(BCH_ERR_ARGUMENT, "logits_edit: operands must be 4-byte aligned");
+  const uintptr_t from = reinterpret_cast<uintptr_t>(a.logits), to = reinterpret_cast<uintptr_t>(a.out);
+  if (from != to && from < to + bytes && to < from + bytes)
+    return fail(BCH_ERR_ARGUMENT, "logits_edit: the outputs lie over the logits (the same place or another is wanted)");
+  a.n_vocab = n_vocab;
+  a.n_history = rules->n_history;
+  a.n_bias = rules->n_bias;
+  a.n_masks = rules->n_masks;
+  constexpr uint32_t kPer = 8;
+  a.slices = div_ceil(n_vocab, kEditThreads * kPer);
+  if ((uint64_t)n_rows * a.slices > 0x7fffffffu) return fail(BCH_ERR_ARGUMENT, "logits_edit: too many logits");
+  return launch(ctx, {"logits_edit", n_rows, n_vocab, 0}, [&](hipStream_t s) {
+    if (n_rows) k_logits_edit<kPer><<<n_rows * a.slices, kEditThreads, 0, s>>>(a);
+  });
+}

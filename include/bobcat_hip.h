@@ -314,6 +314,88 @@ int bch_moe_combine(bch_ctx *ctx, bch_view x, bch_view route, bch_view y, uint32
                     uint32_t n_tokens);
 
 /* ------------------------------------------------------------------ */
+/* Batches over a paged key/value cache (no counterpart in the          */
+/* reference, whose caches hold one sequence each).                     */
+/*                                                                      */
+/* A cache is a buffer of pages, each with the keys and values of        */
+/* page_size positions of every KV head.  A batch is a list of sequences */
+/* of n_past positions already in the cache and n_new tokens that        */
+/* this step brings; the tokens' rows (keys, values, queries, outputs)   */
+/* lie sequence after sequence.  Position p of a sequence is position    */
+/* p % page_size of page p / page_size of the sequence's list.  A plan   */
+/* holds one batch, checked on the host and laid out on the device once, */
+/* for the launches of all layers: their caches have the same shape and  */
+/* the same page numbers, one buffer (or view) for each layer.           */
+/*                                                                      */
+/* The rows x of a position and head are kept as f16, or with a scale of */
+/* their own: s = clamp(max|x| / top, 2^-40, 2^60), y = x / s rounded to */
+/* the nearest int8 (top 127) or e4m3 (top 448), ties to even, and read  */
+/* back as s·y.  A row with a NaN or an infinity reads back as NaN.      */
+/*                                                                      */
+/* Layout, for programs that move pages: a page is [head][16 positions], */
+/* a block of 16 positions of a head its keys, its values and (8-bit     */
+/* formats) its 16 key scales and 16 value scales as f32.  With E        */
+/* elements in 16 bytes (8 or 16) and M = E / 4, element d of the        */
+/* block's position i lies at element (d / E·16 + i)·E + d % E of the    */
+/* keys and (((d / 16M·4 + i / 4)·16 + d % 16)·M + d / 16 % M)·4 + i % 4 */
+/* of the values.  Pages can be copied whole.                            */
+/* ------------------------------------------------------------------ */
+typedef enum bch_kv_format { BCH_KV_F16 = 0, BCH_KV_I8 = 1, BCH_KV_F8 = 2 /* e4m3 */ } bch_kv_format;
+
+typedef struct bch_kv_shape {
+  uint32_t format;     /* bch_kv_format */
+  uint32_t n_kv_heads; /* at most 256 */
+  uint32_t head_dim;   /* 64, 128 or 256 */
+  uint32_t page_size;  /* positions: 16 to 512, a multiple of 16 */
+  uint32_t n_pages;    /* of the cache */
+} bch_kv_shape;
+typedef struct bch_kv_plan bch_kv_plan;
+
+/* Bytes of a page, 0 for a shape that is not supported; a cache needs n_pages
+ * times as many, 16-byte aligned. */
+uint64_t bch_kv_page_bytes(const bch_kv_shape *shape);
+/* What bch_kv_plan_new and bch_kv_plan_set refuse, without a device:
+ * `pages` lists the page numbers of the sequences one after the other,
+ * ceil((n_past + n_new) / page_size) each, n_pages in all.  n_heads query
+ * heads in groups of at most 32 per KV head.  BCH_ERR_UNSUPPORTED_FORMAT and
+ * BCH_ERR_ATTENTION_LIMITS for the shape; BCH_ERR_OUT_OF_BOUNDS for a page
+ * past the cache's; BCH_ERR_ARGUMENT for a list of another length, a sequence
+ * of 2^31 positions, or a page that receives tokens and is named twice in the
+ * batch (pages that are only read may be shared by sequences). */
+int bch_kv_plan_check(const bch_kv_shape *shape, uint32_t n_heads, uint32_t n_seqs, const uint32_t *n_past,
+                      const uint32_t *n_new, const uint32_t *pages, uint64_t n_pages);
+/* A plan without a batch yet; to be freed before its context is closed. */
+int bch_kv_plan_new(bch_ctx *ctx, const bch_kv_shape *shape, uint32_t n_heads, bch_kv_plan **out);
+void bch_kv_plan_free(bch_kv_plan *plan);
+/* Give the plan a batch (copied: the arrays are free on return).  Fails with
+ * BCH_ERR_BUSY while work is recorded or in flight, as bch_write does.  A batch
+ * that is refused leaves the plan as it was; after any other failure it has none. */
+int bch_kv_plan_set(bch_kv_plan *plan, uint32_t n_seqs, const uint32_t *n_past, const uint32_t *n_new,
+                    const uint32_t *pages, uint64_t n_pages);
+
+/* Quantise the new tokens' keys and values, rows of n_kv_heads·head_dim
+ * floats k_stride and v_stride floats apart (16-byte aligned, strides a
+ * multiple of 4), into their pages; every other byte of the cache keeps its
+ * value. */
+int bch_kv_store(bch_ctx *ctx, const bch_kv_plan *plan, bch_view cache, bch_view k, uint32_t k_stride, bch_view v,
+                 uint32_t v_stride);
+/* Read positions first .. first + n of sequence `seq` of the batch back as
+ * floats, [n][n_kv_heads][head_dim] at k and at v. */
+int bch_kv_load(bch_ctx *ctx, const bch_kv_plan *plan, bch_view cache, uint32_t seq, uint32_t first, uint32_t n,
+                bch_view k, bch_view v);
+/* Causal attention of the new tokens, whose keys and values bch_kv_store has
+ * put into the pages before: token i of a sequence attends to its positions
+ * 0 .. n_past + i, softmax(q·k/√head_dim)·v.  Query and output rows of
+ * n_heads·head_dim floats, q_stride and out_stride floats apart (16-byte
+ * aligned, strides a multiple of 4); query head h reads KV head
+ * h / (n_heads / n_kv_heads).  `out` may not lie over `q`.  What a query does
+ * not see has no part in its output, whatever it holds.  The queries and the
+ * probabilities enter the products with ~22 bits, as in
+ * bch_attention_prefill. */
+int bch_attention_paged(bch_ctx *ctx, const bch_kv_plan *plan, bch_view cache, bch_view q, uint32_t q_stride,
+                        bch_view out, uint32_t out_stride);
+
+/* ------------------------------------------------------------------ */
 /* Sampling                                                            */
 /* ------------------------------------------------------------------ */
 
@@ -347,6 +429,41 @@ int bch_sample(bch_ctx *ctx, bch_view logits, uint32_t n_vocab, bch_view recent,
  * for u outside [0, 1). */
 int bch_sample_draw(bch_ctx *ctx, bch_view logits, uint32_t n_vocab, bch_view recent, uint32_t n_recent,
                     const bch_sampling *settings, float u, bch_view out);
+
+/* The rules of one row of logits: where the row's tokens so far and its
+ * biases lie in the lists, which mask it has, and its penalties. */
+#define BCH_NO_MASK 0xffffffffu
+typedef struct bch_logit_row {
+  uint32_t history_at, history_len; /* of `history` */
+  uint32_t bias_at, bias_len;       /* of `bias_tokens` and `bias_values` */
+  uint32_t mask;                    /* of `masks`, or BCH_NO_MASK */
+  float repeat;                     /* above 0; 1 is none */
+  float presence, frequency;        /* 0 is none */
+} bch_logit_row;
+
+/* The lists that the rows share, in device memory; a list of no entries
+ * needs no view. */
+typedef struct bch_logit_rules {
+  bch_view rows;                     /* n_rows bch_logit_row */
+  bch_view history;                  /* u32 tokens */
+  bch_view bias_tokens, bias_values; /* u32 tokens, and floats */
+  bch_view masks;                    /* ceil(n_vocab / 32) u32 each: token t is allowed by bit t % 32 of word t / 32 */
+  uint32_t n_history, n_bias, n_masks;
+} bch_logit_rules;
+
+/* Penalties, biases and masks on n_rows rows of n_vocab logits, from
+ * `logits` to `out` (the same place, or one apart from it), for each token
+ * that occurs c > 0 times in the row's history
+ *   x <- (x > 0 ? x / repeat : x·repeat) - (presence + frequency·c),
+ * then x <- x + b for each of the row's biases, in list order where a token
+ * has several, then -inf for each token that the row's mask does not allow
+ * (whatever its logit was).  The whole history counts, as often as a token
+ * occurs; bch_sample's penalty takes the last 64 tokens and no counts.
+ * Tokens that are not below n_vocab change nothing, lists end where their
+ * buffers' entries do, and a mask that is not below n_masks (other than
+ * BCH_NO_MASK) allows nothing.  No counterpart in the reference. */
+int bch_logits_edit(bch_ctx *ctx, bch_view logits, bch_view out, uint32_t n_rows, uint32_t n_vocab,
+                    const bch_logit_rules *rules);
 
 /* ------------------------------------------------------------------ */
 /* Gated DeltaNet and gated attention (Qwen3.5)                        */
