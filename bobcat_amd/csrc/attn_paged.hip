@@ -1,11 +1,32 @@
-// Attention of a batch's new tokens over the paged cache: row i of a sequence
+// Attention of a batch's new tokens over the paged cache: token i of a sequence
 // with `past` positions attends to positions 0 .. past + i of its pages,
-// softmax(q·k/√hd)·v with the keys and values that the cache holds (in the
-// 8-bit formats scale·integer).
+// softmax(q·k/√hd)·v, with the rows that the cache holds (in the 8-bit formats
+// scale·integer or scale·e4m3).
 //
-// One wave per token and query head: a lane scores one key of 64 at a time
-// (the running maximum and sum of an online softmax), then owns every 64th
-// element of the output.
+// The query heads of a KV head's group and a sequence's tokens are one list of
+// packed rows, row = token·group + head: every row of a tile reads the same
+// keys, whatever the group.  Two kernels share the mathematics:
+//   k_attn_tokens: sequences of at most 16 packed rows (decoding, drafts).  A
+//     wave takes 32 keys at a time from memory straight into the operands of
+//     16x16x32 MFMAs; the waves of a workgroup, and the splits of a sequence,
+//     have keys of their own and are joined.  Bound by the cache's bytes.
+//   k_attn_chunk: tiles of 128 packed rows, 32 a wave, that share the keys
+//     through LDS.  Bound by the matrix cores and the softmax's instructions.
+// (The rule: with 16 rows or fewer the narrow tile wastes no matrix work and
+// needs no barrier; above, the wide one reads the cache once for 128 rows.)
+//
+// Scores come as S^T = K·Q^T (keys x rows), so that a lane holds scores of one
+// row, and as probabilities they are in place as an operand of O^T = V^T·P^T.
+// The cache's elements are exact in f16.  Queries, taken times scale·log2 e,
+// and probabilities enter as f16 high and low parts (~22 bits) and accumulate
+// in f32.  With a row's key scale a and value scale b (1 in f16) and a running
+// reference m,
+//   u = a·s − m,  p = 2^u,  l += p,  O += (p·b)·v,
+// where m follows the largest u + log2 b: p·b then stays near 1 as f16 wants
+// it, whatever the scales, and p needs no bound of its own (scales lie in
+// 2^-40 .. 2^60).  m moves only when p·b would pass 2^8, so most steps rescale
+// nothing.
+#include <algorithm>
 #include <cmath>
 
 #include "device.h"
@@ -15,62 +36,698 @@
 
 namespace bch {
 
+typedef _Float16 ah2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 ah4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 ah8_t __attribute__((ext_vector_type(8)));
+typedef float af2_t __attribute__((ext_vector_type(2)));
+typedef float af4_t __attribute__((ext_vector_type(4)));
+typedef float af16_t __attribute__((ext_vector_type(16)));
+typedef uint32_t au4_t __attribute__((ext_vector_type(4)));
+
+constexpr float kLazy = 8.f;             // p·b may pass its reference by 2^kLazy
+constexpr float kUnset = -INFINITY;      // in its place, of a row that has seen no key yet
+
+// Four elements of 8 bits as f16, exactly.
 template <uint32_t FORMAT>
-__device__ __forceinline__ float paged_float(const uint8_t *p) {
-  if constexpr (FORMAT == BCH_KV_F16) return half_bits_to_float(*reinterpret_cast<const uint16_t *>(p));
-  if constexpr (FORMAT == BCH_KV_I8) return (float)*reinterpret_cast<const int8_t *>(p);
-  return __builtin_amdgcn_cvt_f32_fp8((int)*p, 0);
+__device__ __forceinline__ ah4_t widen(uint32_t w) {
+  if constexpr (FORMAT == BCH_KV_I8) {
+    // Behind 0x64 the byte v + 128 is the f16 number 1024 + 128 + v.
+    const uint32_t x = w ^ 0x80808080u;
+    const uint32_t lo = __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u);
+    const uint32_t hi = __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u);
+    const ah2_t bias = {(_Float16)1152.f, (_Float16)1152.f};
+    const ah2_t a = __builtin_bit_cast(ah2_t, lo) - bias, b = __builtin_bit_cast(ah2_t, hi) - bias;
+    return {a[0], a[1], b[0], b[1]};
+  } else {
+    const ah2_t a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, false);
+    const ah2_t b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, true);
+    return {a[0], a[1], b[0], b[1]};
+  }
+}
+__device__ __forceinline__ ah8_t join(ah4_t a, ah4_t b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+__device__ __forceinline__ ah4_t halves(uint32_t a, uint32_t b) { return __builtin_bit_cast(ah4_t, ((uint64_t)b << 32) | a); }
+
+// log2 b to within 0.09, plus 127, from a scale's bits (0 for b = 0).
+__device__ __forceinline__ float scale_log(float b) { return (float)__float_as_int(b) * 0x1p-23f; }
+
+__device__ __forceinline__ bool not_finite(_Float16 x) { return (__builtin_bit_cast(uint16_t, x) & 0x7c00) == 0x7c00; }
+
+// The lowest n bytes (0 to 4, clamped).
+__device__ __forceinline__ uint32_t bytes_below(int n) { return n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1; }
+
+// A query's factor to and from f16's range: 1 unless its largest element
+// (times scale·log2 e) passes 2^15.
+__device__ __forceinline__ float query_down(float largest) {
+  if (!(largest > 32768.f) || !(largest <= 3.402823466e38f)) return 1.f;
+  return __int_as_float((127 + 14 - ((__float_as_int(largest) >> 23) - 127)) << 23);
 }
 
-template <uint32_t FORMAT, uint32_t HD>
-__global__ __launch_bounds__(64) void k_attn_paged(KvGeometry g, const KvSeq *__restrict__ seqs, uint32_t n_seqs,
-                                                   const float *__restrict__ q, uint32_t q_stride, float *__restrict__ out,
-                                                   uint32_t out_stride, uint32_t n_heads, float scale) {
-  constexpr uint32_t BYTES = kv_block_bytes(FORMAT, HD), SIZE = kv_elem_bytes(FORMAT), PART = kKvBlock * HD * SIZE;
-  __shared__ float q_s[HD], p_s[64];
-  const uint32_t row = blockIdx.x, head = blockIdx.y, kv = head / (n_heads / g.n_kv), lane = threadIdx.x;
-  uint32_t lo = 0, hi = n_seqs;  // the last sequence whose rows begin at or before this one (and that has rows)
-  while (hi - lo > 1) {
-    const uint32_t mid = (lo + hi) / 2;
-    if (seqs[mid].row <= row) lo = mid; else hi = mid;
+struct AttnOut {
+  float *out;       // batch rows
+  uint32_t stride;
+  float *partials;  // records of hd + 4 floats: O, the reference m, l
+};
+
+// One record or output quad: elements d .. d + 3 of a row with O, m and l.
+template <uint32_t HD>
+__device__ __forceinline__ void put_row(const AttnOut &o, uint32_t part, uint32_t record, uint64_t row, uint32_t head, uint32_t d,
+                                        float4 acc, float m, float l) {
+  if (part == ~0u) {
+    const float inv = 1.f / l;
+    *reinterpret_cast<float4 *>(o.out + row * o.stride + (uint64_t)head * HD + d) =
+        float4{acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+  } else {
+    float *p = o.partials + ((uint64_t)part + record) * (HD + 4);
+    *reinterpret_cast<float4 *>(p + d) = acc;
+    if (d == 0) p[HD] = m, p[HD + 1] = l;
   }
-  const KvSeq seq = seqs[lo];
-  const uint32_t n_keys = seq.past + (row - seq.row) + 1;
-  for (uint32_t d = lane; d < HD; d += 64) q_s[d] = q[(uint64_t)row * q_stride + head * HD + d] * scale;
-  float m = -INFINITY, l = 0.f, o[HD / 64];
-  for (uint32_t j = 0; j < HD / 64; j++) o[j] = 0.f;
-  __syncthreads();
-  for (uint32_t t0 = 0; t0 < n_keys; t0 += 64) {
-    const uint32_t key = t0 + lane, len = min(64u, n_keys - t0);
-    float s = -INFINITY;
-    if (lane < len) {
-      const uint8_t *block = g.block<BYTES>(seq.table, key / kKvBlock, kv);
-      s = 0.f;
-      for (uint32_t d = 0; d < HD; d++) s = fmaf(q_s[d], paged_float<FORMAT>(block + kv_key_at<FORMAT>(key % kKvBlock, d) * SIZE), s);
-      if constexpr (FORMAT != BCH_KV_F16) s *= reinterpret_cast<const float *>(block + 2 * PART)[key % kKvBlock];
+}
+
+// --- at most 16 packed rows ---------------------------------------------------
+
+// ROWS 8: the high parts of the queries and probabilities are the operands'
+// columns 0..7, the low parts columns 8..15, so one MFMA does both and the
+// halves of O are added once at the end.  ROWS 16: two MFMAs each.
+template <uint32_t FORMAT, uint32_t HD, uint32_t ROWS>
+__global__ __launch_bounds__(256) void k_attn_tokens(KvGeometry g, const KvAttnItem *__restrict__ items,
+                                                     const float *__restrict__ q, uint32_t q_stride, AttnOut to,
+                                                     uint32_t group, float c2) {
+  constexpr bool PACK = ROWS == 8, QUANT = FORMAT != BCH_KV_F16;
+  constexpr uint32_t SIZE = kv_elem_bytes(FORMAT), BYTES = kv_block_bytes(FORMAT, HD), PART = kKvBlock * HD * SIZE;
+  constexpr uint32_t NL = PART / 1024;  // KB of a block's keys, and of its values
+  constexpr uint32_t KS = HD / 32, OB = HD / 16, M = 4 / SIZE;
+  __shared__ __align__(16) float o_s[4][ROWS][HD];
+  __shared__ float m_s[4][ROWS], l_s[4][ROWS];
+  const uint32_t kv = blockIdx.x % g.n_kv;
+  const KvAttnItem it = items[blockIdx.x / g.n_kv];
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+  const uint32_t col = lane % 16, quad = lane / 16;
+  const uint32_t r = PACK ? col % 8 : col, packed = it.first + min(r, it.rows - 1);
+  const uint32_t token = packed / group, head = kv * group + packed % group, pos = it.past + token;
+  const uint32_t pos0 = it.past + it.first / group;                             // of the tile's first row
+  const uint32_t n_keys = it.past + (it.first + it.rows - 1) / group + 1;       // of its last
+  const uint32_t last = (n_keys - 1) / kKvBlock;
+
+  struct Raw {
+    au4_t x[2][NL];
+    float4 s[2];
+  } kr, vr;
+  auto block = [&](uint32_t step, int t) {
+    return g.block<BYTES>(it.table, min(2 * step + t, last), kv);  // (past the end: the last block, masked)
+  };
+  auto load = [&](Raw &raw, uint32_t step, uint32_t part) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+      const uint8_t *p = block(step, t);
+#pragma unroll
+      for (uint32_t c = 0; c < NL; c++)
+        raw.x[t][c] = *reinterpret_cast<const au4_t *>(p + part * PART + 1024 * c + 16 * lane);
+      if constexpr (QUANT) raw.s[t] = *reinterpret_cast<const float4 *>(p + 2 * PART + 64 * part + 16 * quad);
     }
-    // (A NaN score passes the maximum by and makes the sum NaN.)
-    const float m_new = fmaxf(m, wave_max(s)), m_use = m_new == -INFINITY ? 0.f : m_new;
-    const float p = lane < len ? expf(s - m_use) : 0.f;
-    const float corr = expf(m - m_use);
-    l = l * corr + wave_sum(p);
-    m = m_new;
-    __syncthreads();
-    p_s[lane] = p;
-    __syncthreads();
-    for (uint32_t j = 0; j < HD / 64; j++) {
-      const uint32_t d = lane + 64 * j;
-      float a = o[j] * corr;
-      for (uint32_t i = 0; i < len; i++) {
-        const uint8_t *block = g.block<BYTES>(seq.table, (t0 + i) / kKvBlock, kv);
-        float x = paged_float<FORMAT>(block + PART + kv_value_at<FORMAT>((t0 + i) % kKvBlock, d) * SIZE);
-        if constexpr (FORMAT != BCH_KV_F16) x *= reinterpret_cast<const float *>(block + 2 * PART)[kKvBlock + (t0 + i) % kKvBlock];
-        a = fmaf(p_s[i], x, a);
+  };
+  uint32_t step = it.lo + wave;
+  const bool any = step < it.hi;
+  if (any) {
+    load(kr, step, 0);
+    load(vr, step, 1);
+  }
+
+  // The row's elements as the keys' operand has them: k-step s of the MFMA
+  // takes elements 32s + 8·quad .. + 8 (f16), or of 16-byte pieces of 8-bit
+  // elements the first and then the second halves.
+  ah8_t qh[KS], ql[PACK ? 1 : KS];
+  float back = 1.f;
+  {
+    const float *qr = q + (uint64_t)(it.row + token) * q_stride + (uint64_t)head * HD;
+    float x[KS][8], largest = 0.f;
+#pragma unroll
+    for (uint32_t s = 0; s < KS; s++) {
+      const uint32_t e = QUANT ? 64 * (s / 2) + 16 * quad + 8 * (s % 2) : 32 * s + 8 * quad;
+      const float4 a = *reinterpret_cast<const float4 *>(qr + e), b = *reinterpret_cast<const float4 *>(qr + e + 4);
+      const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        x[s][j] = v[j] * c2;
+        largest = fmaxf(largest, fabsf(x[s][j]));
       }
-      o[j] = a;
+    }
+    largest = fmaxf(largest, __shfl_xor(largest, 16, 64));
+    largest = fmaxf(largest, __shfl_xor(largest, 32, 64));
+    const float down = query_down(largest);
+    back = 1.f / down;
+#pragma unroll
+    for (uint32_t s = 0; s < KS; s++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float v = x[s][j] * down;
+        const _Float16 hi = (_Float16)v, lo = (_Float16)(v - (float)hi);
+        if constexpr (PACK) {
+          qh[s][j] = col < 8 ? hi : lo;
+        } else {
+          qh[s][j] = hi;
+          ql[s][j] = lo;
+        }
+      }
+  }
+  const bool far = __builtin_amdgcn_ballot_w64(back != 1.f) != 0;
+  const float low = col < 8 ? 0.f : 1.f;  // PACK: this lane's columns carry the low parts
+
+  af4_t o[OB];
+#pragma unroll
+  for (uint32_t b = 0; b < OB; b++) o[b] = af4_t{0.f, 0.f, 0.f, 0.f};
+  float m = 0.f, l = 0.f, lazy = kUnset;
+
+  for (; step < it.hi; step += 4) {
+    const uint32_t next = min(step + 4, it.hi - 1);
+    // Scores of the tile's 2 x 16 keys: this lane's are 16t + 4·quad + i.
+    float u[2][4];
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+      af4_t s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (uint32_t k = 0; k < KS; k++) {
+        ah8_t a;
+        if constexpr (QUANT)
+          a = join(widen<FORMAT>(kr.x[t][k / 2][2 * (k % 2)]), widen<FORMAT>(kr.x[t][k / 2][2 * (k % 2) + 1]));
+        else
+          a = __builtin_bit_cast(ah8_t, kr.x[t][k]);
+        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[k], s, 0, 0, 0);
+        if constexpr (!PACK) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[k], s, 0, 0, 0);
+      }
+      const float ks[4] = {kr.s[t].x, kr.s[t].y, kr.s[t].z, kr.s[t].w};
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        float x = s[i];
+        if constexpr (PACK) x += dpp<kDppRor8>(x);
+        if (far) x *= back;
+        u[t][i] = QUANT ? fmaf(x, ks[i], -m) : x - m;
+      }
+    }
+    load(kr, next, 0);
+    float vs[2][4];
+    if constexpr (QUANT) {
+#pragma unroll
+      for (int t = 0; t < 2; t++) vs[t][0] = vr.s[t].x, vs[t][1] = vr.s[t].y, vs[t][2] = vr.s[t].z, vs[t][3] = vr.s[t].w;
+    }
+    const bool masked = 32 * step + 31 > pos0;
+    if (masked) {
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const bool seen = 32 * step + 16 * t + 4 * quad + i <= pos;
+          u[t][i] = seen ? u[t][i] : -INFINITY;
+          if constexpr (QUANT) vs[t][i] = seen ? vs[t][i] : 0.f;
+        }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) top = fmaxf(top, QUANT ? u[t][i] + scale_log(vs[t][i]) : u[t][i]);
+    if constexpr (QUANT) top -= 127.f;
+    if (__builtin_amdgcn_ballot_w64(top > lazy)) {
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const bool move = top > lazy;  // the same in the four lanes of a row
+      const float d = move ? top : 0.f, corr = !move || lazy == kUnset ? 1.f : __builtin_amdgcn_exp2f(-d);
+      m += d;
+      l *= corr;
+      lazy = move ? kLazy : lazy;
+#pragma unroll
+      for (uint32_t b = 0; b < OB; b++) o[b] *= corr;
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) u[t][i] -= d;
+    }
+    ah8_t ph, pl;
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float p = __builtin_amdgcn_exp2f(u[t][i]);
+        l += p;
+        const float pv = QUANT ? p * vs[t][i] : p;
+        const _Float16 hi = (_Float16)pv;
+        if constexpr (PACK) {
+          ph[4 * t + i] = (_Float16)fmaf(-(float)hi, low, pv);
+        } else {
+          ph[4 * t + i] = hi;
+          pl[4 * t + i] = (_Float16)(pv - (float)hi);
+        }
+      }
+    if constexpr (FORMAT == BCH_KV_F8) {
+      // Bytes behind the last key may be NaN.  (Those of stored rows never are.)
+      if (32 * step + 31 >= n_keys) {
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+          const uint32_t keep = bytes_below((int)(n_keys - (32 * step + 16 * t + 4 * quad)));
+#pragma unroll
+          for (uint32_t c = 0; c < NL; c++) vr.x[t][c] &= keep;
+        }
+      }
+    }
+    // O^T += V^T·P^T: the lane's k-indices are the same 2 x 4 keys, of element
+    // 16·b + lane % 16.
+#pragma unroll
+    for (uint32_t b = 0; b < OB; b++) {
+      const uint32_t c = b / M, x = b % M;
+      ah8_t a;
+      if constexpr (QUANT)
+        a = join(widen<FORMAT>(vr.x[0][c][x]), widen<FORMAT>(vr.x[1][c][x]));
+      else
+        a = join(halves(vr.x[0][c][2 * x], vr.x[0][c][2 * x + 1]), halves(vr.x[1][c][2 * x], vr.x[1][c][2 * x + 1]));
+      if constexpr (!QUANT) {
+        // f16 values may be infinite or NaN, and 0 times those is NaN: what no
+        // row of the tile sees becomes 0, and what some see and others do not
+        // makes NaN of the former's element below.
+        if (masked) {
+          bool odd = false;
+#pragma unroll
+          for (int j = 0; j < 8; j++) {
+            if (32 * step + 16 * (j / 4) + 4 * quad + j % 4 >= n_keys) a[j] = (_Float16)0.f;
+            odd |= not_finite(a[j]);
+          }
+          if (__builtin_amdgcn_ballot_w64(odd)) {
+            ah8_t seen, bad;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+              seen[j] = (_Float16)(32 * step + 16 * (j / 4) + 4 * quad + j % 4 <= pos ? 1.f : 0.f);
+              bad[j] = (_Float16)(not_finite(a[j]) ? 1.f : 0.f);
+              a[j] = not_finite(a[j]) ? (_Float16)0.f : a[j];
+            }
+            const af4_t count = __builtin_amdgcn_mfma_f32_16x16x32_f16(bad, seen, af4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[b][i] = count[i] > 0.f ? NAN : o[b][i];
+          }
+        }
+      }
+      o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph, o[b], 0, 0, 0);
+      if constexpr (!PACK) o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl, o[b], 0, 0, 0);
+    }
+    load(vr, next, 1);
+  }
+
+  // Join the waves.
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  if (quad == 0 && col < ROWS) {
+    m_s[wave][col] = lazy == kUnset ? -INFINITY : m;
+    l_s[wave][col] = l;
+  }
+#pragma unroll
+  for (uint32_t b = 0; b < OB; b++) {
+    if constexpr (PACK) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) o[b][i] += dpp<kDppRor8>(o[b][i]);
+    }
+    if (col < ROWS) *reinterpret_cast<af4_t *>(&o_s[wave][col][16 * b + 4 * quad]) = o[b];
+  }
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < it.rows * (HD / 4); i += 256) {
+    const uint32_t row = i / (HD / 4), d = 4 * (i % (HD / 4));
+    const float top = fmaxf(fmaxf(m_s[0][row], m_s[1][row]), fmaxf(m_s[2][row], m_s[3][row]));
+    float4 acc = {0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      const float f = m_s[w][row] == top ? 1.f : __builtin_amdgcn_exp2f(m_s[w][row] - top);
+      const float4 x = *reinterpret_cast<const float4 *>(&o_s[w][row][d]);
+      acc.x = fmaf(x.x, f, acc.x), acc.y = fmaf(x.y, f, acc.y), acc.z = fmaf(x.z, f, acc.z), acc.w = fmaf(x.w, f, acc.w);
+      sum = fmaf(l_s[w][row], f, sum);
+    }
+    const uint32_t at = it.first + row;
+    put_row<HD>(to, it.part, kv * it.rows + row, it.row + at / group, kv * group + at % group, d, acc, top, sum);
+  }
+}
+
+// --- more rows ------------------------------------------------------------------
+
+template <uint32_t HD>
+constexpr uint32_t kChunkKeys = HD == 256 ? 32 : 64;  // keys of a step
+constexpr uint32_t kChunkRows = 128;
+
+template <uint32_t FORMAT, uint32_t HD>
+__global__ __launch_bounds__(256, HD == 64 ? 3 : HD == 128 ? 2 : 1) void k_attn_chunk(
+    KvGeometry g, const KvAttnItem *__restrict__ items, const float *__restrict__ q, uint32_t q_stride, AttnOut to,
+    uint32_t group, float c2) {
+  constexpr bool QUANT = FORMAT != BCH_KV_F16;
+  constexpr uint32_t SIZE = kv_elem_bytes(FORMAT), BYTES = kv_block_bytes(FORMAT, HD), PART = kKvBlock * HD * SIZE;
+  constexpr uint32_t KEYS = kChunkKeys<HD>, TILES = KEYS / 32, KS = HD / 16, OB = HD / 32, M = 4 / SIZE;
+  constexpr uint32_t PIECES = HD * SIZE;              // 16-byte pieces of a block's keys, and of its values
+  constexpr uint32_t NP = KEYS / 16 * PIECES / 256;   // of each per thread and step
+  // Keys: 8 elements of key k at slot (element / 8)·KEYS + k.  Values: the keys
+  // {0..3, 8..11} + 4h of 16 keys of element d at slot (2·(key / 16) + h)·HD + d.
+  __shared__ __align__(16) _Float16 k_s[2][KEYS * HD], v_s[2][KEYS * HD];
+  __shared__ __align__(16) float ks_s[2][KEYS], vs_s[2][KEYS];
+  __shared__ float top_s[2];
+  __shared__ uint32_t odd_s[2];
+  const uint32_t kv = blockIdx.x % g.n_kv;
+  const KvAttnItem it = items[blockIdx.x / g.n_kv];
+  const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
+  const uint32_t col = lane % 32, half_id = lane / 32;
+  const bool active = 32 * wave < it.rows;
+  const uint32_t row0 = it.first + (active ? 32 * wave : 0);
+  const uint32_t rows = active ? min(32u, it.rows - 32 * wave) : 1;
+  const uint32_t packed = row0 + min(col, rows - 1);
+  const uint32_t token = packed / group, head = kv * group + packed % group, pos = it.past + token;
+  const uint32_t pos0 = it.past + row0 / group;                          // of the wave's first row
+  const uint32_t kend = it.past + (row0 + rows - 1) / group + 1;         // keys of the wave's last row
+  const uint32_t wg_pos0 = it.past + it.first / group;
+  const uint32_t wg_kend = it.past + (it.first + it.rows - 1) / group + 1;
+  const uint32_t last = (wg_kend - 1) / kKvBlock;
+  const uint32_t lo = it.lo * 32, hi = min(it.hi * 32, wg_kend);         // keys of this split
+
+  au4_t kr[NP], vr[NP];
+  float sk = 0.f, sv = 0.f;
+  // Lanes of a value piece: quads of keys in the order 0, 2, 1, 3, so that the
+  // two quads whose halves of a slot interleave are written together.
+  const uint32_t swapped = (lane & 15) | (lane & 16) << 1 | (lane & 32) >> 1;
+  auto load = [&](uint32_t kb) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t p = 0; p < NP; p++) {
+      const uint32_t at = 64 * wave + 256 * p, j = at / PIECES, within = at % PIECES;
+      const uint8_t *b = g.block<BYTES>(it.table, min(kb / kKvBlock + j, last), kv);
+      kr[p] = *reinterpret_cast<const au4_t *>(b + 16 * (within + lane));
+      vr[p] = *reinterpret_cast<const au4_t *>(b + PART + 16 * (within + swapped));
+    }
+    if constexpr (QUANT) {
+      if (tid < KEYS) {
+        const uint8_t *b = g.block<BYTES>(it.table, min(kb / kKvBlock + tid / kKvBlock, last), kv) + 2 * PART;
+        sk = reinterpret_cast<const float *>(b)[tid % kKvBlock];
+        sv = reinterpret_cast<const float *>(b)[kKvBlock + tid % kKvBlock];
+      }
+    }
+  };
+  auto stage = [&](int buf, uint32_t kb) __attribute__((always_inline)) {
+    bool odd = false;
+#pragma unroll
+    for (uint32_t p = 0; p < NP; p++) {
+      const uint32_t at = 64 * wave + 256 * p, j = at / PIECES, within = at % PIECES;
+      const uint32_t piece = (within + lane) / 16, key = 16 * j + lane % 16;
+      if constexpr (QUANT) {
+        *reinterpret_cast<ah8_t *>(&k_s[buf][(2 * piece * KEYS + key) * 8]) = join(widen<FORMAT>(kr[p][0]), widen<FORMAT>(kr[p][1]));
+        *reinterpret_cast<ah8_t *>(&k_s[buf][((2 * piece + 1) * KEYS + key) * 8]) = join(widen<FORMAT>(kr[p][2]), widen<FORMAT>(kr[p][3]));
+      } else {
+        *reinterpret_cast<au4_t *>(&k_s[buf][(piece * KEYS + key) * 8]) = kr[p];
+      }
+      const uint32_t v = within + swapped, quad = v / 16 % 4;
+      // Bytes behind the last key may be NaN.  (Those of stored rows never are.)
+      if constexpr (FORMAT == BCH_KV_F8) {
+        if (kb + KEYS > wg_kend) vr[p] &= bytes_below((int)(wg_kend - (kb + 16 * j + 4 * quad)));
+      }
+#pragma unroll
+      for (uint32_t x = 0; x < M; x++) {
+        const uint32_t d = v / 64 * 16 * M + 16 * x + v % 16;
+        ah4_t a;
+        if constexpr (QUANT)
+          a = widen<FORMAT>(vr[p][x]);
+        else
+          a = halves(vr[p][2 * x], vr[p][2 * x + 1]);
+        if constexpr (!QUANT) {
+          if (kb + KEYS - 1 > wg_pos0) {
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+              if (kb + 16 * j + 4 * quad + i >= wg_kend) a[i] = (_Float16)0.f;
+              odd |= not_finite(a[i]);
+            }
+          }
+        }
+        *reinterpret_cast<ah4_t *>(&v_s[buf][((2 * j + quad % 2) * HD + d) * 8 + quad / 2 * 4]) = a;
+      }
+    }
+    if constexpr (QUANT) {
+      if (wave == 0) {
+        const float b = lane < KEYS && kb + lane < wg_kend ? sv : 0.f;
+        if (lane < KEYS) ks_s[buf][lane] = sk, vs_s[buf][lane] = b;
+        const float top = wave_max(b == b ? scale_log(b) : 0.f);
+        if (lane == 0) top_s[buf] = top - 127.f;
+      }
+    } else if (kb + KEYS - 1 > wg_pos0) {
+      if (__builtin_amdgcn_ballot_w64(odd) && lane == 0) odd_s[buf] = 1;  // (cleared after each masked step)
+    }
+  };
+  if (tid < 2) odd_s[tid] = 0;
+  if (lo < hi) load(lo);
+
+  ah8_t qh[KS], ql[KS];
+  float back = 1.f;
+  {
+    const float *qr = q + (uint64_t)(it.row + token) * q_stride + (uint64_t)head * HD + 8 * half_id;
+    float largest = 0.f;
+#pragma unroll
+    for (uint32_t s = 0; s < KS; s++) {
+      const float4 a = *reinterpret_cast<const float4 *>(qr + 16 * s), b = *reinterpret_cast<const float4 *>(qr + 16 * s + 4);
+      const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int j = 0; j < 8; j++) largest = fmaxf(largest, fabsf(v[j] * c2));
+    }
+    largest = fmaxf(largest, __shfl_xor(largest, 32, 64));
+    const float down = query_down(largest);
+    back = 1.f / down;
+#pragma unroll
+    for (uint32_t s = 0; s < KS; s++) {
+      const float4 a = *reinterpret_cast<const float4 *>(qr + 16 * s), b = *reinterpret_cast<const float4 *>(qr + 16 * s + 4);
+      const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float x = v[j] * c2 * down;
+        qh[s][j] = (_Float16)x;
+        ql[s][j] = (_Float16)(x - (float)qh[s][j]);
+      }
     }
   }
-  for (uint32_t j = 0; j < HD / 64; j++) out[(uint64_t)row * out_stride + head * HD + lane + 64 * j] = o[j] / l;
+  const bool far = __builtin_amdgcn_ballot_w64(back != 1.f) != 0;
+  af16_t o[OB];
+#pragma unroll
+  for (uint32_t b = 0; b < OB; b++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) o[b][i] = 0.f;
+  float m = 0.f, l = 0.f, lazy = kUnset;
+
+  // One step of KEYS keys; score r of tile t is of key kb + 32t + 8·(r / 4) +
+  // 4·half + r % 4.
+  auto step = [&](uint32_t kb, int buf, auto is_masked) __attribute__((always_inline)) {
+    constexpr bool masked = decltype(is_masked)::value;
+    af16_t u[TILES];
+    float vs[TILES][16];
+#pragma unroll
+    for (uint32_t t = 0; t < TILES; t++) {
+#pragma unroll
+      for (int i = 0; i < 16; i++) u[t][i] = 0.f;
+#pragma unroll
+      for (uint32_t s = 0; s < KS; s++) {
+        const ah8_t a = *reinterpret_cast<const ah8_t *>(&k_s[buf][((2 * s + half_id) * KEYS + 32 * t + col) * 8]);
+        u[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[s], u[t], 0, 0, 0);
+        u[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[s], u[t], 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (uint32_t t = 0; t < TILES; t++)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; q4++) {
+        float4 a, b;
+        if constexpr (QUANT) {
+          a = *reinterpret_cast<const float4 *>(&ks_s[buf][32 * t + 8 * q4 + 4 * half_id]);
+          b = *reinterpret_cast<const float4 *>(&vs_s[buf][32 * t + 8 * q4 + 4 * half_id]);
+        }
+        const float as[4] = {a.x, a.y, a.z, a.w}, bs[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int r = 4 * q4 + i;
+          float x = u[t][r];
+          if (far) x *= back;
+          u[t][r] = QUANT ? fmaf(x, as[i], -m) : x - m;
+          vs[t][r] = QUANT ? bs[i] : 1.f;
+          if constexpr (masked) {
+            const bool seen = kb + 32 * t + 8 * q4 + 4 * half_id + i <= pos;
+            u[t][r] = seen ? u[t][r] : -INFINITY;
+            vs[t][r] = seen ? vs[t][r] : 0.f;
+          }
+        }
+      }
+    // The largest u + log2 b: key by key where some are not seen (those must
+    // change nothing), else from the largest of both.
+    float top = -INFINITY;
+#pragma unroll
+    for (uint32_t t = 0; t < TILES; t++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) top = fmaxf(top, QUANT && masked ? u[t][r] + scale_log(vs[t][r]) : u[t][r]);
+    if constexpr (QUANT) top += masked ? -127.f : top_s[buf];
+    if (__builtin_amdgcn_ballot_w64(top > lazy)) {
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const bool move = top > lazy;  // the same in both lanes of a row
+      const float d = move ? top : 0.f, corr = !move || lazy == kUnset ? 1.f : __builtin_amdgcn_exp2f(-d);
+      m += d;
+      l *= corr;
+      lazy = move ? kLazy : lazy;
+#pragma unroll
+      for (uint32_t b = 0; b < OB; b++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[b][i] *= corr;
+#pragma unroll
+      for (uint32_t t = 0; t < TILES; t++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) u[t][r] -= d;
+    }
+#pragma unroll
+    for (uint32_t t = 0; t < TILES; t++) {
+      ah8_t ph[2], pl[2];
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(u[t][r]), p1 = __builtin_amdgcn_exp2f(u[t][r + 1]);
+        l += p0 + p1;
+        const af2_t pv = {QUANT ? p0 * vs[t][r] : p0, QUANT ? p1 * vs[t][r + 1] : p1};
+        const ah2_t h = __builtin_convertvector(pv, ah2_t);
+        const af2_t rest = {pv[0] - (float)h[0], pv[1] - (float)h[1]};
+        const ah2_t e = __builtin_convertvector(rest, ah2_t);
+        ph[r / 8][r % 8] = h[0], ph[r / 8][r % 8 + 1] = h[1];
+        pl[r / 8][r % 8] = e[0], pl[r / 8][r % 8 + 1] = e[1];
+      }
+#pragma unroll
+      for (int j = 0; j < 2; j++)
+#pragma unroll
+        for (uint32_t b = 0; b < OB; b++) {
+          ah8_t a = *reinterpret_cast<const ah8_t *>(&v_s[buf][((2 * (2 * t + j) + half_id) * HD + 32 * b + col) * 8]);
+          if constexpr (masked && !QUANT) {
+            // 0 times a value that is not finite is NaN: rows that see such a
+            // value get it from a count, and the product leaves it out.
+            if (odd_s[buf]) {
+              ah8_t seen, bad;
+              af16_t count;
+#pragma unroll
+              for (int i = 0; i < 16; i++) count[i] = 0.f;
+#pragma unroll
+              for (int i = 0; i < 8; i++) {
+                seen[i] = (_Float16)(kb + 32 * t + 16 * j + 4 * half_id + (i & 4) * 2 + (i & 3) <= pos ? 1.f : 0.f);
+                bad[i] = (_Float16)(not_finite(a[i]) ? 1.f : 0.f);
+                a[i] = not_finite(a[i]) ? (_Float16)0.f : a[i];
+              }
+              count = __builtin_amdgcn_mfma_f32_32x32x16_f16(bad, seen, count, 0, 0, 0);
+#pragma unroll
+              for (int i = 0; i < 16; i++) o[b][i] = count[i] > 0.f ? NAN : o[b][i];
+            }
+          }
+          o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[j], o[b], 0, 0, 0);
+          o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[j], o[b], 0, 0, 0);
+        }
+    }
+  };
+  if (lo < hi) {
+    __syncthreads();  // odd_s is clear
+    stage(0, lo);
+    load(min(lo + KEYS, hi - 1) / KEYS * KEYS);
+    lds_barrier();
+    int buf = 0;
+    for (uint32_t kb = lo; kb < hi; kb += KEYS, buf ^= 1) {
+      // The other buffer was read before the last barrier.
+      if (kb + KEYS < hi) {
+        stage(buf ^ 1, kb + KEYS);
+        load(min(kb + 2 * KEYS, hi - 1) / KEYS * KEYS);
+      }
+      if (active && kb < kend) {
+        if (kb + KEYS - 1 > pos0)
+          step(kb, buf, std::true_type{});
+        else
+          step(kb, buf, std::false_type{});
+      }
+      lds_barrier();
+      if constexpr (!QUANT) {
+        if (kb + KEYS - 1 > wg_pos0) {
+          if (tid == 0) odd_s[buf] = 0;
+          lds_barrier();
+        }
+      }
+    }
+  }
+  if (!active) return;
+  l += __shfl_xor(l, 32, 64);
+  if (col >= rows) return;
+  const float ref = lazy == kUnset ? -INFINITY : m;
+#pragma unroll
+  for (uint32_t b = 0; b < OB; b++)
+#pragma unroll
+    for (int q4 = 0; q4 < 4; q4++)
+      put_row<HD>(to, it.part, kv * it.rows + (packed - it.first), it.row + token, head, 32 * b + 8 * q4 + 4 * half_id,
+                  float4{o[b][4 * q4], o[b][4 * q4 + 1], o[b][4 * q4 + 2], o[b][4 * q4 + 3]}, ref, l);
+}
+
+// The rows of tiles whose keys were split, from the splits' records.
+template <uint32_t HD>
+__global__ __launch_bounds__(256) void k_attn_join(const KvJoinItem *__restrict__ items, uint32_t n_kv, uint32_t group, AttnOut to) {
+  const KvJoinItem it = items[blockIdx.x];
+  const uint32_t kv = blockIdx.y, i = blockIdx.z * 256 + threadIdx.x, row = i / (HD / 4), d = 4 * (i % (HD / 4));
+  if (row >= it.rows) return;
+  const uint64_t apart = (uint64_t)n_kv * it.rows * (HD + 4);
+  const float *p = to.partials + ((uint64_t)it.part + kv * it.rows + row) * (HD + 4);
+  float top = -INFINITY, sum = 0.f;
+  for (uint32_t s = 0; s < it.splits; s++) top = fmaxf(top, p[s * apart + HD]);
+  float4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (uint32_t s = 0; s < it.splits; s++) {
+    const float m = p[s * apart + HD], f = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
+    const float4 x = *reinterpret_cast<const float4 *>(p + s * apart + d);
+    acc.x = fmaf(x.x, f, acc.x), acc.y = fmaf(x.y, f, acc.y), acc.z = fmaf(x.z, f, acc.z), acc.w = fmaf(x.w, f, acc.w);
+    sum = fmaf(p[s * apart + HD + 1], f, sum);
+  }
+  const uint32_t at = it.first + row;
+  put_row<HD>(to, ~0u, 0, it.row + at / group, kv * group + at % group, d, acc, top, sum);
+}
+
+// --- the work of a batch ----------------------------------------------------------
+
+// Splits: a workgroup takes about `share` steps of 32 keys, so that the batch's
+// keys make kTargetGroups workgroups for each CU, and no fewer steps than cost
+// what joining a split costs.
+static void split_tile(KvSchedule &w, std::vector<KvAttnItem> &items, KvAttnItem it, uint32_t steps, uint32_t share,
+                       uint32_t n_kv, uint32_t granule, uint64_t records) {
+  uint32_t splits = (steps + share - 1) / share;
+  if (splits > 1 && w.records + (uint64_t)splits * n_kv * it.rows > records) splits = 1;
+  if (splits > 1) w.join.push_back({it.row, it.first, it.rows, splits, (uint32_t)w.records});
+  const uint32_t units = (steps + granule - 1) / granule;
+  for (uint32_t s = 0; s < splits; s++) {
+    it.lo = (uint32_t)((uint64_t)units * s / splits) * granule;
+    it.hi = std::min((uint32_t)((uint64_t)units * (s + 1) / splits) * granule, steps);
+    it.part = splits > 1 ? (uint32_t)w.records : ~0u;
+    if (splits > 1) w.records += (uint64_t)n_kv * it.rows;
+    items.push_back(it);
+  }
+}
+
+KvSchedule kv_schedule(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t n_kv, uint32_t head_dim, uint32_t n_cus,
+                       uint64_t partial_floats) {
+  KvSchedule w;
+  const uint64_t records = std::min<uint64_t>(partial_floats / (head_dim + 4), 0xfffffffeu);
+  constexpr uint32_t kTokenGroups = 4, kTokenMin = 8, kChunkGroups = 3, kChunkMin = 8;
+  if (!n_cus) n_cus = 256;
+  uint64_t token_steps = 0, chunk_steps = 0;
+  auto tiles = [&](const KvSeq &q, auto &&f) {
+    const uint32_t rows = q.n_new * group, wide = rows <= 16 ? 16 : kChunkRows;
+    for (uint32_t first = 0; first < rows; first += wide) {
+      const uint32_t n = std::min(wide, rows - first), keys = q.past + (first + n - 1) / group + 1;
+      f(first, n, (keys + 31) / 32, rows <= 16);
+    }
+  };
+  for (const KvSeq &q : seqs)
+    tiles(q, [&](uint32_t, uint32_t, uint32_t steps, bool few) { (few ? token_steps : chunk_steps) += steps; });
+  auto share = [&](uint64_t steps, uint32_t groups, uint32_t least) {
+    const uint64_t want = (uint64_t)n_cus * groups;
+    return (uint32_t)std::max<uint64_t>((steps * n_kv + want - 1) / want, least);
+  };
+  const uint32_t token_share = share(token_steps, kTokenGroups, kTokenMin);
+  const uint32_t chunk_share = share(chunk_steps, kChunkGroups, kChunkMin);
+  for (const KvSeq &q : seqs)
+    tiles(q, [&](uint32_t first, uint32_t n, uint32_t steps, bool few) {
+      KvAttnItem it{q.table, q.past, q.row, first, n, 0, 0, ~0u};
+      if (few)
+        split_tile(w, n <= 8 ? w.narrow : w.tokens, it, steps, token_share, n_kv, 4, records);
+      else
+        split_tile(w, w.chunks, it, steps, chunk_share, n_kv, head_dim == 256 ? 1 : 2, records);
+    });
+  // The longest first, so that the last workgroups are short ones.
+  auto longer = [](const KvAttnItem &a, const KvAttnItem &b) { return a.hi - a.lo > b.hi - b.lo; };
+  for (auto *items : {&w.narrow, &w.tokens, &w.chunks}) std::stable_sort(items->begin(), items->end(), longer);
+  return w;
 }
 
 }  // namespace bch
@@ -97,10 +754,20 @@ extern "C" int bch_attention_paged(bch_ctx *ctx, const bch_kv_plan *plan, bch_vi
   }
   return launch(ctx, {"attention_paged", plan->n_tokens, width, 0}, [&](hipStream_t st) {
     if (!plan->n_tokens) return;
+    const KvGeometry geo = plan->geometry(cp);
+    const AttnOut to{op, out_stride, ctx->attn_partials};
+    const uint32_t n_kv = s.n_kv_heads, group = plan->n_heads / n_kv;
+    const float c2 = (float)(1.44269504088896340736 / std::sqrt((double)s.head_dim));
     kv_dispatch(s.format, s.head_dim, [&](auto format, auto hd) {
-      k_attn_paged<decltype(format)::value, decltype(hd)::value><<<dim3(plan->n_tokens, plan->n_heads), 64, 0, st>>>(
-          plan->geometry(cp), plan->d_seqs, plan->n_seqs, qp, q_stride, op, out_stride, plan->n_heads,
-          1.0f / sqrtf((float)s.head_dim));
+      constexpr uint32_t F = decltype(format)::value, HD = decltype(hd)::value;
+      if (plan->n_chunks) k_attn_chunk<F, HD><<<plan->n_chunks * n_kv, 256, 0, st>>>(geo, plan->d_chunks, qp, q_stride, to, group, c2);
+      if (plan->n_tiles16)
+        k_attn_tokens<F, HD, 16><<<plan->n_tiles16 * n_kv, 256, 0, st>>>(geo, plan->d_tiles16, qp, q_stride, to, group, c2);
+      if (plan->n_tiles8)
+        k_attn_tokens<F, HD, 8><<<plan->n_tiles8 * n_kv, 256, 0, st>>>(geo, plan->d_tiles8, qp, q_stride, to, group, c2);
+      if (plan->n_join)
+        k_attn_join<HD><<<dim3(plan->n_join, n_kv, div_ceil(plan->join_rows * (HD / 4), 256)), 256, 0, st>>>(
+            plan->d_join, n_kv, group, to);
     });
   });
 }

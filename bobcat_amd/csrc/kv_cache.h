@@ -76,6 +76,28 @@ struct KvStoreItem {
   uint32_t page, block, row;
   uint16_t lo, n;
 };
+// A tile of packed rows (row = token·group + head of the group) of a sequence
+// and a part of its keys.
+struct KvAttnItem {
+  uint32_t table, past, row;  // of the sequence (KvSeq)
+  uint32_t first, rows;       // packed rows first .. first + rows
+  uint32_t lo, hi;            // steps of 32 keys
+  uint32_t part;              // the first of its n_kv·rows records, ~0: writes the outputs itself
+};
+// The tiles whose keys are split, with the first split's records.
+struct KvJoinItem {
+  uint32_t row, first, rows, splits, part;
+};
+struct KvSchedule {
+  std::vector<KvAttnItem> narrow, tokens, chunks;  // of at most 8, at most 16, and up to 128 rows
+  std::vector<KvJoinItem> join;
+  uint64_t records = 0;
+};
+// attn_paged.hip: the attention's work of a batch, with no more partial
+// results than partial_floats hold.
+KvSchedule kv_schedule(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t n_kv, uint32_t head_dim, uint32_t n_cus,
+                       uint64_t partial_floats);
+
 struct KvGeometry {
   uint8_t *cache;
   const uint32_t *pages;
@@ -98,15 +120,20 @@ struct bch_kv_plan {
   bch_kv_shape shape;
   uint32_t n_heads;
   bool ready = false;  // bch_kv_plan_set has succeeded
+  // The ticket of the last recording that used the plan (the open one's
+  // next): its launches read the plan's memory until it has been waited for.
+  mutable uint64_t last_use = 0;
   uint32_t n_seqs = 0, n_tokens = 0;
   std::vector<bch::KvSeq> seqs;
   // One device allocation with all of the below, grown on demand.
   uint8_t *memory = nullptr;
   uint64_t memory_bytes = 0;
-  const bch::KvSeq *d_seqs = nullptr;
   const uint32_t *d_pages = nullptr;
   const bch::KvStoreItem *d_store = nullptr;
   uint32_t n_store = 0;
+  const bch::KvAttnItem *d_tiles8 = nullptr, *d_tiles16 = nullptr, *d_chunks = nullptr;
+  const bch::KvJoinItem *d_join = nullptr;
+  uint32_t n_tiles8 = 0, n_tiles16 = 0, n_chunks = 0, n_join = 0, join_rows = 0;
 
   bch::KvGeometry geometry(void *cache) const {
     const uint32_t blocks = shape.page_size / bch::kKvBlock;
@@ -117,7 +144,7 @@ struct bch_kv_plan {
 
 namespace bch {
 // The plan of a recorded op: BCH_OK if it belongs to ctx, is ready, and the
-// view `cache` holds its pages, whose address goes to *ptr.
+// view `cache` holds its pages, whose address goes to *ptr; notes the use.
 int kv_plan_cache(bch_ctx *ctx, const char *kernel, const bch_kv_plan *plan, bch_view cache, void **ptr);
 // Rows of `width` floats, `stride` apart, one for each of the plan's tokens.
 int kv_plan_rows(bch_ctx *ctx, const char *kernel, const bch_kv_plan *plan, bch_view view, uint32_t width,

@@ -15,6 +15,7 @@
 namespace bch {
 
 constexpr uint32_t kKvMaxPositions = 0x7fffffffu;
+constexpr uint32_t kKvMaxTokens = 1u << 26;  // of a batch: packed rows and workgroups then stay below 2^31
 
 static int check_shape(const char *kernel, const bch_kv_shape *s) {
   if (!s) return fail(BCH_ERR_ARGUMENT, "%s: no shape", kernel);
@@ -51,7 +52,7 @@ static int check_batch(const char *kernel, const bch_kv_shape *s, uint32_t n_seq
   if (want != n_pages)
     return fail(BCH_ERR_ARGUMENT, "%s: the sequences need %llu pages, got %llu", kernel, (unsigned long long)want,
                 (unsigned long long)n_pages);
-  if (tokens > kKvMaxPositions) return fail(BCH_ERR_ARGUMENT, "%s: more than 2^31 - 1 tokens", kernel);
+  if (tokens > kKvMaxTokens) return fail(BCH_ERR_ARGUMENT, "%s: more than 2^26 new tokens", kernel);
   uint32_t last = 0;
   for (uint64_t i = 0; i < n_pages; i++) {
     if (pages[i] >= s->n_pages)
@@ -84,6 +85,7 @@ int kv_plan_cache(bch_ctx *ctx, const char *kernel, const bch_kv_plan *plan, bch
   if (!plan->ready) return fail(BCH_ERR_ARGUMENT, "%s: the plan has no batch", kernel);
   BCH_TRY(check_view(ctx, kernel, cache, bch_kv_page_bytes(&plan->shape) * plan->shape.n_pages, ptr));
   if (reinterpret_cast<uintptr_t>(*ptr) % 16) return fail(BCH_ERR_ARGUMENT, "%s: the cache must be 16-byte aligned", kernel);
+  plan->last_use = ctx->committed + 1;
   return BCH_OK;
 }
 
@@ -126,15 +128,22 @@ static int plan_set(bch_kv_plan *plan, uint32_t n_seqs, const uint32_t *n_past, 
     row += n_new[i];
     table += (end + plan->shape.page_size - 1) / plan->shape.page_size;
   }
+  const KvSchedule work = kv_schedule(seqs, plan->n_heads / plan->shape.n_kv_heads, plan->shape.n_kv_heads,
+                                      plan->shape.head_dim, plan->ctx->n_cus, plan->ctx->attn_partials ? kAttnPartialFloats : 0);
   Layout all;
-  const uint64_t at_seqs = all.add(seqs.data(), seqs.size());
   const uint64_t at_pages = all.add(pages, n_pages);
   const uint64_t at_store = all.add(store.data(), store.size());
+  const uint64_t at8 = all.add(work.narrow.data(), work.narrow.size());
+  const uint64_t at16 = all.add(work.tokens.data(), work.tokens.size());
+  const uint64_t at_chunks = all.add(work.chunks.data(), work.chunks.size());
+  const uint64_t at_join = all.add(work.join.data(), work.join.size());
 
-  // Launches that were recorded and discarded still read the last batch.
-  hipStream_t s = plan->ctx->stream;
   plan->ready = false;
-  if (hipStreamSynchronize(s) != hipSuccess) return fail(BCH_ERR_EXECUTION, "kv_plan_set: the stream failed");
+  // Launches of a recording that was discarded have no ticket and may still
+  // read the last batch.
+  if (plan->last_use > plan->ctx->committed && hipStreamSynchronize(plan->ctx->stream) != hipSuccess)
+    return fail(BCH_ERR_EXECUTION, "kv_plan_set: the stream failed");
+  plan->last_use = 0;
   if (all.bytes.size() > plan->memory_bytes) {
     if (plan->memory) hipFree(plan->memory);
     plan->memory = nullptr;
@@ -148,17 +157,28 @@ static int plan_set(bch_kv_plan *plan, uint32_t n_seqs, const uint32_t *n_past, 
     plan->memory = static_cast<uint8_t *>(p);
     plan->memory_bytes = room;
   }
+  // Not on the context's stream, where the copy would wait for the steps of
+  // other plans; done before this returns, so before any launch that reads it.
   if (!all.bytes.empty() &&
-      (hipMemcpyAsync(plan->memory, all.bytes.data(), all.bytes.size(), hipMemcpyHostToDevice, s) != hipSuccess ||
-       hipStreamSynchronize(s) != hipSuccess))
+      (hipMemcpy(plan->memory, all.bytes.data(), all.bytes.size(), hipMemcpyHostToDevice) != hipSuccess ||
+       hipStreamSynchronize(nullptr) != hipSuccess))
     return fail(BCH_ERR_EXECUTION, "kv_plan_set: host-to-device copy failed");
   plan->seqs.swap(seqs);
   plan->n_seqs = n_seqs;
   plan->n_tokens = row;
-  plan->d_seqs = reinterpret_cast<const KvSeq *>(plan->memory + at_seqs);
   plan->d_pages = reinterpret_cast<const uint32_t *>(plan->memory + at_pages);
   plan->d_store = reinterpret_cast<const KvStoreItem *>(plan->memory + at_store);
   plan->n_store = (uint32_t)store.size();
+  plan->d_tiles8 = reinterpret_cast<const KvAttnItem *>(plan->memory + at8);
+  plan->d_tiles16 = reinterpret_cast<const KvAttnItem *>(plan->memory + at16);
+  plan->d_chunks = reinterpret_cast<const KvAttnItem *>(plan->memory + at_chunks);
+  plan->d_join = reinterpret_cast<const KvJoinItem *>(plan->memory + at_join);
+  plan->n_tiles8 = (uint32_t)work.narrow.size();
+  plan->n_tiles16 = (uint32_t)work.tokens.size();
+  plan->n_chunks = (uint32_t)work.chunks.size();
+  plan->n_join = (uint32_t)work.join.size();
+  plan->join_rows = 0;
+  for (const KvJoinItem &j : work.join) plan->join_rows = std::max(plan->join_rows, j.rows);
   plan->ready = true;
   return BCH_OK;
 }
@@ -212,8 +232,10 @@ void bch_kv_plan_free(bch_kv_plan *plan) {
 int bch_kv_plan_set(bch_kv_plan *plan, uint32_t n_seqs, const uint32_t *n_past, const uint32_t *n_new,
                     const uint32_t *pages, uint64_t n_pages) {
   if (!plan) return fail(BCH_ERR_ARGUMENT, "kv_plan_set: no plan");
-  if (plan->ctx->committed > plan->ctx->waited || plan->ctx->recording)
-    return fail(BCH_ERR_BUSY, "kv_plan_set: the batch cannot change while work is in flight");
+  // In the open recording, or in one that has not been waited for.
+  const bch_ctx *ctx = plan->ctx;
+  if (plan->last_use > ctx->waited && (plan->last_use <= ctx->committed || ctx->recording))
+    return fail(BCH_ERR_BUSY, "kv_plan_set: the batch cannot change while work that uses it is in flight");
   BCH_TRY(bch_kv_plan_check(&plan->shape, plan->n_heads, n_seqs, n_past, n_new, pages, n_pages));
   try {
     return plan_set(plan, n_seqs, n_past, n_new, pages, n_pages);

@@ -3,8 +3,8 @@
 //
 // A row x of hd floats (one position and KV head) is kept as f16, or as
 // y = clamp(x / s, -top, top) rounded to int8 (top 127) or e4m3 (top 448) with
-// the row's own scale s = clamp(max|x| / top, 2^-40, 2^60); it reads back as
-// s·y.  A row that holds a NaN or an infinity gets the scale NaN, so all of it
+// the row's own scale s = clamp(max|x|·(1/top), 2^-40, 2^60), 1/top rounded to
+// f32; it reads back as s·y.  A row that holds a NaN or an infinity gets the scale NaN, so all of it
 // reads back as NaN.
 #include <cmath>
 
@@ -20,7 +20,7 @@ constexpr uint32_t kStoreThreads = 256;  // 16 lanes for each of a block's 16 ro
 // The scale of a row from the largest magnitude of its elements, of which one
 // that is not finite counts as infinite.
 __device__ __forceinline__ float kv_scale(float largest, float top) {
-  const float s = fminf(fmaxf(largest / top, kKvScaleMin), kKvScaleMax);
+  const float s = fminf(fmaxf(largest * (1.f / top), kKvScaleMin), kKvScaleMax);
   return largest <= 3.402823466e38f ? s : __int_as_float(0x7fc00000);
 }
 

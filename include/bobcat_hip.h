@@ -328,9 +328,10 @@ int bch_moe_combine(bch_ctx *ctx, bch_view x, bch_view route, bch_view y, uint32
 /* the same page numbers, one buffer (or view) for each layer.           */
 /*                                                                      */
 /* The rows x of a position and head are kept as f16, or with a scale of */
-/* their own: s = clamp(max|x| / top, 2^-40, 2^60), y = x / s rounded to */
-/* the nearest int8 (top 127) or e4m3 (top 448), ties to even, and read  */
-/* back as s·y.  A row with a NaN or an infinity reads back as NaN.      */
+/* their own: s = clamp(max|x|·(1/top), 2^-40, 2^60), y = x / s rounded  */
+/* to the nearest int8 (top 127) or e4m3 (top 448), ties to even, and    */
+/* read back as s·y (1/top, s and x / s are f32).  A row with a NaN or   */
+/* an infinity reads back as NaN.                                        */
 /*                                                                      */
 /* Layout, for programs that move pages: a page is [head][16 positions], */
 /* a block of 16 positions of a head its keys, its values and (8-bit     */
@@ -368,8 +369,9 @@ int bch_kv_plan_check(const bch_kv_shape *shape, uint32_t n_heads, uint32_t n_se
 int bch_kv_plan_new(bch_ctx *ctx, const bch_kv_shape *shape, uint32_t n_heads, bch_kv_plan **out);
 void bch_kv_plan_free(bch_kv_plan *plan);
 /* Give the plan a batch (copied: the arrays are free on return).  Fails with
- * BCH_ERR_BUSY while work is recorded or in flight, as bch_write does.  A batch
- * that is refused leaves the plan as it was; after any other failure it has none. */
+ * BCH_ERR_BUSY while work that uses the plan is recorded or in flight (another
+ * plan can be set meanwhile).  A batch that is refused leaves the plan as it
+ * was; after any other failure it has none. */
 int bch_kv_plan_set(bch_kv_plan *plan, uint32_t n_seqs, const uint32_t *n_past, const uint32_t *n_new,
                     const uint32_t *pages, uint64_t n_pages);
 
@@ -389,7 +391,8 @@ int bch_kv_load(bch_ctx *ctx, const bch_kv_plan *plan, bch_view cache, uint32_t 
  * n_heads·head_dim floats, q_stride and out_stride floats apart (16-byte
  * aligned, strides a multiple of 4); query head h reads KV head
  * h / (n_heads / n_kv_heads).  `out` may not lie over `q`.  What a query does
- * not see has no part in its output, whatever it holds.  The queries and the
+ * not see has no part in its output, whatever it holds; a value that it sees
+ * and that is infinite or NaN makes that element of its output NaN.  The queries and the
  * probabilities enter the products with ~22 bits, as in
  * bch_attention_prefill. */
 int bch_attention_paged(bch_ctx *ctx, const bch_kv_plan *plan, bch_view cache, bch_view q, uint32_t q_stride,

@@ -39,7 +39,7 @@ def quantise(x: np.ndarray, fmt: str):
     fine = np.isfinite(x).all(-1)
     with np.errstate(invalid="ignore", over="ignore"):
         largest = np.abs(x).max(-1)
-        scale = np.clip(largest / TOP[fmt], np.float32(2.0 ** -40), np.float32(2.0 ** 60)).astype(np.float32)
+        scale = np.clip(largest * (np.float32(1) / TOP[fmt]), np.float32(2.0 ** -40), np.float32(2.0 ** 60)).astype(np.float32)
         y = np.clip(x / scale[..., None], -TOP[fmt], TOP[fmt])
     y = np.where(fine[..., None], y, np.float32(0))
     bits = np.rint(y).astype(np.int8).view(np.uint8) if fmt == "i8" else to_e4m3(y)

@@ -414,11 +414,13 @@ def test_plans_of_other_contexts_and_busy_plans(hip):
         with pytest.raises(BobcatError) as e:
             hip.attention_paged(foreign, cache.at(0), b.at(0), 256, b.at(1 << 15), 256)
         assert e.value.status == STATUS["ForeignBuffer"]
+        plan.set(batch.past, batch.new, batch.pages)  # nothing that uses it has been recorded
+        hip.attention_paged(plan, cache.at(0), b.at(0), 256, b.at(1 << 15), 256)
         with pytest.raises(BobcatError) as e:
             plan.set(batch.past, batch.new, batch.pages)
         assert e.value.status == STATUS["Busy"]
-        hip.attention_paged(plan, cache.at(0), b.at(0), 256, b.at(1 << 15), 256)
         ticket = hip.commit()
+        plan_of(hip, pool, batch, 4)  # another plan is free
         with pytest.raises(BobcatError) as e:
             plan.set(batch.past, batch.new, batch.pages)
         assert e.value.status == STATUS["Busy"]
@@ -426,6 +428,12 @@ def test_plans_of_other_contexts_and_busy_plans(hip):
         # A batch that is refused leaves the one before.
         with pytest.raises(BobcatError):
             plan.set(batch.past, batch.new, [[99] * 2])
+        check_attention(hip, pool, batch, 4, q, plan=plan)
+        # A discarded recording's launches run on; its plan can be set again.
+        hip.begin()
+        hip.attention_paged(plan, cache.at(0), b.at(0), 256, b.at(1 << 15), 256)
+        hip.discard()
+        plan.set(batch.past, batch.new, batch.pages)
         check_attention(hip, pool, batch, 4, q, plan=plan)
     finally:
         other.close()
