@@ -22,9 +22,9 @@
 // in f32.  With a row's key scale a and value scale b (1 in f16) and a running
 // reference m,
 //   u = a·s − m,  p = 2^u,  l += p,  O += (p·b)·v,
-// where m follows the largest u + log2 b: p·b then stays near 1 as f16 wants
-// it, whatever the scales, and p needs no bound of its own (scales lie in
-// 2^-40 .. 2^60).  m moves only when p·b would pass 2^8, so most steps rescale
+// where m follows the largest u + log2 b: p·b then stays inside f16's range,
+// whatever the scales, and p needs no bound of its own (scales lie in 2^-40 ..
+// 2^60).  m moves only when p·b would leave its range, so most steps rescale
 // nothing.
 #include <algorithm>
 #include <cmath>
@@ -44,7 +44,10 @@ typedef float af4_t __attribute__((ext_vector_type(4)));
 typedef float af16_t __attribute__((ext_vector_type(16)));
 typedef uint32_t au4_t __attribute__((ext_vector_type(4)));
 
-constexpr float kLazy = 8.f;             // p·b may pass its reference by 2^kLazy
+// The reference is set so that the largest p·b is 2^kPeak, and moves when one
+// passes 2^kLazy: high in f16's range, so that the low parts of much smaller
+// ones are still normal numbers, with room for scale_log's error.
+constexpr float kPeak = 8.f, kLazy = 14.f;
 constexpr float kUnset = -INFINITY;      // in its place, of a row that has seen no key yet
 
 // Four elements of 8 bits as f16, exactly.
@@ -250,7 +253,7 @@ __global__ __launch_bounds__(256) void k_attn_tokens(KvGeometry g, const KvAttnI
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
       const bool move = top > lazy;  // the same in the four lanes of a row
-      const float d = move ? top : 0.f, corr = !move || lazy == kUnset ? 1.f : __builtin_amdgcn_exp2f(-d);
+      const float d = move ? top - kPeak : 0.f, corr = !move || lazy == kUnset ? 1.f : __builtin_amdgcn_exp2f(-d);
       m += d;
       l *= corr;
       lazy = move ? kLazy : lazy;
@@ -374,98 +377,102 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : HD == 128 ? 2 : 1) void k_attn_
     uint32_t group, float c2) {
   constexpr bool QUANT = FORMAT != BCH_KV_F16;
   constexpr uint32_t SIZE = kv_elem_bytes(FORMAT), BYTES = kv_block_bytes(FORMAT, HD), PART = kKvBlock * HD * SIZE;
-  constexpr uint32_t KEYS = kChunkKeys<HD>, TILES = KEYS / 32, KS = HD / 16, OB = HD / 32, M = 4 / SIZE;
+  constexpr uint32_t KEYS = kChunkKeys<HD>, KS = HD / 16, OB = HD / 32, M = 4 / SIZE;
   constexpr uint32_t PIECES = HD * SIZE;              // 16-byte pieces of a block's keys, and of its values
   constexpr uint32_t NP = KEYS / 16 * PIECES / 256;   // of each per thread and step
   // Keys: 8 elements of key k at slot (element / 8)·KEYS + k.  Values: the keys
   // {0..3, 8..11} + 4h of 16 keys of element d at slot (2·(key / 16) + h)·HD + d.
   __shared__ __align__(16) _Float16 k_s[2][KEYS * HD], v_s[2][KEYS * HD];
-  __shared__ __align__(16) float ks_s[2][KEYS], vs_s[2][KEYS];
-  __shared__ float top_s[2];
+  __shared__ __align__(16) float s_s[2][2][KEYS];         // the keys' and the values' scales
+  __shared__ float top_s[2][KEYS / kKvBlock];             // the largest scale_log of each block's values
   __shared__ uint32_t odd_s[2];
   const uint32_t kv = blockIdx.x % g.n_kv;
   const KvAttnItem it = items[blockIdx.x / g.n_kv];
-  const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
+  const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64) & 3, lane = tid % 64;
   const uint32_t col = lane % 32, half_id = lane / 32;
   const bool active = 32 * wave < it.rows;
   const uint32_t row0 = it.first + (active ? 32 * wave : 0);
   const uint32_t rows = active ? min(32u, it.rows - 32 * wave) : 1;
   const uint32_t packed = row0 + min(col, rows - 1);
   const uint32_t token = packed / group, head = kv * group + packed % group, pos = it.past + token;
-  const uint32_t pos0 = it.past + row0 / group;                          // of the wave's first row
   const uint32_t kend = it.past + (row0 + rows - 1) / group + 1;         // keys of the wave's last row
-  const uint32_t wg_pos0 = it.past + it.first / group;
+  const uint32_t wg_pos0 = it.past + it.first / group;                   // the workgroup's first row's
   const uint32_t wg_kend = it.past + (it.first + it.rows - 1) / group + 1;
   const uint32_t last = (wg_kend - 1) / kKvBlock;
   const uint32_t lo = it.lo * 32, hi = min(it.hi * 32, wg_kend);         // keys of this split
 
   au4_t kr[NP], vr[NP];
-  float sk = 0.f, sv = 0.f;
+  float scale = 0.f;  // of wave w: lanes 0..15 the key scales of block w of the step, 16..31 the value scales
   // Lanes of a value piece: quads of keys in the order 0, 2, 1, 3, so that the
   // two quads whose halves of a slot interleave are written together.
   const uint32_t swapped = (lane & 15) | (lane & 16) << 1 | (lane & 32) >> 1;
+  // This wave's pieces of part p are within .. + 64 of block j of the step.
+  auto part_block = [&](uint32_t p) { return 64 * wave / PIECES + 256 * p / PIECES; };
+  auto part_within = [&](uint32_t p) { return 64 * wave % PIECES + 256 * p % PIECES; };
   auto load = [&](uint32_t kb) __attribute__((always_inline)) {
 #pragma unroll
     for (uint32_t p = 0; p < NP; p++) {
-      const uint32_t at = 64 * wave + 256 * p, j = at / PIECES, within = at % PIECES;
+      const uint32_t j = part_block(p), within = part_within(p);
       const uint8_t *b = g.block<BYTES>(it.table, min(kb / kKvBlock + j, last), kv);
       kr[p] = *reinterpret_cast<const au4_t *>(b + 16 * (within + lane));
       vr[p] = *reinterpret_cast<const au4_t *>(b + PART + 16 * (within + swapped));
     }
     if constexpr (QUANT) {
-      if (tid < KEYS) {
-        const uint8_t *b = g.block<BYTES>(it.table, min(kb / kKvBlock + tid / kKvBlock, last), kv) + 2 * PART;
-        sk = reinterpret_cast<const float *>(b)[tid % kKvBlock];
-        sv = reinterpret_cast<const float *>(b)[kKvBlock + tid % kKvBlock];
-      }
+      if (wave < KEYS / kKvBlock && lane < 32)
+        scale = reinterpret_cast<const float *>(g.block<BYTES>(it.table, min(kb / kKvBlock + wave, last), kv) + 2 * PART)[lane];
     }
   };
-  auto stage = [&](int buf, uint32_t kb) __attribute__((always_inline)) {
+  // With `ends`, keys behind the last are cleared where they could be NaN, and
+  // f16 values that are not finite noted.
+  auto stage = [&](int buf, uint32_t kb, auto at_end) __attribute__((always_inline)) {
+    constexpr bool ends = decltype(at_end)::value;
     bool odd = false;
 #pragma unroll
     for (uint32_t p = 0; p < NP; p++) {
-      const uint32_t at = 64 * wave + 256 * p, j = at / PIECES, within = at % PIECES;
-      const uint32_t piece = (within + lane) / 16, key = 16 * j + lane % 16;
+      const uint32_t j = part_block(p), within = part_within(p);
+      const uint32_t piece = within / 16 + lane / 16, key = 16 * j + lane % 16;
       if constexpr (QUANT) {
         *reinterpret_cast<ah8_t *>(&k_s[buf][(2 * piece * KEYS + key) * 8]) = join(widen<FORMAT>(kr[p][0]), widen<FORMAT>(kr[p][1]));
         *reinterpret_cast<ah8_t *>(&k_s[buf][((2 * piece + 1) * KEYS + key) * 8]) = join(widen<FORMAT>(kr[p][2]), widen<FORMAT>(kr[p][3]));
       } else {
         *reinterpret_cast<au4_t *>(&k_s[buf][(piece * KEYS + key) * 8]) = kr[p];
       }
-      const uint32_t v = within + swapped, quad = v / 16 % 4;
+      const uint32_t quad = swapped / 16;
       // Bytes behind the last key may be NaN.  (Those of stored rows never are.)
-      if constexpr (FORMAT == BCH_KV_F8) {
+      if constexpr (FORMAT == BCH_KV_F8 && ends) {
         if (kb + KEYS > wg_kend) vr[p] &= bytes_below((int)(wg_kend - (kb + 16 * j + 4 * quad)));
       }
 #pragma unroll
       for (uint32_t x = 0; x < M; x++) {
-        const uint32_t d = v / 64 * 16 * M + 16 * x + v % 16;
+        const uint32_t d = within / 4 * M + 16 * x + lane % 16;
         ah4_t a;
         if constexpr (QUANT)
           a = widen<FORMAT>(vr[p][x]);
         else
           a = halves(vr[p][2 * x], vr[p][2 * x + 1]);
-        if constexpr (!QUANT) {
-          if (kb + KEYS - 1 > wg_pos0) {
+        if constexpr (!QUANT && ends) {
 #pragma unroll
-            for (uint32_t i = 0; i < 4; i++) {
-              if (kb + 16 * j + 4 * quad + i >= wg_kend) a[i] = (_Float16)0.f;
-              odd |= not_finite(a[i]);
-            }
+          for (uint32_t i = 0; i < 4; i++) {
+            if (kb + 16 * j + 4 * quad + i >= wg_kend) a[i] = (_Float16)0.f;
+            odd |= not_finite(a[i]);
           }
         }
         *reinterpret_cast<ah4_t *>(&v_s[buf][((2 * j + quad % 2) * HD + d) * 8 + quad / 2 * 4]) = a;
       }
     }
     if constexpr (QUANT) {
-      if (wave == 0) {
-        const float b = lane < KEYS && kb + lane < wg_kend ? sv : 0.f;
-        if (lane < KEYS) ks_s[buf][lane] = sk, vs_s[buf][lane] = b;
-        const float top = wave_max(b == b ? scale_log(b) : 0.f);
-        if (lane == 0) top_s[buf] = top - 127.f;
+      if (wave < KEYS / kKvBlock && lane < 32) {
+        const float x = ends && lane >= 16 && kb + 16 * wave + lane % 16 >= wg_kend ? 0.f : scale;
+        s_s[buf][lane / 16][16 * wave + lane % 16] = x;
+        float top = x == x ? scale_log(x) : 0.f;
+        top = fmaxf(top, dpp<kDppXor1>(top));
+        top = fmaxf(top, dpp<kDppXor2>(top));
+        top = fmaxf(top, dpp<kDppHalfMirror>(top));
+        top = fmaxf(top, dpp<kDppMirror>(top));
+        if (lane == 16) top_s[buf][wave] = top - 127.f;
       }
-    } else if (kb + KEYS - 1 > wg_pos0) {
-      if (__builtin_amdgcn_ballot_w64(odd) && lane == 0) odd_s[buf] = 1;  // (cleared after each masked step)
+    } else if constexpr (ends) {
+      if (__builtin_amdgcn_ballot_w64(odd) && lane == 0) odd_s[buf] = 1;  // (cleared after the step)
     }
   };
   if (tid < 2) odd_s[tid] = 0;
@@ -475,27 +482,26 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : HD == 128 ? 2 : 1) void k_attn_
   float back = 1.f;
   {
     const float *qr = q + (uint64_t)(it.row + token) * q_stride + (uint64_t)head * HD + 8 * half_id;
-    float largest = 0.f;
+    auto take = [&](float factor) __attribute__((always_inline)) {
+      float largest = 0.f;
 #pragma unroll
-    for (uint32_t s = 0; s < KS; s++) {
-      const float4 a = *reinterpret_cast<const float4 *>(qr + 16 * s), b = *reinterpret_cast<const float4 *>(qr + 16 * s + 4);
-      const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+      for (uint32_t s = 0; s < KS; s++) {
+        const float4 a = *reinterpret_cast<const float4 *>(qr + 16 * s), b = *reinterpret_cast<const float4 *>(qr + 16 * s + 4);
+        const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-      for (int j = 0; j < 8; j++) largest = fmaxf(largest, fabsf(v[j] * c2));
-    }
-    largest = fmaxf(largest, __shfl_xor(largest, 32, 64));
-    const float down = query_down(largest);
-    back = 1.f / down;
-#pragma unroll
-    for (uint32_t s = 0; s < KS; s++) {
-      const float4 a = *reinterpret_cast<const float4 *>(qr + 16 * s), b = *reinterpret_cast<const float4 *>(qr + 16 * s + 4);
-      const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const float x = v[j] * c2 * down;
-        qh[s][j] = (_Float16)x;
-        ql[s][j] = (_Float16)(x - (float)qh[s][j]);
+        for (int j = 0; j < 8; j++) {
+          const float x = v[j] * c2 * factor;
+          largest = fmaxf(largest, fabsf(x));
+          qh[s][j] = (_Float16)x;
+          ql[s][j] = (_Float16)(x - (float)qh[s][j]);
+        }
       }
+      return fmaxf(largest, __shfl_xor(largest, 32, 64));
+    };
+    const float down = query_down(take(1.f));
+    if (__builtin_amdgcn_ballot_w64(down != 1.f)) {
+      take(down);
+      back = 1.f / down;
     }
   }
   const bool far = __builtin_amdgcn_ballot_w64(back != 1.f) != 0;
@@ -506,59 +512,62 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : HD == 128 ? 2 : 1) void k_attn_
     for (int i = 0; i < 16; i++) o[b][i] = 0.f;
   float m = 0.f, l = 0.f, lazy = kUnset;
 
-  // One step of KEYS keys; score r of tile t is of key kb + 32t + 8·(r / 4) +
-  // 4·half + r % 4.
-  auto step = [&](uint32_t kb, int buf, auto is_masked) __attribute__((always_inline)) {
+  // 32 keys of a step from key kb on, in LDS from key k0 on; score r is of key
+  // kb + 8·(r / 4) + 4·half + r % 4.
+  auto tile = [&](uint32_t kb, uint32_t k0, int buf, auto is_masked) __attribute__((always_inline)) {
     constexpr bool masked = decltype(is_masked)::value;
-    af16_t u[TILES];
-    float vs[TILES][16];
+    af16_t u;
 #pragma unroll
-    for (uint32_t t = 0; t < TILES; t++) {
+    for (int i = 0; i < 16; i++) u[i] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; i++) u[t][i] = 0.f;
-#pragma unroll
-      for (uint32_t s = 0; s < KS; s++) {
-        const ah8_t a = *reinterpret_cast<const ah8_t *>(&k_s[buf][((2 * s + half_id) * KEYS + 32 * t + col) * 8]);
-        u[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[s], u[t], 0, 0, 0);
-        u[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[s], u[t], 0, 0, 0);
-      }
+    for (uint32_t s = 0; s < KS; s++) {
+      const ah8_t a = *reinterpret_cast<const ah8_t *>(&k_s[buf][((2 * s + half_id) * KEYS + k0 + col) * 8]);
+      u = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[s], u, 0, 0, 0);
+      u = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[s], u, 0, 0, 0);
     }
+    // The values' operands come while the softmax is computed (heads of 256
+    // have no registers for them).
+    auto value = [&](int j, uint32_t b) __attribute__((always_inline)) {
+      return *reinterpret_cast<const ah8_t *>(&v_s[buf][((k0 / 8 + 2 * j + half_id) * HD + 32 * b + col) * 8]);
+    };
+    ah8_t v[2][HD == 256 ? 1 : OB];
+    if constexpr (HD != 256) {
 #pragma unroll
-    for (uint32_t t = 0; t < TILES; t++)
+      for (int j = 0; j < 2; j++)
 #pragma unroll
-      for (int q4 = 0; q4 < 4; q4++) {
-        float4 a, b;
-        if constexpr (QUANT) {
-          a = *reinterpret_cast<const float4 *>(&ks_s[buf][32 * t + 8 * q4 + 4 * half_id]);
-          b = *reinterpret_cast<const float4 *>(&vs_s[buf][32 * t + 8 * q4 + 4 * half_id]);
-        }
-        const float as[4] = {a.x, a.y, a.z, a.w}, bs[4] = {b.x, b.y, b.z, b.w};
+        for (uint32_t b = 0; b < OB; b++) v[j][b] = value(j, b);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (far) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int r = 4 * q4 + i;
-          float x = u[t][r];
-          if (far) x *= back;
-          u[t][r] = QUANT ? fmaf(x, as[i], -m) : x - m;
-          vs[t][r] = QUANT ? bs[i] : 1.f;
-          if constexpr (masked) {
-            const bool seen = kb + 32 * t + 8 * q4 + 4 * half_id + i <= pos;
-            u[t][r] = seen ? u[t][r] : -INFINITY;
-            vs[t][r] = seen ? vs[t][r] : 0.f;
-          }
-        }
-      }
+      for (int r = 0; r < 16; r++) u[r] *= back;
+    }
     // The largest u + log2 b: key by key where some are not seen (those must
     // change nothing), else from the largest of both.
     float top = -INFINITY;
+    auto scales = [&](const float *from, int q4) __attribute__((always_inline)) {
+      const float4 a = *reinterpret_cast<const float4 *>(from + k0 + 8 * q4 + 4 * half_id);
+      return af4_t{a.x, a.y, a.z, a.w};
+    };
+    auto seen = [&](int r) __attribute__((always_inline)) { return kb + 8 * (r / 4) + 4 * half_id + r % 4 <= pos; };
 #pragma unroll
-    for (uint32_t t = 0; t < TILES; t++)
+    for (int q4 = 0; q4 < 4; q4++) {
+      af4_t a, b;
+      if constexpr (QUANT) a = scales(s_s[buf][0], q4);
+      if constexpr (QUANT && masked) b = scales(s_s[buf][1], q4);
 #pragma unroll
-      for (int r = 0; r < 16; r++) top = fmaxf(top, QUANT && masked ? u[t][r] + scale_log(vs[t][r]) : u[t][r]);
-    if constexpr (QUANT) top += masked ? -127.f : top_s[buf];
+      for (int i = 0; i < 4; i++) {
+        const int r = 4 * q4 + i;
+        u[r] = QUANT ? fmaf(u[r], a[i], -m) : u[r] - m;
+        if constexpr (masked) u[r] = seen(r) ? u[r] : -INFINITY;
+        top = fmaxf(top, QUANT && masked ? u[r] + scale_log(b[i]) : u[r]);
+      }
+    }
+    if constexpr (QUANT) top += masked ? -127.f : fmaxf(top_s[buf][k0 / 16], top_s[buf][k0 / 16 + 1]);
     if (__builtin_amdgcn_ballot_w64(top > lazy)) {
       top = fmaxf(top, __shfl_xor(top, 32, 64));
       const bool move = top > lazy;  // the same in both lanes of a row
-      const float d = move ? top : 0.f, corr = !move || lazy == kUnset ? 1.f : __builtin_amdgcn_exp2f(-d);
+      const float d = move ? top - kPeak : 0.f, corr = !move || lazy == kUnset ? 1.f : __builtin_amdgcn_exp2f(-d);
       m += d;
       l *= corr;
       lazy = move ? kLazy : lazy;
@@ -567,77 +576,92 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : HD == 128 ? 2 : 1) void k_attn_
 #pragma unroll
         for (int i = 0; i < 16; i++) o[b][i] *= corr;
 #pragma unroll
-      for (uint32_t t = 0; t < TILES; t++)
-#pragma unroll
-        for (int r = 0; r < 16; r++) u[t][r] -= d;
+      for (int r = 0; r < 16; r++) u[r] -= d;
     }
+    ah8_t ph[2], pl[2];
 #pragma unroll
-    for (uint32_t t = 0; t < TILES; t++) {
-      ah8_t ph[2], pl[2];
+    for (int q4 = 0; q4 < 4; q4++) {
+      af4_t b;
+      if constexpr (QUANT) b = scales(s_s[buf][1], q4);
 #pragma unroll
-      for (int r = 0; r < 16; r += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(u[t][r]), p1 = __builtin_amdgcn_exp2f(u[t][r + 1]);
+      for (int i = 0; i < 4; i += 2) {
+        const int r = 4 * q4 + i;
+        const float p0 = __builtin_amdgcn_exp2f(u[r]), p1 = __builtin_amdgcn_exp2f(u[r + 1]);
         l += p0 + p1;
-        const af2_t pv = {QUANT ? p0 * vs[t][r] : p0, QUANT ? p1 * vs[t][r + 1] : p1};
+        af2_t pv = {p0, p1};
+        if constexpr (QUANT) {
+          // (A scale may be NaN, which 0 times it would be too.)
+          if constexpr (masked) b[i] = seen(r) ? b[i] : 0.f, b[i + 1] = seen(r + 1) ? b[i + 1] : 0.f;
+          pv = {p0 * b[i], p1 * b[i + 1]};
+        }
         const ah2_t h = __builtin_convertvector(pv, ah2_t);
         const af2_t rest = {pv[0] - (float)h[0], pv[1] - (float)h[1]};
         const ah2_t e = __builtin_convertvector(rest, ah2_t);
         ph[r / 8][r % 8] = h[0], ph[r / 8][r % 8 + 1] = h[1];
         pl[r / 8][r % 8] = e[0], pl[r / 8][r % 8 + 1] = e[1];
       }
-#pragma unroll
-      for (int j = 0; j < 2; j++)
-#pragma unroll
-        for (uint32_t b = 0; b < OB; b++) {
-          ah8_t a = *reinterpret_cast<const ah8_t *>(&v_s[buf][((2 * (2 * t + j) + half_id) * HD + 32 * b + col) * 8]);
-          if constexpr (masked && !QUANT) {
-            // 0 times a value that is not finite is NaN: rows that see such a
-            // value get it from a count, and the product leaves it out.
-            if (odd_s[buf]) {
-              ah8_t seen, bad;
-              af16_t count;
-#pragma unroll
-              for (int i = 0; i < 16; i++) count[i] = 0.f;
-#pragma unroll
-              for (int i = 0; i < 8; i++) {
-                seen[i] = (_Float16)(kb + 32 * t + 16 * j + 4 * half_id + (i & 4) * 2 + (i & 3) <= pos ? 1.f : 0.f);
-                bad[i] = (_Float16)(not_finite(a[i]) ? 1.f : 0.f);
-                a[i] = not_finite(a[i]) ? (_Float16)0.f : a[i];
-              }
-              count = __builtin_amdgcn_mfma_f32_32x32x16_f16(bad, seen, count, 0, 0, 0);
-#pragma unroll
-              for (int i = 0; i < 16; i++) o[b][i] = count[i] > 0.f ? NAN : o[b][i];
-            }
-          }
-          o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[j], o[b], 0, 0, 0);
-          o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[j], o[b], 0, 0, 0);
-        }
     }
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+#pragma unroll
+      for (uint32_t b = 0; b < OB; b++) {
+        ah8_t a = HD == 256 ? value(j, b) : v[j][HD == 256 ? 0 : b];
+        if constexpr (masked && !QUANT) {
+          // 0 times a value that is not finite is NaN: rows that see such a
+          // value get it from a count, and the product leaves it out.
+          if (odd_s[buf]) {
+            ah8_t seen, bad;
+            af16_t count;
+#pragma unroll
+            for (int i = 0; i < 16; i++) count[i] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              seen[i] = (_Float16)(kb + 16 * j + 4 * half_id + (i & 4) * 2 + (i & 3) <= pos ? 1.f : 0.f);
+              bad[i] = (_Float16)(not_finite(a[i]) ? 1.f : 0.f);
+              a[i] = not_finite(a[i]) ? (_Float16)0.f : a[i];
+            }
+            count = __builtin_amdgcn_mfma_f32_32x32x16_f16(bad, seen, count, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[b][i] = count[i] > 0.f ? NAN : o[b][i];
+          }
+        }
+        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[j], o[b], 0, 0, 0);
+        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[j], o[b], 0, 0, 0);
+      }
   };
   if (lo < hi) {
+    const uint32_t last_step = (hi - 1) / KEYS * KEYS;
     __syncthreads();  // odd_s is clear
-    stage(0, lo);
-    load(min(lo + KEYS, hi - 1) / KEYS * KEYS);
+    stage(0, lo, std::true_type{});
+    load(min(lo + KEYS, last_step));
     lds_barrier();
+    uint32_t kb = lo;
     int buf = 0;
-    for (uint32_t kb = lo; kb < hi; kb += KEYS, buf ^= 1) {
+    // Steps that every row sees whole, the next one too.
+    for (; kb + KEYS <= last_step && kb + 2 * KEYS - 1 <= wg_pos0; kb += KEYS, buf ^= 1) {
       // The other buffer was read before the last barrier.
-      if (kb + KEYS < hi) {
-        stage(buf ^ 1, kb + KEYS);
-        load(min(kb + 2 * KEYS, hi - 1) / KEYS * KEYS);
+      stage(buf ^ 1, kb + KEYS, std::false_type{});
+      load(min(kb + 2 * KEYS, last_step));
+      if (active) {
+#pragma unroll 1
+        for (uint32_t k0 = 0; k0 < KEYS; k0 += 32) tile(kb + k0, k0, buf, std::false_type{});
       }
-      if (active && kb < kend) {
-        if (kb + KEYS - 1 > pos0)
-          step(kb, buf, std::true_type{});
-        else
-          step(kb, buf, std::false_type{});
+      lds_barrier();
+    }
+    // The others.
+    for (; kb < hi; kb += KEYS, buf ^= 1) {
+      if (kb < last_step) {
+        stage(buf ^ 1, kb + KEYS, std::true_type{});
+        load(min(kb + 2 * KEYS, last_step));
+      }
+      if (active) {
+#pragma unroll 1
+        for (uint32_t k0 = 0; k0 < KEYS && kb + k0 < kend; k0 += 32) tile(kb + k0, k0, buf, std::true_type{});
       }
       lds_barrier();
       if constexpr (!QUANT) {
-        if (kb + KEYS - 1 > wg_pos0) {
-          if (tid == 0) odd_s[buf] = 0;
-          lds_barrier();
-        }
+        if (tid == 0) odd_s[buf] = 0;
+        lds_barrier();
       }
     }
   }
@@ -676,15 +700,14 @@ __global__ __launch_bounds__(256) void k_attn_join(const KvJoinItem *__restrict_
 
 // --- the work of a batch ----------------------------------------------------------
 
-// Splits: a workgroup takes about `share` steps of 32 keys, so that the batch's
-// keys make kTargetGroups workgroups for each CU, and no fewer steps than cost
-// what joining a split costs.
+// A tile's keys in splits of at most `share` steps of 32, in whole granules;
+// unsplit where the partial results have no room.
 static void split_tile(KvSchedule &w, std::vector<KvAttnItem> &items, KvAttnItem it, uint32_t steps, uint32_t share,
                        uint32_t n_kv, uint32_t granule, uint64_t records) {
+  const uint32_t units = (steps + granule - 1) / granule;
   uint32_t splits = (steps + share - 1) / share;
   if (splits > 1 && w.records + (uint64_t)splits * n_kv * it.rows > records) splits = 1;
   if (splits > 1) w.join.push_back({it.row, it.first, it.rows, splits, (uint32_t)w.records});
-  const uint32_t units = (steps + granule - 1) / granule;
   for (uint32_t s = 0; s < splits; s++) {
     it.lo = (uint32_t)((uint64_t)units * s / splits) * granule;
     it.hi = std::min((uint32_t)((uint64_t)units * (s + 1) / splits) * granule, steps);
@@ -694,13 +717,33 @@ static void split_tile(KvSchedule &w, std::vector<KvAttnItem> &items, KvAttnItem
   }
 }
 
+// The share of steps that makes at most `groups` workgroups of the tiles, so
+// that all of them run at once (a last round of a few would take as long as a
+// whole one); with more tiles than that, the share of an even division.  No
+// fewer steps than `least`, below which joining the splits costs more.
+static uint32_t best_share(const std::vector<uint32_t> &steps, uint64_t groups, uint32_t least) {
+  uint64_t total = 0;
+  uint32_t longest = 1;
+  for (uint32_t n : steps) total += n, longest = std::max(longest, n);
+  groups = std::max<uint64_t>(groups, 1);
+  uint32_t lo = (uint32_t)std::max<uint64_t>((total + groups - 1) / groups, least), hi = std::max(longest, lo);
+  if (steps.size() >= groups) return lo;
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    uint64_t n = 0;
+    for (uint32_t x : steps) n += (x + mid - 1) / mid;
+    if (n <= groups) hi = mid; else lo = mid + 1;
+  }
+  return lo;
+}
+
 KvSchedule kv_schedule(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t n_kv, uint32_t head_dim, uint32_t n_cus,
                        uint64_t partial_floats) {
   KvSchedule w;
   const uint64_t records = std::min<uint64_t>(partial_floats / (head_dim + 4), 0xfffffffeu);
-  constexpr uint32_t kTokenGroups = 4, kTokenMin = 8, kChunkGroups = 3, kChunkMin = 8;
+  constexpr uint32_t kTokenGroups = 4, kTokenLeast = 8, kChunkLeast = 8;  // workgroups per CU, steps
+  const uint32_t chunk_groups = head_dim == 64 ? 3 : head_dim == 128 ? 2 : 1;
   if (!n_cus) n_cus = 256;
-  uint64_t token_steps = 0, chunk_steps = 0;
   auto tiles = [&](const KvSeq &q, auto &&f) {
     const uint32_t rows = q.n_new * group, wide = rows <= 16 ? 16 : kChunkRows;
     for (uint32_t first = 0; first < rows; first += wide) {
@@ -708,21 +751,18 @@ KvSchedule kv_schedule(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t 
       f(first, n, (keys + 31) / 32, rows <= 16);
     }
   };
+  std::vector<uint32_t> few_steps, many_steps;
   for (const KvSeq &q : seqs)
-    tiles(q, [&](uint32_t, uint32_t, uint32_t steps, bool few) { (few ? token_steps : chunk_steps) += steps; });
-  auto share = [&](uint64_t steps, uint32_t groups, uint32_t least) {
-    const uint64_t want = (uint64_t)n_cus * groups;
-    return (uint32_t)std::max<uint64_t>((steps * n_kv + want - 1) / want, least);
-  };
-  const uint32_t token_share = share(token_steps, kTokenGroups, kTokenMin);
-  const uint32_t chunk_share = share(chunk_steps, kChunkGroups, kChunkMin);
+    tiles(q, [&](uint32_t, uint32_t, uint32_t steps, bool few) { (few ? few_steps : many_steps).push_back(steps); });
+  const uint32_t few_share = best_share(few_steps, (uint64_t)n_cus * kTokenGroups / n_kv, kTokenLeast);
+  const uint32_t many_share = best_share(many_steps, (uint64_t)n_cus * chunk_groups / n_kv, kChunkLeast);
   for (const KvSeq &q : seqs)
     tiles(q, [&](uint32_t first, uint32_t n, uint32_t steps, bool few) {
-      KvAttnItem it{q.table, q.past, q.row, first, n, 0, 0, ~0u};
+      const KvAttnItem it{q.table, q.past, q.row, first, n, 0, 0, ~0u};
       if (few)
-        split_tile(w, n <= 8 ? w.narrow : w.tokens, it, steps, token_share, n_kv, 4, records);
+        split_tile(w, n <= 8 ? w.narrow : w.tokens, it, steps, few_share, n_kv, 1, records);
       else
-        split_tile(w, w.chunks, it, steps, chunk_share, n_kv, head_dim == 256 ? 1 : 2, records);
+        split_tile(w, w.chunks, it, steps, many_share, n_kv, head_dim == 256 ? 1 : 2, records);
     });
   // The longest first, so that the last workgroups are short ones.
   auto longer = [](const KvAttnItem &a, const KvAttnItem &b) { return a.hi - a.lo > b.hi - b.lo; };

@@ -102,13 +102,15 @@ struct KvGeometry {
   uint8_t *cache;
   const uint32_t *pages;
   uint32_t n_kv, page_blocks;  // blocks of a page and head
-  uint32_t page_magic;         // ceil(2^32 / page_blocks), 0 for pages of one block
-  // Block b of a sequence whose pages start at `table`, KV head `head`.  (The
-  // product is exact for b < 2^27 and page_blocks <= 32.)
+  uint32_t page_magic;         // ceil(2^31 / page_blocks)
+  // Block b of a sequence whose pages start at `table`, KV head `head`: a
+  // scalar load (the pages are constant while a kernel runs) where all three
+  // are uniform.  (The quotient is exact for b < 2^26 and page_blocks <= 32.)
   template <uint32_t BYTES>
   __device__ __forceinline__ uint8_t *block(uint32_t table, uint32_t b, uint32_t head) const {
-    const uint32_t p = page_magic ? __umulhi(b, page_magic) : b;
-    return cache + (((uint64_t)pages[table + p] * n_kv + head) * page_blocks + (b - p * page_blocks)) * BYTES;
+    using Constant = const __attribute__((address_space(4))) uint32_t;
+    const uint32_t p = __umulhi(2 * b, page_magic);
+    return cache + (((uint64_t)((Constant *)pages)[table + p] * n_kv + head) * page_blocks + (b - p * page_blocks)) * BYTES;
   }
 };
 
@@ -138,7 +140,7 @@ struct bch_kv_plan {
   bch::KvGeometry geometry(void *cache) const {
     const uint32_t blocks = shape.page_size / bch::kKvBlock;
     return {static_cast<uint8_t *>(cache), d_pages, shape.n_kv_heads, blocks,
-            blocks == 1 ? 0u : (uint32_t)(((1ull << 32) + blocks - 1) / blocks)};
+            ((1u << 31) + blocks - 1) / blocks};
   }
 };
 

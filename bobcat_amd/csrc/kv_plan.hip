@@ -14,7 +14,7 @@
 
 namespace bch {
 
-constexpr uint32_t kKvMaxPositions = 0x7fffffffu;
+constexpr uint32_t kKvMaxPositions = (1u << 30) - 1;  // of a sequence (KvGeometry::block)
 constexpr uint32_t kKvMaxTokens = 1u << 26;  // of a batch: packed rows and workgroups then stay below 2^31
 
 static int check_shape(const char *kernel, const bch_kv_shape *s) {
@@ -40,7 +40,7 @@ static int check_batch(const char *kernel, const bch_kv_shape *s, uint32_t n_seq
                        const uint32_t *n_new, const uint32_t *pages, uint64_t n_pages) {
   if (n_seqs && (!n_past || !n_new)) return fail(BCH_ERR_ARGUMENT, "%s: no lengths", kernel);
   if (n_pages && !pages) return fail(BCH_ERR_ARGUMENT, "%s: no pages", kernel);
-  if (n_pages > kKvMaxPositions) return fail(BCH_ERR_ARGUMENT, "%s: more than 2^31 - 1 pages", kernel);
+  if (n_pages > 0x7fffffffu) return fail(BCH_ERR_ARGUMENT, "%s: more than 2^31 - 1 pages", kernel);
   uint64_t want = 0, tokens = 0;
   for (uint32_t i = 0; i < n_seqs; i++) {
     const uint64_t len = (uint64_t)n_past[i] + n_new[i];

@@ -361,7 +361,7 @@ uint64_t bch_kv_page_bytes(const bch_kv_shape *shape);
  * heads in groups of at most 32 per KV head.  BCH_ERR_UNSUPPORTED_FORMAT and
  * BCH_ERR_ATTENTION_LIMITS for the shape; BCH_ERR_OUT_OF_BOUNDS for a page
  * past the cache's; BCH_ERR_ARGUMENT for a list of another length, a sequence
- * of 2^31 positions, or a page that receives tokens and is named twice in the
+ * of 2^30 positions, more than 2^26 new tokens, or a page that receives tokens and is named twice in the
  * batch (pages that are only read may be shared by sequences). */
 int bch_kv_plan_check(const bch_kv_shape *shape, uint32_t n_heads, uint32_t n_seqs, const uint32_t *n_past,
                       const uint32_t *n_new, const uint32_t *pages, uint64_t n_pages);

@@ -46,7 +46,7 @@ def test_batches_that_are_refused():
     refused("Argument", pages=((4,),))
     refused("Argument", pages=((4, 7, 8),))
     refused("Argument", past=(0,), new=(0,), pages=((1,),))
-    refused("Argument", past=(0x7FFFFFFF,), new=(1,), pages=((),))
+    refused("Argument", past=(0x3FFFFFFF,), new=(1,), pages=((),))
     refused("Argument", past=(0xFFFFFFFF,), new=(0xFFFFFFFF,), pages=((),))
     # A page that receives tokens, named twice: by two sequences, by one, and as another's prefix.
     refused("Argument", past=(40, 0), new=(3, 5), pages=((4, 7), (7,)))
