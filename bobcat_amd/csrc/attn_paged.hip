@@ -685,14 +685,34 @@ __global__ __launch_bounds__(256) void k_attn_join(const KvJoinItem *__restrict_
   if (row >= it.rows) return;
   const uint64_t apart = (uint64_t)n_kv * it.rows * (HD + 4);
   const float *p = to.partials + ((uint64_t)it.part + kv * it.rows + row) * (HD + 4);
+  constexpr uint32_t N = 8;  // records in flight
   float top = -INFINITY, sum = 0.f;
-  for (uint32_t s = 0; s < it.splits; s++) top = fmaxf(top, p[s * apart + HD]);
   float4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (uint32_t s = 0; s < it.splits; s++) {
-    const float m = p[s * apart + HD], f = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
-    const float4 x = *reinterpret_cast<const float4 *>(p + s * apart + d);
-    acc.x = fmaf(x.x, f, acc.x), acc.y = fmaf(x.y, f, acc.y), acc.z = fmaf(x.z, f, acc.z), acc.w = fmaf(x.w, f, acc.w);
-    sum = fmaf(p[s * apart + HD + 1], f, sum);
+  for (uint32_t s0 = 0; s0 < it.splits; s0 += N) {
+    float2 ml[N];
+    float4 x[N];
+#pragma unroll
+    for (uint32_t j = 0; j < N; j++) {
+      const float *r = p + min(s0 + j, it.splits - 1) * apart;
+      ml[j] = *reinterpret_cast<const float2 *>(r + HD);
+      x[j] = *reinterpret_cast<const float4 *>(r + d);
+    }
+    float next = top;
+#pragma unroll
+    for (uint32_t j = 0; j < N; j++) next = fmaxf(next, ml[j].x);
+    auto weight = [&](float m) { return m == next ? 1.f : __builtin_amdgcn_exp2f(m - next); };
+    const float f0 = weight(top);
+    top = next;
+    sum *= f0;
+    acc.x *= f0, acc.y *= f0, acc.z *= f0, acc.w *= f0;
+#pragma unroll
+    for (uint32_t j = 0; j < N; j++) {
+      if (s0 + j >= it.splits) break;
+      const float f = weight(ml[j].x);
+      acc.x = fmaf(x[j].x, f, acc.x), acc.y = fmaf(x[j].y, f, acc.y);
+      acc.z = fmaf(x[j].z, f, acc.z), acc.w = fmaf(x[j].w, f, acc.w);
+      sum = fmaf(ml[j].y, f, sum);
+    }
   }
   const uint32_t at = it.first + row;
   put_row<HD>(to, ~0u, 0, it.row + at / group, kv * group + at % group, d, acc, top, sum);
