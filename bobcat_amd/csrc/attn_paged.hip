@@ -677,43 +677,65 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : HD == 128 ? 2 : 1) void k_attn_
                   float4{o[b][4 * q4], o[b][4 * q4 + 1], o[b][4 * q4 + 2], o[b][4 * q4 + 3]}, ref, l);
 }
 
-// The rows of tiles whose keys were split, from the splits' records.
+// The rows of tiles whose keys were split, from the splits' records.  HD / 4
+// threads read a record; `parts` (a power of two) such groups have every
+// parts-th of a row's records each, eight in flight, and meet in LDS.
 template <uint32_t HD>
-__global__ __launch_bounds__(256) void k_attn_join(const KvJoinItem *__restrict__ items, uint32_t n_kv, uint32_t group, AttnOut to) {
+__global__ __launch_bounds__(256) void k_attn_join(const KvJoinItem *__restrict__ items, uint32_t n_kv, uint32_t group,
+                                                   uint32_t parts, AttnOut to) {
+  constexpr uint32_t N = 8, WIDE = HD / 4, GROUPS = 256 / WIDE;
+  __shared__ float4 acc_s[GROUPS][WIDE];
+  __shared__ float2 ml_s[GROUPS];
   const KvJoinItem it = items[blockIdx.x];
-  const uint32_t kv = blockIdx.y, i = blockIdx.z * 256 + threadIdx.x, row = i / (HD / 4), d = 4 * (i % (HD / 4));
-  if (row >= it.rows) return;
+  const uint32_t kv = blockIdx.y, lane = threadIdx.x % WIDE, mine = threadIdx.x / WIDE, part = mine % parts, d = 4 * lane;
+  const uint32_t row = blockIdx.z * (GROUPS / parts) + mine / parts;
+  if (blockIdx.z * (GROUPS / parts) >= it.rows) return;
   const uint64_t apart = (uint64_t)n_kv * it.rows * (HD + 4);
-  const float *p = to.partials + ((uint64_t)it.part + kv * it.rows + row) * (HD + 4);
-  constexpr uint32_t N = 8;  // records in flight
+  const float *p = to.partials + ((uint64_t)it.part + kv * it.rows + min(row, it.rows - 1)) * (HD + 4);
   float top = -INFINITY, sum = 0.f;
   float4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (uint32_t s0 = 0; s0 < it.splits; s0 += N) {
+  // The weight of a reference m under another that is no smaller.
+  auto weight = [](float m, float under) { return m == under ? 1.f : __builtin_amdgcn_exp2f(m - under); };
+  auto add = [&](float f, float4 x, float l) {
+    acc.x = fmaf(x.x, f, acc.x), acc.y = fmaf(x.y, f, acc.y), acc.z = fmaf(x.z, f, acc.z), acc.w = fmaf(x.w, f, acc.w);
+    sum = fmaf(l, f, sum);
+  };
+  for (uint32_t s0 = part; s0 < it.splits; s0 += N * parts) {
     float2 ml[N];
     float4 x[N];
 #pragma unroll
     for (uint32_t j = 0; j < N; j++) {
-      const float *r = p + min(s0 + j, it.splits - 1) * apart;
+      const float *r = p + min(s0 + j * parts, it.splits - 1) * apart;
       ml[j] = *reinterpret_cast<const float2 *>(r + HD);
       x[j] = *reinterpret_cast<const float4 *>(r + d);
     }
     float next = top;
 #pragma unroll
     for (uint32_t j = 0; j < N; j++) next = fmaxf(next, ml[j].x);
-    auto weight = [&](float m) { return m == next ? 1.f : __builtin_amdgcn_exp2f(m - next); };
-    const float f0 = weight(top);
+    const float f0 = weight(top, next);
     top = next;
     sum *= f0;
     acc.x *= f0, acc.y *= f0, acc.z *= f0, acc.w *= f0;
 #pragma unroll
     for (uint32_t j = 0; j < N; j++) {
-      if (s0 + j >= it.splits) break;
-      const float f = weight(ml[j].x);
-      acc.x = fmaf(x[j].x, f, acc.x), acc.y = fmaf(x[j].y, f, acc.y);
-      acc.z = fmaf(x[j].z, f, acc.z), acc.w = fmaf(x[j].w, f, acc.w);
-      sum = fmaf(ml[j].y, f, sum);
+      if (s0 + j * parts >= it.splits) break;
+      add(weight(ml[j].x, top), x[j], ml[j].y);
     }
   }
+  if (parts > 1) {
+    acc_s[mine][lane] = acc;
+    if (lane == 0) ml_s[mine] = {top, sum};
+    __syncthreads();
+    if (part) return;
+    float all = top;
+    for (uint32_t j = 1; j < parts; j++) all = fmaxf(all, ml_s[mine + j].x);
+    const float f0 = weight(top, all);
+    acc.x *= f0, acc.y *= f0, acc.z *= f0, acc.w *= f0;
+    sum *= f0;
+    for (uint32_t j = 1; j < parts; j++) add(weight(ml_s[mine + j].x, all), acc_s[mine + j][lane], ml_s[mine + j].y);
+    top = all;
+  }
+  if (row >= it.rows) return;
   const uint32_t at = it.first + row;
   put_row<HD>(to, ~0u, 0, it.row + at / group, kv * group + at % group, d, acc, top, sum);
 }
@@ -761,21 +783,45 @@ KvSchedule kv_schedule(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t 
                        uint64_t partial_floats) {
   KvSchedule w;
   const uint64_t records = std::min<uint64_t>(partial_floats / (head_dim + 4), 0xfffffffeu);
-  constexpr uint32_t kTokenGroups = 4, kTokenLeast = 8, kChunkLeast = 8;  // workgroups per CU, steps
-  const uint32_t chunk_groups = head_dim == 64 ? 3 : head_dim == 128 ? 2 : 1;
   if (!n_cus) n_cus = 256;
+  // Which tiles.  Up to 32 rows take narrow tiles, which read the keys again
+  // for every 16 rows (twelve sequences of about 2,000 keys, 20 and 32 rows,
+  // heads of 64: 23 and 24 us against 26 and 26 in wide ones; of 256: 27 and 37
+  // against 44 and 46).  Up to 128 rows do while the batch is small, because a
+  // wide tile's few waves then wait for one another (1,000 keys, 96 rows, heads
+  // of 128: 11 us against 20; at ten times the keys they are level).
+  constexpr uint32_t kFewRows = 32;
+  constexpr uint64_t kSmallBatch = 1u << 20;  // narrow tiles x steps x KV heads x head_dim
+  uint64_t narrow_work = 0;
+  for (const KvSeq &q : seqs) {
+    const uint64_t rows = (uint64_t)q.n_new * group;
+    if (rows > 16 && rows <= kChunkRows) narrow_work += (rows + 15) / 16 * ((q.past + q.n_new + 31) / 32) * n_kv * head_dim;
+  }
+  const uint32_t few_rows = narrow_work <= kSmallBatch ? kChunkRows : kFewRows;
   auto tiles = [&](const KvSeq &q, auto &&f) {
-    const uint32_t rows = q.n_new * group, wide = rows <= 16 ? 16 : kChunkRows;
+    const uint32_t rows = q.n_new * group, wide = rows <= few_rows ? 16 : kChunkRows;
     for (uint32_t first = 0; first < rows; first += wide) {
       const uint32_t n = std::min(wide, rows - first), keys = q.past + (first + n - 1) / group + 1;
-      f(first, n, (keys + 31) / 32, rows <= 16);
+      f(first, n, (keys + 31) / 32, rows <= few_rows);
     }
   };
   std::vector<uint32_t> few_steps, many_steps;
+  uint32_t longest = 0;
   for (const KvSeq &q : seqs)
-    tiles(q, [&](uint32_t, uint32_t, uint32_t steps, bool few) { (few ? few_steps : many_steps).push_back(steps); });
-  const uint32_t few_share = best_share(few_steps, (uint64_t)n_cus * kTokenGroups / n_kv, kTokenLeast);
-  const uint32_t many_share = best_share(many_steps, (uint64_t)n_cus * chunk_groups / n_kv, kChunkLeast);
+    tiles(q, [&](uint32_t, uint32_t, uint32_t steps, bool few) {
+      (few ? few_steps : many_steps).push_back(steps);
+      if (few) longest = std::max(longest, steps);
+    });
+  // Narrow tiles: splits of eight steps (two a wave) are as short as pays, and
+  // a join (about 2.5 us) pays from 24 steps on with heads of 64, 19 of 128, 16
+  // of 256 (300 keys of 64: 5.6 us unsplit, 7.6 split; 2,000: 14.2 and 9.0).
+  // Four workgroups a CU; two to eight measured within 5%.
+  const uint32_t unsplit = 14 + 640 / head_dim;
+  const uint32_t few_share = best_share(few_steps, (uint64_t)n_cus * 4 / n_kv, longest <= unsplit ? unsplit : 8);
+  // Wide tiles: what the registers let run at once, and four trips of the loop
+  // at least (64 queries over 1,000 keys of 256: 28 us, with eight 34).
+  const uint32_t many_share = best_share(many_steps, (uint64_t)n_cus * (head_dim == 64 ? 3 : head_dim == 128 ? 2 : 1) / n_kv,
+                                         head_dim == 256 ? 4 : 8);
   for (const KvSeq &q : seqs)
     tiles(q, [&](uint32_t first, uint32_t n, uint32_t steps, bool few) {
       const KvAttnItem it{q.table, q.past, q.row, first, n, 0, 0, ~0u};
@@ -825,9 +871,14 @@ extern "C" int bch_attention_paged(bch_ctx *ctx, const bch_kv_plan *plan, bch_vi
         k_attn_tokens<F, HD, 16><<<plan->n_tiles16 * n_kv, 256, 0, st>>>(geo, plan->d_tiles16, qp, q_stride, to, group, c2);
       if (plan->n_tiles8)
         k_attn_tokens<F, HD, 8><<<plan->n_tiles8 * n_kv, 256, 0, st>>>(geo, plan->d_tiles8, qp, q_stride, to, group, c2);
-      if (plan->n_join)
-        k_attn_join<HD><<<dim3(plan->n_join, n_kv, div_ceil(plan->join_rows * (HD / 4), 256)), 256, 0, st>>>(
-            plan->d_join, n_kv, group, to);
+      if (plan->n_join) {
+        // Up to eight records each in one round of loads.
+        constexpr uint32_t kGroups = 1024 / HD;
+        uint32_t parts = 1;
+        while (parts < kGroups && parts * 8 < plan->join_splits) parts *= 2;
+        k_attn_join<HD><<<dim3(plan->n_join, n_kv, div_ceil(plan->join_rows * parts, kGroups)), 256, 0, st>>>(
+            plan->d_join, n_kv, group, parts, to);
+      }
     });
   });
 }

@@ -135,7 +135,7 @@ struct bch_kv_plan {
   uint32_t n_store = 0;
   const bch::KvAttnItem *d_tiles8 = nullptr, *d_tiles16 = nullptr, *d_chunks = nullptr;
   const bch::KvJoinItem *d_join = nullptr;
-  uint32_t n_tiles8 = 0, n_tiles16 = 0, n_chunks = 0, n_join = 0, join_rows = 0;
+  uint32_t n_tiles8 = 0, n_tiles16 = 0, n_chunks = 0, n_join = 0, join_rows = 0, join_splits = 0;  // the most rows and splits of a joined tile
 
   bch::KvGeometry geometry(void *cache) const {
     const uint32_t blocks = shape.page_size / bch::kKvBlock;

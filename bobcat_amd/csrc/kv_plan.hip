@@ -177,8 +177,11 @@ static int plan_set(bch_kv_plan *plan, uint32_t n_seqs, const uint32_t *n_past, 
   plan->n_tiles16 = (uint32_t)work.tokens.size();
   plan->n_chunks = (uint32_t)work.chunks.size();
   plan->n_join = (uint32_t)work.join.size();
-  plan->join_rows = 0;
-  for (const KvJoinItem &j : work.join) plan->join_rows = std::max(plan->join_rows, j.rows);
+  plan->join_rows = plan->join_splits = 0;
+  for (const KvJoinItem &j : work.join) {
+    plan->join_rows = std::max(plan->join_rows, j.rows);
+    plan->join_splits = std::max(plan->join_splits, j.splits);
+  }
   plan->ready = true;
   return BCH_OK;
 }
