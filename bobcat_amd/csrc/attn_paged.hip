@@ -106,23 +106,32 @@ __device__ __forceinline__ void put_row(const AttnOut &o, uint32_t part, uint32_
   }
 }
 
+// Workgroups of a CU that the registers let run at once.
+constexpr uint32_t token_groups(uint32_t format, uint32_t hd) {
+  return format == BCH_KV_F16 ? (hd == 64 ? 4 : hd == 128 ? 2 : 1) : (hd == 64 ? 4 : hd == 128 ? 3 : 2);
+}
+constexpr uint32_t chunk_groups(uint32_t hd) { return hd == 64 ? 3 : hd == 128 ? 2 : 1; }
+
 // --- at most 16 packed rows ---------------------------------------------------
 
 // ROWS 8: the high parts of the queries and probabilities are the operands'
 // columns 0..7, the low parts columns 8..15, so one MFMA does both and the
 // halves of O are added once at the end.  ROWS 16: two MFMAs each.
 template <uint32_t FORMAT, uint32_t HD, uint32_t ROWS>
-__global__ __launch_bounds__(256) void k_attn_tokens(KvGeometry g, const KvAttnItem *__restrict__ items,
-                                                     const float *__restrict__ q, uint32_t q_stride, AttnOut to,
-                                                     uint32_t group, float c2) {
+__global__ __launch_bounds__(256, token_groups(FORMAT, HD)) void k_attn_tokens(
+    KvGeometry g, const KvAttnItem *__restrict__ items,
+                                                                       const uint32_t *__restrict__ starts,
+                                                                       const float *__restrict__ q, uint32_t q_stride,
+                                                                       AttnOut to, uint32_t group, float c2) {
   constexpr bool PACK = ROWS == 8, QUANT = FORMAT != BCH_KV_F16;
   constexpr uint32_t SIZE = kv_elem_bytes(FORMAT), BYTES = kv_block_bytes(FORMAT, HD), PART = kKvBlock * HD * SIZE;
   constexpr uint32_t NL = PART / 1024;  // KB of a block's keys, and of its values
   constexpr uint32_t KS = HD / 32, OB = HD / 16, M = 4 / SIZE;
   __shared__ __align__(16) float o_s[4][ROWS][HD];
   __shared__ float m_s[4][ROWS], l_s[4][ROWS];
-  const uint32_t kv = blockIdx.x % g.n_kv;
-  const KvAttnItem it = items[blockIdx.x / g.n_kv];
+  const uint32_t kv = blockIdx.x % g.n_kv, end = starts[blockIdx.x / g.n_kv + 1];
+  for (uint32_t item = starts[blockIdx.x / g.n_kv]; item < end; item++) {
+  const KvAttnItem it = items[item];
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
   const uint32_t col = lane % 16, quad = lane / 16;
   const uint32_t r = PACK ? col % 8 : col, packed = it.first + min(r, it.rows - 1);
@@ -363,6 +372,8 @@ __global__ __launch_bounds__(256) void k_attn_tokens(KvGeometry g, const KvAttnI
     const uint32_t at = it.first + row;
     put_row<HD>(to, it.part, kv * it.rows + row, it.row + at / group, kv * group + at % group, d, acc, top, sum);
   }
+  __syncthreads();  // the next item's sums come to the same place
+  }
 }
 
 // --- more rows ------------------------------------------------------------------
@@ -372,9 +383,9 @@ constexpr uint32_t kChunkKeys = HD == 256 ? 32 : 64;  // keys of a step
 constexpr uint32_t kChunkRows = 128;
 
 template <uint32_t FORMAT, uint32_t HD>
-__global__ __launch_bounds__(256, HD == 64 ? 3 : HD == 128 ? 2 : 1) void k_attn_chunk(
-    KvGeometry g, const KvAttnItem *__restrict__ items, const float *__restrict__ q, uint32_t q_stride, AttnOut to,
-    uint32_t group, float c2) {
+__global__ __launch_bounds__(256, chunk_groups(HD)) void k_attn_chunk(
+    KvGeometry g, const KvAttnItem *__restrict__ items, const uint32_t *__restrict__ starts, const float *__restrict__ q,
+    uint32_t q_stride, AttnOut to, uint32_t group, float c2) {
   constexpr bool QUANT = FORMAT != BCH_KV_F16;
   constexpr uint32_t SIZE = kv_elem_bytes(FORMAT), BYTES = kv_block_bytes(FORMAT, HD), PART = kKvBlock * HD * SIZE;
   constexpr uint32_t KEYS = kChunkKeys<HD>, KS = HD / 16, OB = HD / 32, M = 4 / SIZE;
@@ -386,8 +397,9 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : HD == 128 ? 2 : 1) void k_attn_
   __shared__ __align__(16) float s_s[2][2][KEYS];         // the keys' and the values' scales
   __shared__ float top_s[2][KEYS / kKvBlock];             // the largest scale_log of each block's values
   __shared__ uint32_t odd_s[2];
-  const uint32_t kv = blockIdx.x % g.n_kv;
-  const KvAttnItem it = items[blockIdx.x / g.n_kv];
+  const uint32_t kv = blockIdx.x % g.n_kv, end = starts[blockIdx.x / g.n_kv + 1];
+  for (uint32_t item = starts[blockIdx.x / g.n_kv]; item < end; item++) {
+  const KvAttnItem it = items[item];
   const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64) & 3, lane = tid % 64;
   const uint32_t col = lane % 32, half_id = lane / 32;
   const bool active = 32 * wave < it.rows;
@@ -665,16 +677,19 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : HD == 128 ? 2 : 1) void k_attn_
       }
     }
   }
-  if (!active) return;
+  // (Every wave has passed the last step's barrier: the next item may write to
+  // the stages.)
   l += __shfl_xor(l, 32, 64);
-  if (col >= rows) return;
-  const float ref = lazy == kUnset ? -INFINITY : m;
+  if (active && col < rows) {
+    const float ref = lazy == kUnset ? -INFINITY : m;
 #pragma unroll
-  for (uint32_t b = 0; b < OB; b++)
+    for (uint32_t b = 0; b < OB; b++)
 #pragma unroll
-    for (int q4 = 0; q4 < 4; q4++)
-      put_row<HD>(to, it.part, kv * it.rows + (packed - it.first), it.row + token, head, 32 * b + 8 * q4 + 4 * half_id,
-                  float4{o[b][4 * q4], o[b][4 * q4 + 1], o[b][4 * q4 + 2], o[b][4 * q4 + 3]}, ref, l);
+      for (int q4 = 0; q4 < 4; q4++)
+        put_row<HD>(to, it.part, kv * it.rows + (packed - it.first), it.row + token, head, 32 * b + 8 * q4 + 4 * half_id,
+                    float4{o[b][4 * q4], o[b][4 * q4 + 1], o[b][4 * q4 + 2], o[b][4 * q4 + 3]}, ref, l);
+  }
+  }
 }
 
 // The rows of tiles whose keys were split, from the splits' records.  HD / 4
@@ -742,45 +757,67 @@ __global__ __launch_bounds__(256) void k_attn_join(const KvJoinItem *__restrict_
 
 // --- the work of a batch ----------------------------------------------------------
 
-// A tile's keys in splits of at most `share` steps of 32, in whole granules;
-// unsplit where the partial results have no room.
-static void split_tile(KvSchedule &w, std::vector<KvAttnItem> &items, KvAttnItem it, uint32_t steps, uint32_t share,
-                       uint32_t n_kv, uint32_t granule, uint64_t records) {
-  const uint32_t units = (steps + granule - 1) / granule;
-  uint32_t splits = (steps + share - 1) / share;
-  if (splits > 1 && w.records + (uint64_t)splits * n_kv * it.rows > records) splits = 1;
-  if (splits > 1) w.join.push_back({it.row, it.first, it.rows, splits, (uint32_t)w.records});
-  for (uint32_t s = 0; s < splits; s++) {
-    it.lo = (uint32_t)((uint64_t)units * s / splits) * granule;
-    it.hi = std::min((uint32_t)((uint64_t)units * (s + 1) / splits) * granule, steps);
-    it.part = splits > 1 ? (uint32_t)w.records : ~0u;
-    if (splits > 1) w.records += (uint64_t)n_kv * it.rows;
-    items.push_back(it);
-  }
-}
+// Tiles whose rows are dealt out, with their keys in steps of 32.
+struct Tile {
+  KvAttnItem it;
+  uint32_t steps;
+};
 
-// The share of steps that makes at most `groups` workgroups of the tiles, so
-// that all of them run at once (a last round of a few would take as long as a
-// whole one); with more tiles than that, the share of an even division.  No
-// fewer steps than `least`, below which joining the splits costs more.
-static uint32_t best_share(const std::vector<uint32_t> &steps, uint64_t groups, uint32_t least) {
+// Deals the tiles' steps to at most `most` workgroups for each KV head in equal
+// shares, cutting a tile where a share ends: all workgroups run at once and end
+// together, and a tile is cut no more often than that takes.  A piece costs
+// kStart steps besides its own (its queries, its results) and has `least` at
+// least; with `whole` no tile is cut.  Tiles whose pieces' records have no room
+// stay whole.
+static void deal(KvSchedule &w, KvWork &work, std::vector<Tile> &tiles, uint64_t most, uint32_t least, bool whole,
+                 uint32_t n_kv, uint32_t granule, uint64_t records) {
+  constexpr uint64_t kStart = 4;
+  work.starts.push_back(0);
+  if (tiles.empty()) return;
   uint64_t total = 0;
-  uint32_t longest = 1;
-  for (uint32_t n : steps) total += n, longest = std::max(longest, n);
-  groups = std::max<uint64_t>(groups, 1);
-  uint32_t lo = (uint32_t)std::max<uint64_t>((total + groups - 1) / groups, least), hi = std::max(longest, lo);
-  if (steps.size() >= groups) return lo;
-  while (lo < hi) {
-    const uint32_t mid = lo + (hi - lo) / 2;
-    uint64_t n = 0;
-    for (uint32_t x : steps) n += (x + mid - 1) / mid;
-    if (n <= groups) hi = mid; else lo = mid + 1;
+  for (const Tile &t : tiles) total += t.steps + kStart;
+  most = std::max<uint64_t>(most, 1);
+  uint64_t groups = whole ? std::min<uint64_t>(most, tiles.size()) : std::min(most, std::max<uint64_t>(total / (least + kStart), 1));
+  const uint64_t share = std::max<uint64_t>((total + kStart * groups + groups - 1) / groups, least + kStart);
+  uint64_t room = share, dealt = 1;  // of the open workgroup; workgroups opened
+  auto close = [&]() {
+    if (work.starts.back() == work.items.size() || dealt == groups) return;
+    work.starts.push_back((uint32_t)work.items.size());
+    room = share;
+    dealt++;
+  };
+  for (Tile &t : tiles) {
+    const uint64_t rows = (uint64_t)n_kv * t.it.rows;
+    const size_t first = work.items.size();
+    for (uint32_t at = 0; at < t.steps;) {
+      const uint32_t left = t.steps - at;
+      // No room for a piece: the next workgroup's.
+      if (room < left + kStart && (whole || room < least + kStart)) close();
+      uint32_t take = left;
+      if (!whole && dealt < groups && room < left + kStart && left >= 2 * least && w.records + 2 * rows <= records) {
+        take = std::max((uint32_t)(room > kStart ? room - kStart : 0), least);
+        take = std::min(take, left - least) / granule * granule;
+        take = std::max(take, granule);
+      }
+      t.it.lo = at;
+      t.it.hi = at + take;
+      t.it.part = (uint32_t)w.records;
+      if (take < t.steps) w.records += rows;
+      work.items.push_back(t.it);
+      at += take;
+      room -= std::min<uint64_t>(room, take + kStart);
+    }
+    const uint32_t pieces = (uint32_t)(work.items.size() - first);
+    if (pieces == 1)
+      work.items[first].part = ~0u;
+    else
+      w.join.push_back({t.it.row, t.it.first, t.it.rows, pieces, work.items[first].part});
   }
-  return lo;
+  work.starts.push_back((uint32_t)work.items.size());
 }
 
-KvSchedule kv_schedule(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t n_kv, uint32_t head_dim, uint32_t n_cus,
-                       uint64_t partial_floats) {
+KvSchedule kv_schedule(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t n_kv, uint32_t format, uint32_t head_dim,
+                       uint32_t n_cus, uint64_t partial_floats) {
   KvSchedule w;
   const uint64_t records = std::min<uint64_t>(partial_floats / (head_dim + 4), 0xfffffffeu);
   if (!n_cus) n_cus = 256;
@@ -798,41 +835,37 @@ KvSchedule kv_schedule(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t 
     if (rows > 16 && rows <= kChunkRows) narrow_work += (rows + 15) / 16 * ((q.past + q.n_new + 31) / 32) * n_kv * head_dim;
   }
   const uint32_t few_rows = narrow_work <= kSmallBatch ? kChunkRows : kFewRows;
-  auto tiles = [&](const KvSeq &q, auto &&f) {
-    const uint32_t rows = q.n_new * group, wide = rows <= few_rows ? 16 : kChunkRows;
-    for (uint32_t first = 0; first < rows; first += wide) {
-      const uint32_t n = std::min(wide, rows - first), keys = q.past + (first + n - 1) / group + 1;
-      f(first, n, (keys + 31) / 32, rows <= few_rows);
-    }
-  };
-  std::vector<uint32_t> few_steps, many_steps;
+  std::vector<Tile> narrow, tokens, chunks;
   uint32_t longest = 0;
-  for (const KvSeq &q : seqs)
-    tiles(q, [&](uint32_t, uint32_t, uint32_t steps, bool few) {
-      (few ? few_steps : many_steps).push_back(steps);
-      if (few) longest = std::max(longest, steps);
-    });
-  // Narrow tiles: splits of eight steps (two a wave) are as short as pays, and
+  uint64_t narrow_steps = 0, token_steps = 0;
+  for (const KvSeq &q : seqs) {
+    const uint32_t rows = q.n_new * group;
+    const bool few = rows <= few_rows;
+    for (uint32_t first = 0; first < rows; first += few ? 16 : kChunkRows) {
+      const uint32_t n = std::min(few ? 16 : kChunkRows, rows - first), keys = q.past + (first + n - 1) / group + 1;
+      const Tile t{{q.table, q.past, q.row, first, n, 0, 0, ~0u}, (keys + 31) / 32};
+      (!few ? chunks : n <= 8 ? narrow : tokens).push_back(t);
+      if (few) {
+        longest = std::max(longest, t.steps);
+        (n <= 8 ? narrow_steps : token_steps) += t.steps;
+      }
+    }
+  }
+  // A few tiles of 8 rows join those of 16 in one launch.
+  if (narrow_steps < token_steps) {
+    tokens.insert(tokens.end(), narrow.begin(), narrow.end());
+    narrow.clear();
+  }
+  // Narrow tiles: pieces of eight steps (two a wave) are as short as pays, and
   // a join (about 2.5 us) pays from 24 steps on with heads of 64, 19 of 128, 16
-  // of 256 (300 keys of 64: 5.6 us unsplit, 7.6 split; 2,000: 14.2 and 9.0).
-  // Four workgroups a CU; two to eight measured within 5%.
+  // of 256 (300 keys of 64: 5.6 us whole, 7.6 cut; 2,000: 14.2 and 9.0).
   const uint32_t unsplit = 14 + 640 / head_dim;
-  const uint32_t few_share = best_share(few_steps, (uint64_t)n_cus * 4 / n_kv, longest <= unsplit ? unsplit : 8);
-  // Wide tiles: what the registers let run at once, and four trips of the loop
-  // at least (64 queries over 1,000 keys of 256: 28 us, with eight 34).
-  const uint32_t many_share = best_share(many_steps, (uint64_t)n_cus * (head_dim == 64 ? 3 : head_dim == 128 ? 2 : 1) / n_kv,
-                                         head_dim == 256 ? 4 : 8);
-  for (const KvSeq &q : seqs)
-    tiles(q, [&](uint32_t first, uint32_t n, uint32_t steps, bool few) {
-      const KvAttnItem it{q.table, q.past, q.row, first, n, 0, 0, ~0u};
-      if (few)
-        split_tile(w, n <= 8 ? w.narrow : w.tokens, it, steps, few_share, n_kv, 1, records);
-      else
-        split_tile(w, w.chunks, it, steps, many_share, n_kv, head_dim == 256 ? 1 : 2, records);
-    });
-  // The longest first, so that the last workgroups are short ones.
-  auto longer = [](const KvAttnItem &a, const KvAttnItem &b) { return a.hi - a.lo > b.hi - b.lo; };
-  for (auto *items : {&w.narrow, &w.tokens, &w.chunks}) std::stable_sort(items->begin(), items->end(), longer);
+  const uint64_t few_groups = (uint64_t)n_cus * token_groups(format, head_dim) / n_kv;
+  deal(w, w.tiles8, narrow, few_groups, 8, longest <= unsplit, n_kv, 1, records);
+  deal(w, w.tiles16, tokens, few_groups, 8, longest <= unsplit, n_kv, 1, records);
+  // Wide tiles: four trips of the loop at least (64 queries over 1,000 keys of
+  // 256: 28 us, with eight 34).
+  deal(w, w.chunks, chunks, (uint64_t)n_cus * chunk_groups(head_dim) / n_kv, head_dim == 256 ? 4 : 8, false, n_kv, head_dim == 256 ? 1 : 2, records);
   return w;
 }
 
@@ -866,11 +899,13 @@ extern "C" int bch_attention_paged(bch_ctx *ctx, const bch_kv_plan *plan, bch_vi
     const float c2 = (float)(1.44269504088896340736 / std::sqrt((double)s.head_dim));
     kv_dispatch(s.format, s.head_dim, [&](auto format, auto hd) {
       constexpr uint32_t F = decltype(format)::value, HD = decltype(hd)::value;
-      if (plan->n_chunks) k_attn_chunk<F, HD><<<plan->n_chunks * n_kv, 256, 0, st>>>(geo, plan->d_chunks, qp, q_stride, to, group, c2);
-      if (plan->n_tiles16)
-        k_attn_tokens<F, HD, 16><<<plan->n_tiles16 * n_kv, 256, 0, st>>>(geo, plan->d_tiles16, qp, q_stride, to, group, c2);
-      if (plan->n_tiles8)
-        k_attn_tokens<F, HD, 8><<<plan->n_tiles8 * n_kv, 256, 0, st>>>(geo, plan->d_tiles8, qp, q_stride, to, group, c2);
+      const bch_kv_plan::Work &c = plan->chunks, &t16 = plan->tiles16, &t8 = plan->tiles8;
+      if (c.groups)
+        k_attn_chunk<F, HD><<<c.groups * n_kv, 256, 0, st>>>(geo, c.items, c.starts, qp, q_stride, to, group, c2);
+      if (t16.groups)
+        k_attn_tokens<F, HD, 16><<<t16.groups * n_kv, 256, 0, st>>>(geo, t16.items, t16.starts, qp, q_stride, to, group, c2);
+      if (t8.groups)
+        k_attn_tokens<F, HD, 8><<<t8.groups * n_kv, 256, 0, st>>>(geo, t8.items, t8.starts, qp, q_stride, to, group, c2);
       if (plan->n_join) {
         // Up to eight records each in one round of loads.
         constexpr uint32_t kGroups = 1024 / HD;

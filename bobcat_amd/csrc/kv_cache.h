@@ -88,15 +88,21 @@ struct KvAttnItem {
 struct KvJoinItem {
   uint32_t row, first, rows, splits, part;
 };
+// Items dealt to workgroups: workgroup w of a KV head takes items starts[w] ..
+// starts[w + 1].
+struct KvWork {
+  std::vector<KvAttnItem> items;
+  std::vector<uint32_t> starts;
+};
 struct KvSchedule {
-  std::vector<KvAttnItem> narrow, tokens, chunks;  // of at most 8, at most 16, and up to 128 rows
+  KvWork tiles8, tiles16, chunks;  // tiles of at most 8, at most 16, and up to 128 rows
   std::vector<KvJoinItem> join;
   uint64_t records = 0;
 };
 // attn_paged.hip: the attention's work of a batch, with no more partial
 // results than partial_floats hold.
-KvSchedule kv_schedule(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t n_kv, uint32_t head_dim, uint32_t n_cus,
-                       uint64_t partial_floats);
+KvSchedule kv_schedule(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t n_kv, uint32_t format, uint32_t head_dim,
+                       uint32_t n_cus, uint64_t partial_floats);
 
 struct KvGeometry {
   uint8_t *cache;
@@ -133,9 +139,13 @@ struct bch_kv_plan {
   const uint32_t *d_pages = nullptr;
   const bch::KvStoreItem *d_store = nullptr;
   uint32_t n_store = 0;
-  const bch::KvAttnItem *d_tiles8 = nullptr, *d_tiles16 = nullptr, *d_chunks = nullptr;
+  struct Work {
+    const bch::KvAttnItem *items = nullptr;
+    const uint32_t *starts = nullptr;
+    uint32_t groups = 0;  // workgroups for each KV head
+  } tiles8, tiles16, chunks;
   const bch::KvJoinItem *d_join = nullptr;
-  uint32_t n_tiles8 = 0, n_tiles16 = 0, n_chunks = 0, n_join = 0, join_rows = 0, join_splits = 0;  // the most rows and splits of a joined tile
+  uint32_t n_join = 0, join_rows = 0, join_splits = 0;  // the most rows and splits of a joined tile
 
   bch::KvGeometry geometry(void *cache) const {
     const uint32_t blocks = shape.page_size / bch::kKvBlock;

@@ -129,13 +129,16 @@ static int plan_set(bch_kv_plan *plan, uint32_t n_seqs, const uint32_t *n_past, 
     table += (end + plan->shape.page_size - 1) / plan->shape.page_size;
   }
   const KvSchedule work = kv_schedule(seqs, plan->n_heads / plan->shape.n_kv_heads, plan->shape.n_kv_heads,
-                                      plan->shape.head_dim, plan->ctx->n_cus, plan->ctx->attn_partials ? kAttnPartialFloats : 0);
+                                      plan->shape.format, plan->shape.head_dim, plan->ctx->n_cus, plan->ctx->attn_partials ? kAttnPartialFloats : 0);
   Layout all;
   const uint64_t at_pages = all.add(pages, n_pages);
   const uint64_t at_store = all.add(store.data(), store.size());
-  const uint64_t at8 = all.add(work.narrow.data(), work.narrow.size());
-  const uint64_t at16 = all.add(work.tokens.data(), work.tokens.size());
-  const uint64_t at_chunks = all.add(work.chunks.data(), work.chunks.size());
+  const KvWork *const works[] = {&work.tiles8, &work.tiles16, &work.chunks};
+  uint64_t at_items[3], at_starts[3];
+  for (int i = 0; i < 3; i++) {
+    at_items[i] = all.add(works[i]->items.data(), works[i]->items.size());
+    at_starts[i] = all.add(works[i]->starts.data(), works[i]->starts.size());
+  }
   const uint64_t at_join = all.add(work.join.data(), work.join.size());
 
   plan->ready = false;
@@ -169,13 +172,11 @@ static int plan_set(bch_kv_plan *plan, uint32_t n_seqs, const uint32_t *n_past, 
   plan->d_pages = reinterpret_cast<const uint32_t *>(plan->memory + at_pages);
   plan->d_store = reinterpret_cast<const KvStoreItem *>(plan->memory + at_store);
   plan->n_store = (uint32_t)store.size();
-  plan->d_tiles8 = reinterpret_cast<const KvAttnItem *>(plan->memory + at8);
-  plan->d_tiles16 = reinterpret_cast<const KvAttnItem *>(plan->memory + at16);
-  plan->d_chunks = reinterpret_cast<const KvAttnItem *>(plan->memory + at_chunks);
+  bch_kv_plan::Work *const kept[] = {&plan->tiles8, &plan->tiles16, &plan->chunks};
+  for (int i = 0; i < 3; i++)
+    *kept[i] = {reinterpret_cast<const KvAttnItem *>(plan->memory + at_items[i]),
+                reinterpret_cast<const uint32_t *>(plan->memory + at_starts[i]), (uint32_t)works[i]->starts.size() - 1};
   plan->d_join = reinterpret_cast<const KvJoinItem *>(plan->memory + at_join);
-  plan->n_tiles8 = (uint32_t)work.narrow.size();
-  plan->n_tiles16 = (uint32_t)work.tokens.size();
-  plan->n_chunks = (uint32_t)work.chunks.size();
   plan->n_join = (uint32_t)work.join.size();
   plan->join_rows = plan->join_splits = 0;
   for (const KvJoinItem &j : work.join) {
