@@ -109,14 +109,18 @@ struct KvGeometry {
   const uint32_t *pages;
   uint32_t n_kv, page_blocks;  // blocks of a page and head
   uint32_t page_magic;         // ceil(2^31 / page_blocks)
-  // Block b of a sequence whose pages start at `table`, KV head `head`: a
-  // scalar load (the pages are constant while a kernel runs) where all three
-  // are uniform.  (The quotient is exact for b < 2^26 and page_blocks <= 32.)
-  template <uint32_t BYTES>
-  __device__ __forceinline__ uint8_t *block(uint32_t table, uint32_t b, uint32_t head) const {
+  // Block b of a sequence whose pages start at `table`: its page, by a scalar
+  // load where both are uniform (the pages are constant while a kernel runs),
+  // and its address for KV head `head`.  (The quotient is exact for b < 2^26 and
+  // page_blocks <= 32.)
+  __device__ __forceinline__ uint32_t page(uint32_t table, uint32_t b) const {
     using Constant = const __attribute__((address_space(4))) uint32_t;
-    const uint32_t p = __umulhi(2 * b, page_magic);
-    return cache + (((uint64_t)((Constant *)pages)[table + p] * n_kv + head) * page_blocks + (b - p * page_blocks)) * BYTES;
+    return ((Constant *)pages)[table + __umulhi(2 * b, page_magic)];
+  }
+  template <uint32_t BYTES>
+  __device__ __forceinline__ uint8_t *block(uint32_t page, uint32_t b, uint32_t head) const {
+    const uint32_t in_page = b - __umulhi(2 * b, page_magic) * page_blocks;
+    return cache + (((uint64_t)page * n_kv + head) * page_blocks + in_page) * BYTES;
   }
 };
 

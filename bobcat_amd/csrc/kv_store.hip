@@ -149,7 +149,7 @@ __global__ __launch_bounds__(kStoreThreads) void k_kv_load(KvGeometry g, uint32_
   constexpr uint32_t J = HD / 64, BYTES = kv_block_bytes(FORMAT, HD), PART = kKvBlock * HD * sizeof(Elem);
   __shared__ __align__(16) uint8_t s[BYTES];
   const uint32_t b = first / kKvBlock + blockIdx.x, head = blockIdx.y;
-  const uint8_t *block = g.block<BYTES>(table, b, head);
+  const uint8_t *block = g.block<BYTES>(g.page(table, b), b, head);
   for (uint32_t i = threadIdx.x; i < BYTES / 16; i += kStoreThreads)
     reinterpret_cast<uint4 *>(s)[i] = reinterpret_cast<const uint4 *>(block)[i];
   __syncthreads();
