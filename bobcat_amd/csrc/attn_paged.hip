@@ -110,7 +110,9 @@ __device__ __forceinline__ void put_row(const AttnOut &o, uint32_t part, uint32_
 constexpr uint32_t token_groups(uint32_t format, uint32_t hd) {
   return format == BCH_KV_F16 ? (hd == 64 ? 4 : hd == 128 ? 2 : 1) : (hd == 64 ? 4 : hd == 128 ? 3 : 2);
 }
-constexpr uint32_t chunk_groups(uint32_t hd) { return hd == 64 ? 3 : hd == 128 ? 2 : 1; }
+constexpr uint32_t chunk_groups(uint32_t format, uint32_t hd) {
+  return hd == 64 ? (format == BCH_KV_F16 ? 2 : 3) : hd == 128 ? 2 : 1;
+}
 
 // --- at most 16 packed rows ---------------------------------------------------
 
@@ -144,18 +146,13 @@ __global__ __launch_bounds__(256, token_groups(FORMAT, HD)) void k_attn_tokens(
     au4_t x[2][NL];
     float4 s[2];
   } kr, vr;
-  // (Past the end: the last block, masked.)  The pages are looked up a step
-  // before their blocks are loaded.
-  auto number = [&](uint32_t step, int t) { return min(2 * step + t, last); };
-  uint32_t page[2];
-  auto look_up = [&](uint32_t step) __attribute__((always_inline)) {
-#pragma unroll
-    for (int t = 0; t < 2; t++) page[t] = g.page(it.table, number(step, t));
+  auto block = [&](uint32_t step, int t) {
+    return g.block<BYTES>(g.page(it.table, min(2 * step + t, last)), min(2 * step + t, last), kv);  // (past the end: the last block, masked)
   };
   auto load = [&](Raw &raw, uint32_t step, uint32_t part) __attribute__((always_inline)) {
 #pragma unroll
     for (int t = 0; t < 2; t++) {
-      const uint8_t *p = g.block<BYTES>(page[t], number(step, t), kv);
+      const uint8_t *p = block(step, t);
 #pragma unroll
       for (uint32_t c = 0; c < NL; c++)
         raw.x[t][c] = *reinterpret_cast<const au4_t *>(p + part * PART + 1024 * c + 16 * lane);
@@ -163,12 +160,10 @@ __global__ __launch_bounds__(256, token_groups(FORMAT, HD)) void k_attn_tokens(
     }
   };
   uint32_t step = it.lo + wave;
-  auto after = [&](uint32_t step) { return min(step + 4, it.hi - 1); };
-  if (step < it.hi) {
-    look_up(step);
+  const bool any = step < it.hi;
+  if (any) {
     load(kr, step, 0);
     load(vr, step, 1);
-    look_up(after(step));
   }
 
   // The row's elements as the keys' operand has them: k-step s of the MFMA
@@ -217,7 +212,7 @@ __global__ __launch_bounds__(256, token_groups(FORMAT, HD)) void k_attn_tokens(
   float m = 0.f, l = 0.f, lazy = kUnset;
 
   for (; step < it.hi; step += 4) {
-    const uint32_t next = after(step);
+    const uint32_t next = min(step + 4, it.hi - 1);
     // Scores of the tile's 2 x 16 keys: this lane's are 16t + 4·quad + i.
     float u[2][4];
 #pragma unroll
@@ -346,7 +341,6 @@ __global__ __launch_bounds__(256, token_groups(FORMAT, HD)) void k_attn_tokens(
       if constexpr (!PACK) o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl, o[b], 0, 0, 0);
     }
     load(vr, next, 1);
-    look_up(after(next));
   }
 
   // Join the waves.
@@ -386,32 +380,25 @@ __global__ __launch_bounds__(256, token_groups(FORMAT, HD)) void k_attn_tokens(
 
 // --- more rows ------------------------------------------------------------------
 
+template <uint32_t HD>
+constexpr uint32_t kChunkKeys = HD == 256 ? 32 : 64;  // keys of a step
 constexpr uint32_t kChunkRows = 128;
 
-// Steps of 32 keys, one behind the other: while a wave turns the scores of step
-// t into probabilities, the matrix cores compute those of step t + 1, and while
-// they multiply step t's values, it stages later keys and values in LDS.  (A
-// 32x32x16 MFMA takes 32 cycles of the matrix core and leaves the wave free for
-// about six other instructions; one wave's MFMAs and another's vector
-// instructions hardly overlap by themselves.  With both in one stream ... us,
-// apart ... for attend_mixed's chunks.)
 template <uint32_t FORMAT, uint32_t HD>
-__global__ __launch_bounds__(256, chunk_groups(HD)) void k_attn_chunk(
+__global__ __launch_bounds__(256, chunk_groups(FORMAT, HD)) void k_attn_chunk(
     KvGeometry g, const KvAttnItem *__restrict__ items, const uint32_t *__restrict__ starts, const float *__restrict__ q,
     uint32_t q_stride, AttnOut to, uint32_t group, float c2) {
   constexpr bool QUANT = FORMAT != BCH_KV_F16;
   constexpr uint32_t SIZE = kv_elem_bytes(FORMAT), BYTES = kv_block_bytes(FORMAT, HD), PART = kKvBlock * HD * SIZE;
-  constexpr uint32_t KS = HD / 16, OB = HD / 32, M = 4 / SIZE;
-  constexpr uint32_t PIECES = HD * SIZE;        // 16-byte pieces of a block's keys, and of its values
-  constexpr bool SHARED = 2 * PIECES < 256;     // a step's keys are half the waves' pieces, its values the others'
-  constexpr uint32_t NP = SHARED ? 1 : 2 * PIECES / 256;  // of each per thread and step
-  // Keys: 8 elements of key k at slot (element / 8)·32 + k.  Values: the keys
+  constexpr uint32_t KEYS = kChunkKeys<HD>, KS = HD / 16, OB = HD / 32, M = 4 / SIZE;
+  constexpr uint32_t PIECES = HD * SIZE;              // 16-byte pieces of a block's keys, and of its values
+  constexpr uint32_t NP = KEYS / 16 * PIECES / 256;   // of each per thread and step
+  // Keys: 8 elements of key k at slot (element / 8)·KEYS + k.  Values: the keys
   // {0..3, 8..11} + 4h of 16 keys of element d at slot (2·(key / 16) + h)·HD + d.
-  // Those of step t lie in buffer t % 2.
-  __shared__ __align__(16) _Float16 k_s[2][32 * HD], v_s[2][32 * HD];
-  __shared__ __align__(16) float s_s[2][2][32];           // the keys' and the values' scales
-  __shared__ float top_s[2][2];                           // the largest scale_log of each block's values
-  __shared__ uint32_t odd_s[2][4];                        // of each wave: its f16 values were not all finite
+  __shared__ __align__(16) _Float16 k_s[2][KEYS * HD], v_s[2][KEYS * HD];
+  __shared__ __align__(16) float s_s[2][2][KEYS];         // the keys' and the values' scales
+  __shared__ float top_s[2][KEYS / kKvBlock];             // the largest scale_log of each block's values
+  __shared__ uint32_t odd_s[2];
   const uint32_t kv = blockIdx.x % g.n_kv, end = starts[blockIdx.x / g.n_kv + 1];
   for (uint32_t item = starts[blockIdx.x / g.n_kv]; item < end; item++) {
   const KvAttnItem it = items[item];
@@ -425,97 +412,71 @@ __global__ __launch_bounds__(256, chunk_groups(HD)) void k_attn_chunk(
   const uint32_t kend = it.past + (row0 + rows - 1) / group + 1;         // keys of the wave's last row
   const uint32_t wg_pos0 = it.past + it.first / group;                   // the workgroup's first row's
   const uint32_t wg_kend = it.past + (it.first + it.rows - 1) / group + 1;
-  const uint32_t last = (wg_kend - 1) / kKvBlock, last_step = it.hi - 1;
+  const uint32_t last = (wg_kend - 1) / kKvBlock;
+  const uint32_t lo = it.lo * 32, hi = min(it.hi * 32, wg_kend);         // keys of this split
 
-  au4_t kr[NP], vr[SHARED ? 1 : NP];
-  float scale = 0.f;  // of wave w < 2: lanes 0..15 the key scales of block w of the step, 16..31 the value scales
+  au4_t kr[NP], vr[NP];
+  float scale = 0.f;  // of wave w: lanes 0..15 the key scales of block w of the step, 16..31 the value scales
   // Lanes of a value piece: quads of keys in the order 0, 2, 1, 3, so that the
   // two quads whose halves of a slot interleave are written together.
   const uint32_t swapped = (lane & 15) | (lane & 16) << 1 | (lane & 32) >> 1;
+  auto block_at = [&](uint32_t b) { return g.block<BYTES>(g.page(it.table, min(b, last)), min(b, last), kv); };
   // This wave's pieces of part p are within .. + 64 of block j of the step.
-  const uint32_t wave_of = SHARED ? wave & 1 : wave;
-  const bool keys_here = !SHARED || wave < 2, values_here = !SHARED || wave >= 2;
-  auto part_block = [&](uint32_t p) { return 64 * wave_of / PIECES + 256 * p / PIECES; };
-  auto part_within = [&](uint32_t p) { return 64 * wave_of % PIECES + 256 * p % PIECES; };
-  // (Past the end: the last step and block again.)  The pages of the keys of
-  // step n are looked up before those are loaded, and kept for its values.
-  auto clamp = [&](uint32_t step) { return min(step, last_step); };
-  auto number = [&](uint32_t step, uint32_t j) { return min(2 * clamp(step) + j, last); };
-  uint32_t page[NP], page_before[NP], scale_page = 0;
-  auto look_up = [&](uint32_t step) __attribute__((always_inline)) {
+  auto part_block = [&](uint32_t p) { return 64 * wave / PIECES + 256 * p / PIECES; };
+  auto part_within = [&](uint32_t p) { return 64 * wave % PIECES + 256 * p % PIECES; };
+  auto load = [&](uint32_t kb) __attribute__((always_inline)) {
 #pragma unroll
     for (uint32_t p = 0; p < NP; p++) {
-      page_before[p] = page[p];
-      page[p] = g.page(it.table, number(step, part_block(p)));
-    }
-    if constexpr (QUANT) scale_page = g.page(it.table, number(step - 1, wave & 1));
-  };
-  // The keys of step n and the values of step n - 1.
-  auto load_keys = [&](uint32_t step) __attribute__((always_inline)) {
-    if (!keys_here) return;
-#pragma unroll
-    for (uint32_t p = 0; p < NP; p++)
-      kr[p] = *reinterpret_cast<const au4_t *>(g.block<BYTES>(page[p], number(step, part_block(p)), kv) +
-                                               16 * (part_within(p) + lane));
-  };
-  auto load_values = [&](uint32_t step) __attribute__((always_inline)) {
-    if (values_here) {
-#pragma unroll
-      for (uint32_t p = 0; p < NP; p++)
-        (SHARED ? kr : vr)[p] = *reinterpret_cast<const au4_t *>(g.block<BYTES>(page_before[p], number(step, part_block(p)), kv) +
-                                                                 PART + 16 * (part_within(p) + swapped));
+      const uint32_t j = part_block(p), within = part_within(p);
+      const uint8_t *b = block_at(kb / kKvBlock + j);
+      kr[p] = *reinterpret_cast<const au4_t *>(b + 16 * (within + lane));
+      vr[p] = *reinterpret_cast<const au4_t *>(b + PART + 16 * (within + swapped));
     }
     if constexpr (QUANT) {
-      if (wave < 2 && lane < 32)
-        scale = reinterpret_cast<const float *>(g.block<BYTES>(scale_page, number(step, wave), kv) + 2 * PART)[lane];
+      if (wave < KEYS / kKvBlock && lane < 32)
+        scale = reinterpret_cast<const float *>(block_at(kb / kKvBlock + wave) + 2 * PART)[lane];
     }
   };
-  auto stage_keys = [&](uint32_t buf) __attribute__((always_inline)) {
-    if (!keys_here) return;
-#pragma unroll
-    for (uint32_t p = 0; p < NP; p++) {
-      const uint32_t piece = part_within(p) / 16 + lane / 16, key = 16 * part_block(p) + lane % 16;
-      if constexpr (QUANT) {
-        *reinterpret_cast<ah8_t *>(&k_s[buf][(2 * piece * 32 + key) * 8]) = join(widen<FORMAT>(kr[p][0]), widen<FORMAT>(kr[p][1]));
-        *reinterpret_cast<ah8_t *>(&k_s[buf][((2 * piece + 1) * 32 + key) * 8]) = join(widen<FORMAT>(kr[p][2]), widen<FORMAT>(kr[p][3]));
-      } else {
-        *reinterpret_cast<au4_t *>(&k_s[buf][(piece * 32 + key) * 8]) = kr[p];
-      }
-    }
-  };
-  // With `ends`, values behind the last key are cleared where they could be NaN,
-  // and f16 values that are not finite noted.
-  auto stage_values = [&](uint32_t buf, uint32_t kb, auto at_end) __attribute__((always_inline)) {
+  // With `ends`, keys behind the last are cleared where they could be NaN, and
+  // f16 values that are not finite noted.
+  auto stage = [&](int buf, uint32_t kb, auto at_end) __attribute__((always_inline)) {
     constexpr bool ends = decltype(at_end)::value;
     bool odd = false;
-    if (values_here) {
 #pragma unroll
-      for (uint32_t p = 0; p < NP; p++) {
-        const uint32_t j = part_block(p), quad = swapped / 16;
-        au4_t x = (SHARED ? kr : vr)[p];
-        // Bytes behind the last key may be NaN.  (Those of stored rows never are.)
-        if constexpr (FORMAT == BCH_KV_F8 && ends) x &= bytes_below((int)(wg_kend - (kb + 16 * j + 4 * quad)));
+    for (uint32_t p = 0; p < NP; p++) {
+      const uint32_t j = part_block(p), within = part_within(p);
+      const uint32_t piece = within / 16 + lane / 16, key = 16 * j + lane % 16;
+      if constexpr (QUANT) {
+        *reinterpret_cast<ah8_t *>(&k_s[buf][(2 * piece * KEYS + key) * 8]) = join(widen<FORMAT>(kr[p][0]), widen<FORMAT>(kr[p][1]));
+        *reinterpret_cast<ah8_t *>(&k_s[buf][((2 * piece + 1) * KEYS + key) * 8]) = join(widen<FORMAT>(kr[p][2]), widen<FORMAT>(kr[p][3]));
+      } else {
+        *reinterpret_cast<au4_t *>(&k_s[buf][(piece * KEYS + key) * 8]) = kr[p];
+      }
+      const uint32_t quad = swapped / 16;
+      // Bytes behind the last key may be NaN.  (Those of stored rows never are.)
+      if constexpr (FORMAT == BCH_KV_F8 && ends) {
+        if (kb + KEYS > wg_kend) vr[p] &= bytes_below((int)(wg_kend - (kb + 16 * j + 4 * quad)));
+      }
 #pragma unroll
-        for (uint32_t e = 0; e < M; e++) {
-          const uint32_t d = part_within(p) / 4 * M + 16 * e + lane % 16;
-          ah4_t a;
-          if constexpr (QUANT)
-            a = widen<FORMAT>(x[e]);
-          else
-            a = halves(x[2 * e], x[2 * e + 1]);
-          if constexpr (!QUANT && ends) {
+      for (uint32_t x = 0; x < M; x++) {
+        const uint32_t d = within / 4 * M + 16 * x + lane % 16;
+        ah4_t a;
+        if constexpr (QUANT)
+          a = widen<FORMAT>(vr[p][x]);
+        else
+          a = halves(vr[p][2 * x], vr[p][2 * x + 1]);
+        if constexpr (!QUANT && ends) {
 #pragma unroll
-            for (uint32_t i = 0; i < 4; i++) {
-              if (kb + 16 * j + 4 * quad + i >= wg_kend) a[i] = (_Float16)0.f;
-              odd |= not_finite(a[i]);
-            }
+          for (uint32_t i = 0; i < 4; i++) {
+            if (kb + 16 * j + 4 * quad + i >= wg_kend) a[i] = (_Float16)0.f;
+            odd |= not_finite(a[i]);
           }
-          *reinterpret_cast<ah4_t *>(&v_s[buf][((2 * j + quad % 2) * HD + d) * 8 + quad / 2 * 4]) = a;
         }
+        *reinterpret_cast<ah4_t *>(&v_s[buf][((2 * j + quad % 2) * HD + d) * 8 + quad / 2 * 4]) = a;
       }
     }
     if constexpr (QUANT) {
-      if (wave < 2 && lane < 32) {
+      if (wave < KEYS / kKvBlock && lane < 32) {
         const float x = ends && lane >= 16 && kb + 16 * wave + lane % 16 >= wg_kend ? 0.f : scale;
         s_s[buf][lane / 16][16 * wave + lane % 16] = x;
         float top = x == x ? scale_log(x) : 0.f;
@@ -526,14 +487,11 @@ __global__ __launch_bounds__(256, chunk_groups(HD)) void k_attn_chunk(
         if (lane == 16) top_s[buf][wave] = top - 127.f;
       }
     } else if constexpr (ends) {
-      const bool any = __builtin_amdgcn_ballot_w64(odd) != 0;
-      if (lane == 0) odd_s[buf][wave] = any;
+      if (__builtin_amdgcn_ballot_w64(odd) && lane == 0) odd_s[buf] = 1;  // (cleared after the step)
     }
   };
-#pragma unroll
-  for (uint32_t p = 0; p < NP; p++) page[p] = 0;
-  look_up(it.lo);
-  load_keys(it.lo);
+  if (tid < 2) odd_s[tid] = 0;
+  if (lo < hi) load(lo);
 
   ah8_t qh[KS], ql[KS];
   float back = 1.f;
@@ -562,51 +520,65 @@ __global__ __launch_bounds__(256, chunk_groups(HD)) void k_attn_chunk(
     }
   }
   const bool far = __builtin_amdgcn_ballot_w64(back != 1.f) != 0;
-  af16_t o[OB], u;
+  af16_t o[OB];
 #pragma unroll
   for (uint32_t b = 0; b < OB; b++)
 #pragma unroll
     for (int i = 0; i < 16; i++) o[b][i] = 0.f;
   float m = 0.f, l = 0.f, lazy = kUnset;
 
-  // S^T = K·Q^T of the keys in buffer `buf`: element r is the score of key 8·(r / 4)
-  // + 4·half + r % 4 of the step.
-  auto scores = [&](uint32_t buf) __attribute__((always_inline)) {
-    af16_t x;
+  // 32 keys of a step from key kb on, in LDS from key k0 on; score r is of key
+  // kb + 8·(r / 4) + 4·half + r % 4.
+  auto tile = [&](uint32_t kb, uint32_t k0, int buf, auto is_masked) __attribute__((always_inline)) {
+    constexpr bool masked = decltype(is_masked)::value;
+    af16_t u;
 #pragma unroll
-    for (int i = 0; i < 16; i++) x[i] = 0.f;
+    for (int i = 0; i < 16; i++) u[i] = 0.f;
 #pragma unroll
     for (uint32_t s = 0; s < KS; s++) {
-      const ah8_t a = *reinterpret_cast<const ah8_t *>(&k_s[buf][((2 * s + half_id) * 32 + col) * 8]);
-      x = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[s], x, 0, 0, 0);
-      x = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[s], x, 0, 0, 0);
+      const ah8_t a = *reinterpret_cast<const ah8_t *>(&k_s[buf][((2 * s + half_id) * KEYS + k0 + col) * 8]);
+      u = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[s], u, 0, 0, 0);
+      u = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[s], u, 0, 0, 0);
     }
-    return x;
-  };
-  auto scales = [&](uint32_t buf, int which, int q4) __attribute__((always_inline)) {
-    return *reinterpret_cast<const af4_t *>(&s_s[buf][which][8 * q4 + 4 * half_id]);
-  };
-  auto seen = [&](uint32_t kb, int r) __attribute__((always_inline)) { return kb + 8 * (r / 4) + 4 * half_id + r % 4 <= pos; };
-  // Scores to exponents relative to m, which moves where they need it.
-  auto refer = [&](uint32_t kb, uint32_t buf, auto is_masked) __attribute__((always_inline)) {
-    constexpr bool masked = decltype(is_masked)::value;
+    // The values' operands come while the softmax is computed (heads of 256
+    // have no registers for them).
+    auto value = [&](int j, uint32_t b) __attribute__((always_inline)) {
+      return *reinterpret_cast<const ah8_t *>(&v_s[buf][((k0 / 8 + 2 * j + half_id) * HD + 32 * b + col) * 8]);
+    };
+    ah8_t v[2][HD == 256 ? 1 : OB];
+    if constexpr (HD != 256) {
+#pragma unroll
+      for (int j = 0; j < 2; j++)
+#pragma unroll
+        for (uint32_t b = 0; b < OB; b++) v[j][b] = value(j, b);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (far) {
+#pragma unroll
+      for (int r = 0; r < 16; r++) u[r] *= back;
+    }
     // The largest u + log2 b: key by key where some are not seen (those must
     // change nothing), else from the largest of both.
     float top = -INFINITY;
+    auto scales = [&](const float *from, int q4) __attribute__((always_inline)) {
+      const float4 a = *reinterpret_cast<const float4 *>(from + k0 + 8 * q4 + 4 * half_id);
+      return af4_t{a.x, a.y, a.z, a.w};
+    };
+    auto seen = [&](int r) __attribute__((always_inline)) { return kb + 8 * (r / 4) + 4 * half_id + r % 4 <= pos; };
 #pragma unroll
     for (int q4 = 0; q4 < 4; q4++) {
       af4_t a, b;
-      if constexpr (QUANT) a = scales(buf, 0, q4);
-      if constexpr (QUANT && masked) b = scales(buf, 1, q4);
+      if constexpr (QUANT) a = scales(s_s[buf][0], q4);
+      if constexpr (QUANT && masked) b = scales(s_s[buf][1], q4);
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const int r = 4 * q4 + i;
         u[r] = QUANT ? fmaf(u[r], a[i], -m) : u[r] - m;
-        if constexpr (masked) u[r] = seen(kb, r) ? u[r] : -INFINITY;
+        if constexpr (masked) u[r] = seen(r) ? u[r] : -INFINITY;
         top = fmaxf(top, QUANT && masked ? u[r] + scale_log(b[i]) : u[r]);
       }
     }
-    if constexpr (QUANT) top += masked ? -127.f : fmaxf(top_s[buf][0], top_s[buf][1]);
+    if constexpr (QUANT) top += masked ? -127.f : fmaxf(top_s[buf][k0 / 16], top_s[buf][k0 / 16 + 1]);
     if (__builtin_amdgcn_ballot_w64(top > lazy)) {
       top = fmaxf(top, __shfl_xor(top, 32, 64));
       const bool move = top > lazy;  // the same in both lanes of a row
@@ -621,14 +593,11 @@ __global__ __launch_bounds__(256, chunk_groups(HD)) void k_attn_chunk(
 #pragma unroll
       for (int r = 0; r < 16; r++) u[r] -= d;
     }
-  };
-  ah8_t ph[2], pl[2];
-  auto probabilities = [&](uint32_t kb, uint32_t buf, auto is_masked) __attribute__((always_inline)) {
-    constexpr bool masked = decltype(is_masked)::value;
+    ah8_t ph[2], pl[2];
 #pragma unroll
     for (int q4 = 0; q4 < 4; q4++) {
       af4_t b;
-      if constexpr (QUANT) b = scales(buf, 1, q4);
+      if constexpr (QUANT) b = scales(s_s[buf][1], q4);
 #pragma unroll
       for (int i = 0; i < 4; i += 2) {
         const int r = 4 * q4 + i;
@@ -637,7 +606,7 @@ __global__ __launch_bounds__(256, chunk_groups(HD)) void k_attn_chunk(
         af2_t pv = {p0, p1};
         if constexpr (QUANT) {
           // (A scale may be NaN, which 0 times it would be too.)
-          if constexpr (masked) b[i] = seen(kb, r) ? b[i] : 0.f, b[i + 1] = seen(kb, r + 1) ? b[i + 1] : 0.f;
+          if constexpr (masked) b[i] = seen(r) ? b[i] : 0.f, b[i + 1] = seen(r + 1) ? b[i + 1] : 0.f;
           pv = {p0 * b[i], p1 * b[i + 1]};
         }
         const ah2_t h = __builtin_convertvector(pv, ah2_t);
@@ -647,100 +616,77 @@ __global__ __launch_bounds__(256, chunk_groups(HD)) void k_attn_chunk(
         pl[r / 8][r % 8] = e[0], pl[r / 8][r % 8 + 1] = e[1];
       }
     }
-  };
-  auto value = [&](uint32_t buf, int j, uint32_t b) __attribute__((always_inline)) {
-    return *reinterpret_cast<const ah8_t *>(&v_s[buf][((2 * j + half_id) * HD + 32 * b + col) * 8]);
-  };
-  // O^T += V^T·P^T.
-  auto add = [&](ah8_t a, int j, uint32_t b) __attribute__((always_inline)) {
-    o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[j], o[b], 0, 0, 0);
-    o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[j], o[b], 0, 0, 0);
-  };
-
-  stage_keys(it.lo & 1);
-  look_up(it.lo + 1);
-  load_values(it.lo);
-  load_keys(it.lo + 1);
-  const bool plain = !__syncthreads_or(far || !active);
-  u = scores(it.lo & 1);
-  stage_keys(~it.lo & 1);
-  stage_values(it.lo & 1, 32 * it.lo, std::true_type{});
-  look_up(it.lo + 2);
-  load_values(it.lo + 1);
-  load_keys(it.lo + 2);
-  look_up(it.lo + 3);
-  lds_barrier();
-  // Now, for step t: u its products; the keys of t + 1 and the values of t in
-  // LDS; the keys of t + 2 and the values of t + 1 on their way to registers.
-  uint32_t t = it.lo;
-  if (plain) {
-    // Steps that every row sees whole, the next one too.
-    for (; t < last_step && 32 * t + 63 <= wg_pos0; t++) {
-      const uint32_t now = t & 1, then = ~t & 1;
-      refer(32 * t, now, std::false_type{});
-      const af16_t next = scores(then);
-      probabilities(32 * t, now, std::false_type{});
 #pragma unroll
-      for (int j = 0; j < 2; j++)
+    for (int j = 0; j < 2; j++)
 #pragma unroll
-        for (uint32_t b = 0; b < OB; b++) add(value(now, j, b), j, b);
-      stage_keys(now);
-      stage_values(then, 32 * (t + 1), std::false_type{});
-      load_values(t + 2);
-      load_keys(t + 3);
-      look_up(t + 4);
-      u = next;
+      for (uint32_t b = 0; b < OB; b++) {
+        ah8_t a = HD == 256 ? value(j, b) : v[j][HD == 256 ? 0 : b];
+        if constexpr (masked && !QUANT) {
+          // 0 times a value that is not finite is NaN: rows that see such a
+          // value get it from a count, and the product leaves it out.
+          if (odd_s[buf]) {
+            ah8_t seen, bad;
+            af16_t count;
+#pragma unroll
+            for (int i = 0; i < 16; i++) count[i] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              seen[i] = (_Float16)(kb + 16 * j + 4 * half_id + (i & 4) * 2 + (i & 3) <= pos ? 1.f : 0.f);
+              bad[i] = (_Float16)(not_finite(a[i]) ? 1.f : 0.f);
+              a[i] = not_finite(a[i]) ? (_Float16)0.f : a[i];
+            }
+            count = __builtin_amdgcn_mfma_f32_32x32x16_f16(bad, seen, count, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[b][i] = count[i] > 0.f ? NAN : o[b][i];
+          }
+        }
+        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[j], o[b], 0, 0, 0);
+        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[j], o[b], 0, 0, 0);
+      }
+  };
+  if (lo < hi) {
+    const uint32_t last_step = (hi - 1) / KEYS * KEYS;
+    __syncthreads();  // odd_s is clear
+    stage(0, lo, std::true_type{});
+    load(min(lo + KEYS, last_step));
+    lds_barrier();
+    uint32_t kb = lo;
+    int buf = 0;
+    // Steps that every row sees whole.
+    for (; kb < hi && kb + KEYS - 1 <= wg_pos0; kb += KEYS, buf ^= 1) {
+      // The other buffer was read before the last barrier.
+      if (kb < last_step) {
+        if (kb + 2 * KEYS - 1 <= wg_pos0)
+          stage(buf ^ 1, kb + KEYS, std::false_type{});
+        else
+          stage(buf ^ 1, kb + KEYS, std::true_type{});
+        load(min(kb + 2 * KEYS, last_step));
+      }
+      if (active) {
+#pragma unroll 1
+        for (uint32_t k0 = 0; k0 < KEYS; k0 += 32) tile(kb + k0, k0, buf, std::false_type{});
+      }
       lds_barrier();
     }
-  }
-  // The others.
-  for (; t <= last_step; t++) {
-    const uint32_t kb = 32 * t, now = t & 1, then = ~t & 1;
-    if (active && kb < kend) {
-      if (far) {
-#pragma unroll
-        for (int r = 0; r < 16; r++) u[r] *= back;
+    // The others.
+    for (; kb < hi; kb += KEYS, buf ^= 1) {
+      if (kb < last_step) {
+        stage(buf ^ 1, kb + KEYS, std::true_type{});
+        load(min(kb + 2 * KEYS, last_step));
       }
-      refer(kb, now, std::true_type{});
-      probabilities(kb, now, std::true_type{});
-      if (t < last_step) u = scores(then);
-      const bool odd = !QUANT && (odd_s[now][0] | odd_s[now][1] | odd_s[now][2] | odd_s[now][3]);
-#pragma unroll
-      for (int j = 0; j < 2; j++)
-#pragma unroll
-        for (uint32_t b = 0; b < OB; b++) {
-          ah8_t a = value(now, j, b);
-          if constexpr (!QUANT) {
-            // 0 times a value that is not finite is NaN: rows that see such a
-            // value get it from a count, and the product leaves it out.
-            if (odd) {
-              ah8_t sees, bad;
-              af16_t count;
-#pragma unroll
-              for (int i = 0; i < 16; i++) count[i] = 0.f;
-#pragma unroll
-              for (int i = 0; i < 8; i++) {
-                sees[i] = (_Float16)(kb + 16 * j + 4 * half_id + (i & 4) * 2 + (i & 3) <= pos ? 1.f : 0.f);
-                bad[i] = (_Float16)(not_finite(a[i]) ? 1.f : 0.f);
-                a[i] = not_finite(a[i]) ? (_Float16)0.f : a[i];
-              }
-              count = __builtin_amdgcn_mfma_f32_32x32x16_f16(bad, sees, count, 0, 0, 0);
-#pragma unroll
-              for (int i = 0; i < 16; i++) o[b][i] = count[i] > 0.f ? NAN : o[b][i];
-            }
-          }
-          add(a, j, b);
-        }
+      if (active) {
+#pragma unroll 1
+        for (uint32_t k0 = 0; k0 < KEYS && kb + k0 < kend; k0 += 32) tile(kb + k0, k0, buf, std::true_type{});
+      }
+      lds_barrier();
+      if constexpr (!QUANT) {
+        if (tid == 0) odd_s[buf] = 0;
+        lds_barrier();
+      }
     }
-    stage_keys(now);
-    stage_values(then, 32 * (t + 1), std::true_type{});
-    load_values(t + 2);
-    load_keys(t + 3);
-    look_up(t + 4);
-    lds_barrier();
   }
   // (Every wave has passed the last step's barrier: the next item may write to
-  // the buffers.)
+  // the stages.)
   l += __shfl_xor(l, 32, 64);
   if (active && col < rows) {
     const float ref = lazy == kUnset ? -INFINITY : m;
@@ -825,56 +771,124 @@ struct Tile {
   uint32_t steps;
 };
 
-// Deals the tiles' steps to at most `most` workgroups for each KV head in equal
-// shares, cutting a tile where a share ends: all workgroups run at once and end
-// together, and a tile is cut no more often than that takes.  A piece costs
-// kStart steps besides its own (its queries, its results) and has `least` at
-// least; with `whole` no tile is cut.  Tiles whose pieces' records have no room
-// stay whole.
-static void deal(KvSchedule &w, KvWork &work, std::vector<Tile> &tiles, uint64_t most, uint32_t least, bool whole,
-                 uint32_t n_kv, uint64_t records) {
-  constexpr uint64_t kStart = 4;
+// Deals the tiles' steps to workgroups, at most `most` for each KV head so that
+// all run at once, in one of two ways.  Evenly: a tile makes pieces of about one
+// length, `least` steps or more, a workgroup each.  Or in equal shares: a tile is
+// cut where a workgroup's share ends, which then goes on with the next tile, and
+// all workgroups end together.  A piece counts `start` steps besides its own
+// (its queries, the first keys' way, its results); the way whose longest
+// workgroup is shorter is taken.  (Heads of 64, 12 sequences of 96 rows: 31 us
+// evenly, 34 in shares; of 128, 56 tiles of 200 to 500 steps for 64 workgroups:
+// 834 and 800.)  With `whole` no tile is cut.
+struct Dealer {
+  const std::vector<Tile> &tiles;
+  uint64_t most;
+  uint32_t least;
+  bool whole;
+  uint64_t start;
+  uint32_t granule;
+
+  // Pieces of a tile at an even length of n steps.
+  uint32_t pieces(const Tile &t, uint32_t n) const { return whole ? 1u : std::max((t.steps + n / 2) / n, 1u); }
+
+  // put(tile, lo, hi) for every piece, next() between workgroups.
+  template <class Put, class Next>
+  void evenly(uint32_t n, Put &&put, Next &&next) const {
+    for (const Tile &t : tiles) {
+      const uint32_t parts = pieces(t, n), units = (t.steps + granule - 1) / granule;
+      for (uint32_t i = 0; i < parts; i++) {
+        put(t, (uint32_t)((uint64_t)units * i / parts) * granule,
+            std::min((uint32_t)((uint64_t)units * (i + 1) / parts) * granule, t.steps));
+        next();
+      }
+    }
+  }
+  template <class Put, class Next>
+  void shares(uint64_t share, Put &&put, Next &&next) const {
+    uint64_t room = share;
+    for (const Tile &t : tiles)
+      for (uint32_t at = 0; at < t.steps;) {
+        const uint32_t left = t.steps - at;
+        if (room < share && room < (whole ? left : std::min(left, least)) + start) {  // no room for a piece
+          next();
+          room = share;
+        }
+        uint32_t take = left;
+        if (!whole && room < left + start && left >= 2 * least)
+          take = std::max(std::min(std::max((uint32_t)(room - start), least), left - least) / granule * granule, granule);
+        put(t, at, at + take);
+        at += take;
+        room -= std::min<uint64_t>(room, take + start);
+      }
+  }
+};
+
+static void deal(KvSchedule &w, KvWork &work, const std::vector<Tile> &tiles, uint64_t most, uint32_t least, bool whole,
+                 uint64_t start, uint32_t n_kv, uint32_t granule, uint64_t records) {
   work.starts.push_back(0);
   if (tiles.empty()) return;
-  uint64_t total = 0;
-  for (const Tile &t : tiles) total += t.steps + kStart;
-  most = std::max<uint64_t>(most, 1);
-  uint64_t groups = whole ? std::min<uint64_t>(most, tiles.size()) : std::min(most, std::max<uint64_t>(total / (least + kStart), 1));
-  const uint64_t share = std::max<uint64_t>((total + kStart * groups + groups - 1) / groups, least + kStart);
-  uint64_t room = share, dealt = 1;  // of the open workgroup; workgroups opened
-  auto close = [&]() {
-    if (work.starts.back() == work.items.size() || dealt == groups) return;
-    work.starts.push_back((uint32_t)work.items.size());
-    room = share;
-    dealt++;
-  };
-  for (Tile &t : tiles) {
-    const uint64_t rows = (uint64_t)n_kv * t.it.rows;
-    const size_t first = work.items.size();
-    for (uint32_t at = 0; at < t.steps;) {
-      const uint32_t left = t.steps - at;
-      // No room for a piece: the next workgroup's.
-      if (room < left + kStart && (whole || room < least + kStart)) close();
-      uint32_t take = left;
-      if (!whole && dealt < groups && room < left + kStart && left >= 2 * least && w.records + 2 * rows <= records) {
-        take = std::max((uint32_t)(room > kStart ? room - kStart : 0), least);
-        take = std::min(take, left - least);
-      }
-      t.it.lo = at;
-      t.it.hi = at + take;
-      t.it.part = (uint32_t)w.records;
-      if (take < t.steps) w.records += rows;
-      work.items.push_back(t.it);
-      at += take;
-      room -= std::min<uint64_t>(room, take + kStart);
-    }
-    const uint32_t pieces = (uint32_t)(work.items.size() - first);
-    if (pieces == 1)
-      work.items[first].part = ~0u;
-    else
-      w.join.push_back({t.it.row, t.it.first, t.it.rows, pieces, work.items[first].part});
+  Dealer d{tiles, std::max<uint64_t>(most, 1), least, whole, start, granule};
+  uint64_t total = 0, room = w.records;
+  uint32_t longest = 1;
+  for (const Tile &t : tiles) {
+    total += t.steps + start;
+    longest = std::max(longest, t.steps);
   }
-  work.starts.push_back((uint32_t)work.items.size());
+  // The smallest length and share that make no more than `most` workgroups.
+  auto smallest = [](uint64_t lo, uint64_t hi, auto &&fits) {
+    while (lo < hi) {
+      const uint64_t mid = lo + (hi - lo) / 2;
+      if (fits(mid)) hi = mid; else lo = mid + 1;
+    }
+    return lo;
+  };
+  auto none = [](const Tile &, uint32_t, uint32_t) {};
+  const uint32_t even = (uint32_t)smallest(least, 2ull * std::max(longest, least), [&](uint64_t n) {
+    uint64_t sum = 0;
+    for (const Tile &t : tiles) sum += d.pieces(t, (uint32_t)n);
+    return sum <= d.most;
+  });
+  uint64_t even_groups = 0, even_end = 0;
+  for (const Tile &t : tiles) {
+    even_groups += d.pieces(t, even);
+    even_end = std::max<uint64_t>(even_end, t.steps / d.pieces(t, even) + start);
+  }
+  const uint64_t share = smallest(std::max<uint64_t>(total / d.most, least + start), total + 1, [&](uint64_t n) {
+    uint64_t groups = 1;
+    d.shares(n, none, [&] { groups++; });
+    return groups <= d.most;
+  });
+  const bool evenly = even_groups <= d.most && even_end <= share;
+  // Partial results of more pieces than have room: no tile is cut.
+  auto need = [&](const Tile &t, uint32_t lo, uint32_t hi) {
+    if (hi - lo < t.steps) room += (uint64_t)n_kv * t.it.rows;
+  };
+  if (evenly)
+    d.evenly(even, need, [] {});
+  else
+    d.shares(share, need, [] {});
+  if (room > records) d.whole = true;
+
+  const Tile *open = nullptr;  // the tile that the last piece was of
+  auto put = [&](const Tile &t, uint32_t lo, uint32_t hi) {
+    KvAttnItem it = t.it;
+    it.lo = lo;
+    it.hi = hi;
+    if (hi - lo < t.steps) {
+      if (open != &t) w.join.push_back({it.row, it.first, it.rows, 0, (uint32_t)w.records});
+      w.join.back().splits++;
+      it.part = (uint32_t)w.records;
+      w.records += (uint64_t)n_kv * it.rows;
+    }
+    open = &t;
+    work.items.push_back(it);
+  };
+  auto next = [&] { work.starts.push_back((uint32_t)work.items.size()); };
+  if (evenly)
+    d.evenly(even, put, next);
+  else
+    d.shares(share, put, next);
+  if (work.starts.back() != work.items.size()) next();
 }
 
 KvSchedule kv_schedule(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t n_kv, uint32_t format, uint32_t head_dim,
@@ -882,20 +896,24 @@ KvSchedule kv_schedule(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t 
   KvSchedule w;
   const uint64_t records = std::min<uint64_t>(partial_floats / (head_dim + 4), 0xfffffffeu);
   if (!n_cus) n_cus = 256;
-  // Which tiles.  Up to 32 rows take narrow tiles, which read the keys again
-  // for every 16 rows (twelve sequences of about 2,000 keys, 20 and 32 rows,
-  // heads of 64: 23 and 24 us against 26 and 26 in wide ones; of 256: 27 and 37
-  // against 44 and 46).  Up to 128 rows do while the batch is small, because a
-  // wide tile's few waves then wait for one another (1,000 keys, 96 rows, heads
-  // of 128: 11 us against 20; at ten times the keys they are level).
-  constexpr uint32_t kFewRows = 32;
+  // Which tiles.  Narrow ones read the keys again for every 16 rows but share
+  // them out among the waves; in a wide one's the waves share the keys, and idle
+  // where there are no rows for them.  Twelve sequences of about 2,000 keys, 20,
+  // 64, 96 and 128 rows: 17, 27, 28 and 44 us in narrow tiles, 26, 28, 31 and 36
+  // in wide ones (heads of 64; of 128: 20, 31, 48, 64 and 36, 36, 49, 58; of 256:
+  // 18, 30, 41, 48 and 44, 38, 48, 51).  One sequence of 128 rows and 1,000 keys:
+  // 12 and 20.  Where some sequence needs wide tiles, only those of up to 32 rows
+  // stay narrow, since a second launch costs more than the rows that idle.
   constexpr uint64_t kSmallBatch = 1u << 20;  // narrow tiles x steps x KV heads x head_dim
   uint64_t narrow_work = 0;
+  bool wide = false, large = false;
   for (const KvSeq &q : seqs) {
     const uint64_t rows = (uint64_t)q.n_new * group;
+    wide |= rows > kChunkRows;
+    large |= rows > 96;
     if (rows > 16 && rows <= kChunkRows) narrow_work += (rows + 15) / 16 * ((q.past + q.n_new + 31) / 32) * n_kv * head_dim;
   }
-  const uint32_t few_rows = narrow_work <= kSmallBatch ? kChunkRows : kFewRows;
+  const uint32_t few_rows = wide || (large && narrow_work > kSmallBatch) ? 32 : kChunkRows;
   std::vector<Tile> narrow, tokens, chunks;
   uint32_t longest = 0;
   uint64_t narrow_steps = 0, token_steps = 0;
@@ -913,7 +931,7 @@ KvSchedule kv_schedule(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t 
     }
   }
   // A few tiles of 8 rows join those of 16 in one launch.
-  if (narrow_steps < token_steps) {
+  if (narrow_steps <= token_steps) {
     tokens.insert(tokens.end(), narrow.begin(), narrow.end());
     narrow.clear();
   }
@@ -921,10 +939,16 @@ KvSchedule kv_schedule(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t 
   // a join (about 2.5 us) pays from 24 steps on with heads of 64, 19 of 128, 16
   // of 256 (300 keys of 64: 5.6 us whole, 7.6 cut; 2,000: 14.2 and 9.0).
   const uint32_t unsplit = 14 + 640 / head_dim;
-  const uint64_t few_groups = (uint64_t)n_cus * token_groups(format, head_dim) / n_kv;
-  deal(w, w.tiles8, narrow, few_groups, 8, longest <= unsplit, n_kv, records);
-  deal(w, w.tiles16, tokens, few_groups, 8, longest <= unsplit, n_kv, records);
-  deal(w, w.chunks, chunks, (uint64_t)n_cus * chunk_groups(head_dim) / n_kv, 8, false, n_kv, records);
+  // What the registers let run at once; of heads of 256 one a CU (twelve
+  // sequences of drafts of 256: 19 us, with two 22).
+  const uint64_t few_groups = (uint64_t)n_cus * (head_dim == 256 ? 1 : token_groups(format, head_dim)) / n_kv;
+  deal(w, w.tiles8, narrow, few_groups, 8, longest <= unsplit, 4, n_kv, 1, records);
+  deal(w, w.tiles16, tokens, few_groups, 8, longest <= unsplit, 4, n_kv, 1, records);
+  // Wide tiles: what starting one costs showed in prompts without a past, 2,048
+  // tokens in 64 tiles of 1 to 64 steps (heads of 128): 156 us counted as 4
+  // steps, 114 as 10.
+  deal(w, w.chunks, chunks, (uint64_t)n_cus * chunk_groups(format, head_dim) / n_kv, head_dim == 256 ? 4 : 8, false, 10,
+       n_kv, head_dim == 256 ? 1 : 2, records);
   return w;
 }
 

@@ -205,6 +205,19 @@ def test_attention_groups(hip, heads, kv, fmt, seqs):
     check_attention(hip, *case_args(np.random.default_rng(heads), fmt, heads, kv, 64, 16, seqs))
 
 
+# (past, new) with 4 heads a KV head: 8 and 9, 16 and 17, 32 and 33, 96 and 97, 128 and 129 rows and the like, alone and
+# beside others; a wide tile with each number of rows in its last wave; many pieces of many tiles.
+ROWS = [[(40, 2)], [(40, 3), (7, 2)], [(40, 4), (9, 5)], [(300, 8), (20, 9)], [(100, 24)], [(100, 25)], [(60, 32)],
+        [(60, 33)], [(33, 41), (5, 9), (90, 1), (70, 3)], [(0, 64)], [(2000, 33), (3000, 20)], [(700, 100), (900, 1)] * 3]
+
+
+@pytest.mark.parametrize("fmt,hd", [("f16", 64), ("i8", 64), ("f8", 128), ("f16", 128), ("i8", 256)])
+@pytest.mark.parametrize("seqs", ROWS)
+def test_attention_tiles(hip, fmt, hd, seqs):
+    say("attention_paged tiles", fmt, hd, seqs)
+    check_attention(hip, *case_args(np.random.default_rng(len(seqs)), fmt, 4, 1, hd, 48, seqs))
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("new", [1, 40])
 def test_attention_strides(hip, fmt, new):
