@@ -73,6 +73,15 @@ __device__ __forceinline__ ah4_t halves(uint32_t a, uint32_t b) { return __built
 // log2 b to within 0.09, plus 127, from a scale's bits (0 for b = 0).
 __device__ __forceinline__ float scale_log(float b) { return (float)__float_as_int(b) * 0x1p-23f; }
 
+// x as it is in f32.  A product that is then rounded to f16 may otherwise be
+// rounded once, inside the multiplication, for one of its uses and twice for
+// another: a high part and the low part taken from it would then not belong
+// together (one element in 8,000 was off by an f16 step of its high part).
+__device__ __forceinline__ float in_f32(float x) {
+  asm("" : "+v"(x));
+  return x;
+}
+
 __device__ __forceinline__ bool not_finite(_Float16 x) { return (__builtin_bit_cast(uint16_t, x) & 0x7c00) == 0x7c00; }
 
 // The lowest n bytes (0 to 4, clamped).
@@ -193,7 +202,7 @@ __global__ __launch_bounds__(256, token_groups(FORMAT, HD)) void k_attn_tokens(
     for (uint32_t s = 0; s < KS; s++)
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        const float v = x[s][j] * down;
+        const float v = in_f32(x[s][j] * down);
         const _Float16 hi = (_Float16)v, lo = (_Float16)(v - (float)hi);
         if constexpr (PACK) {
           qh[s][j] = col < 8 ? hi : lo;
@@ -282,7 +291,7 @@ __global__ __launch_bounds__(256, token_groups(FORMAT, HD)) void k_attn_tokens(
       for (int i = 0; i < 4; i++) {
         const float p = __builtin_amdgcn_exp2f(u[t][i]);
         l += p;
-        const float pv = QUANT ? p * vs[t][i] : p;
+        const float pv = QUANT ? in_f32(p * vs[t][i]) : p;
         const _Float16 hi = (_Float16)pv;
         if constexpr (PACK) {
           ph[4 * t + i] = (_Float16)fmaf(-(float)hi, low, pv);
@@ -505,7 +514,7 @@ __global__ __launch_bounds__(256, chunk_groups(FORMAT, HD)) void k_attn_chunk(
         const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-          const float x = v[j] * c2 * factor;
+          const float x = in_f32(v[j] * c2 * factor);
           largest = fmaxf(largest, fabsf(x));
           qh[s][j] = (_Float16)x;
           ql[s][j] = (_Float16)(x - (float)qh[s][j]);
@@ -607,7 +616,7 @@ __global__ __launch_bounds__(256, chunk_groups(FORMAT, HD)) void k_attn_chunk(
         if constexpr (QUANT) {
           // (A scale may be NaN, which 0 times it would be too.)
           if constexpr (masked) b[i] = seen(r) ? b[i] : 0.f, b[i + 1] = seen(r + 1) ? b[i + 1] : 0.f;
-          pv = {p0 * b[i], p1 * b[i + 1]};
+          pv = {in_f32(p0 * b[i]), in_f32(p1 * b[i + 1])};
         }
         const ah2_t h = __builtin_convertvector(pv, ah2_t);
         const af2_t rest = {pv[0] - (float)h[0], pv[1] - (float)h[1]};

@@ -282,6 +282,36 @@ def test_attention_leaves_out_what_a_query_does_not_see(hip, fmt, seqs, what):
         assert np.isnan(after[spoilt:end, :, 9]).all()
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("new", [1, 3, 130])
+def test_attention_probabilities(hip, fmt, new):
+    """Key i has 64 in element i alone and value i has 1 there, so that an output is the softmax of 8·q itself and shows
+    every query element's rounding.  A score s is off by s·(2^-22 + 8·2^-24): the query's two parts and seven f32
+    roundings (its scaling, the constant's, the key's scale, the reference's twice, the product's and the sum's); a
+    probability by twice the largest of that (its own and the sum's), 2^-22 for its parts, 64·2^-24 for the sum and as
+    many as 16 roundings more.  Besides, a part below f16's normal range is a multiple of 2^-24, off by 2^-25 at most,
+    where the row's largest is 2^8 or more: 2^-33 of the sum."""
+    rng = np.random.default_rng(77)
+    heads, kv, hd, page, n = 8, 2, 64, 32, 24 if new < 100 else 2
+    batch = Batch(rng, [(64, new)] * n, page)
+    for pages in batch.pages:
+        pages[:2] = batch.pages[0][:2]
+    pool = Pool(fmt, kv, hd, page, batch.n_pages)
+    eye = np.eye(64, dtype=np.float32)
+    for i in range(64):
+        pool.put(batch.pages[0][i // page], i % page, np.tile(64 * eye[i], (kv, 1)), np.tile(eye[i], (kv, 1)))
+    batch.put(pool, np.zeros((batch.tokens, kv, hd), np.float32), np.zeros((batch.tokens, kv, hd), np.float32))
+    q = rng.standard_normal((batch.tokens, heads, hd)).astype(np.float32)
+    got, row = attend(hip, pool, batch, heads, q), 0
+    size = 8 * np.abs(q).max()
+    bound = 2 * size * (2.0 ** -22 + 8 * 2.0 ** -24) + 2.0 ** -22 + (64 + 16) * 2.0 ** -24
+    for s in range(n):
+        k, v = batch.gather(pool, s)
+        want = attention(q[row:row + new], k, v, 64)
+        assert (np.abs(got[row:row + new] - want) <= bound * want + 2.0 ** -33).all(), s
+        row += new
+
+
 def test_attention_shared_prefix_and_changed_batches(hip):
     """Sequences that share pages, a plan that is given another batch, and batches without tokens."""
     rng = np.random.default_rng(13)
