@@ -285,12 +285,13 @@ __global__ __launch_bounds__(256, token_groups(FORMAT, HD)) void k_attn_tokens(
         for (int i = 0; i < 4; i++) u[t][i] -= d;
     }
     ah8_t ph, pl;
+    float sum = 0.f;  // of the step, so that l takes one rounding from it
 #pragma unroll
     for (int t = 0; t < 2; t++)
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const float p = __builtin_amdgcn_exp2f(u[t][i]);
-        l += p;
+        sum += p;
         const float pv = QUANT ? in_f32(p * vs[t][i]) : p;
         const _Float16 hi = (_Float16)pv;
         if constexpr (PACK) {
@@ -300,6 +301,7 @@ __global__ __launch_bounds__(256, token_groups(FORMAT, HD)) void k_attn_tokens(
           pl[4 * t + i] = (_Float16)(pv - (float)hi);
         }
       }
+    l += sum;
     if constexpr (FORMAT == BCH_KV_F8) {
       // Bytes behind the last key may be NaN.  (Those of stored rows never are.)
       if (32 * step + 31 >= n_keys) {
@@ -603,6 +605,7 @@ __global__ __launch_bounds__(256, chunk_groups(FORMAT, HD)) void k_attn_chunk(
       for (int r = 0; r < 16; r++) u[r] -= d;
     }
     ah8_t ph[2], pl[2];
+    float sum = 0.f;  // of the tile, so that l takes one rounding from it
 #pragma unroll
     for (int q4 = 0; q4 < 4; q4++) {
       af4_t b;
@@ -611,7 +614,7 @@ __global__ __launch_bounds__(256, chunk_groups(FORMAT, HD)) void k_attn_chunk(
       for (int i = 0; i < 4; i += 2) {
         const int r = 4 * q4 + i;
         const float p0 = __builtin_amdgcn_exp2f(u[r]), p1 = __builtin_amdgcn_exp2f(u[r + 1]);
-        l += p0 + p1;
+        sum += p0 + p1;
         af2_t pv = {p0, p1};
         if constexpr (QUANT) {
           // (A scale may be NaN, which 0 times it would be too.)
@@ -625,6 +628,7 @@ __global__ __launch_bounds__(256, chunk_groups(FORMAT, HD)) void k_attn_chunk(
         pl[r / 8][r % 8] = e[0], pl[r / 8][r % 8 + 1] = e[1];
       }
     }
+    l += sum;
 #pragma unroll
     for (int j = 0; j < 2; j++)
 #pragma unroll
