@@ -391,8 +391,8 @@ __global__ __launch_bounds__(256, token_groups(FORMAT, HD)) void k_attn_tokens(
 
 // --- more rows ------------------------------------------------------------------
 
-template <uint32_t HD>
-constexpr uint32_t kChunkKeys = HD == 256 ? 32 : 64;  // keys of a step
+// Keys of a step: what the registers that bring the next step's hold.
+constexpr uint32_t chunk_keys(uint32_t format, uint32_t hd) { return hd == 256 || (hd == 128 && format == BCH_KV_F16) ? 32 : 64; }
 constexpr uint32_t kChunkRows = 128;
 
 template <uint32_t FORMAT, uint32_t HD>
@@ -401,7 +401,7 @@ __global__ __launch_bounds__(256, chunk_groups(FORMAT, HD)) void k_attn_chunk(
     uint32_t q_stride, AttnOut to, uint32_t group, float c2) {
   constexpr bool QUANT = FORMAT != BCH_KV_F16;
   constexpr uint32_t SIZE = kv_elem_bytes(FORMAT), BYTES = kv_block_bytes(FORMAT, HD), PART = kKvBlock * HD * SIZE;
-  constexpr uint32_t KEYS = kChunkKeys<HD>, KS = HD / 16, OB = HD / 32, M = 4 / SIZE;
+  constexpr uint32_t KEYS = chunk_keys(FORMAT, HD), KS = HD / 16, OB = HD / 32, M = 4 / SIZE;
   constexpr uint32_t PIECES = HD * SIZE;              // 16-byte pieces of a block's keys, and of its values
   constexpr uint32_t NP = KEYS / 16 * PIECES / 256;   // of each per thread and step
   // Keys: 8 elements of key k at slot (element / 8)·KEYS + k.  Values: the keys
@@ -957,11 +957,12 @@ KvSchedule kv_schedule(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t 
   const uint64_t few_groups = (uint64_t)n_cus * (head_dim == 256 ? 1 : token_groups(format, head_dim)) / n_kv;
   deal(w, w.tiles8, narrow, few_groups, 8, longest <= unsplit, 4, n_kv, 1, records);
   deal(w, w.tiles16, tokens, few_groups, 8, longest <= unsplit, 4, n_kv, 1, records);
-  // Wide tiles: what starting one costs showed in prompts without a past, 2,048
+  const uint32_t keys = chunk_keys(format, head_dim);
+  // Wide tiles: four trips of the loop at least.  What starting one costs showed in prompts without a past, 2,048
   // tokens in 64 tiles of 1 to 64 steps (heads of 128): 156 us counted as 4
   // steps, 114 as 10.
-  deal(w, w.chunks, chunks, (uint64_t)n_cus * chunk_groups(format, head_dim) / n_kv, head_dim == 256 ? 4 : 8, false, 10,
-       n_kv, head_dim == 256 ? 1 : 2, records);
+  deal(w, w.chunks, chunks, (uint64_t)n_cus * chunk_groups(format, head_dim) / n_kv, keys / 8, false, 10, n_kv,
+       keys / 32, records);
   return w;
 }
 

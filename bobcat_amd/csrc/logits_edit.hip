@@ -12,7 +12,7 @@
 // That a row's history is read by each of its slices costs less than counters
 // in memory would: 4 bytes a token out of the L2 against 8 bytes a logit.
 // Bound by the logits' bytes: 96 rows of 151,936 with histories of 2,000 tokens
-// take 29 us, 22 without (5.3 TB/s); a single row by latency (5.8 us).
+// take 30 us (4.0 TB/s); a single row by latency (5.9 us).
 #include <cmath>
 
 #include "device.h"
@@ -20,7 +20,6 @@
 #include "runtime.h"
 
 namespace bch {
-
 
 constexpr uint32_t kEditPer = 8;  // logits of a thread
 
@@ -43,11 +42,13 @@ __global__ __launch_bounds__(THREADS) void k_logits_edit(EditArgs a) {
   const uint32_t len = min(SLICE, a.n_vocab - base);
   const bch_logit_row r = a.rows[row];
   const uint64_t at = (uint64_t)row * a.n_vocab + base;
+  // (Streamed past the caches: 30 us instead of 36 for 96 rows of 151,936 with
+  // histories of 2,000 tokens.)
   float x[PER];
 #pragma unroll
   for (uint32_t j = 0; j < PER; j++) {
     const uint32_t i = tid + THREADS * j;
-    x[j] = i < len ? a.logits[at + i] : 0.f;
+    x[j] = i < len ? __builtin_nontemporal_load(a.logits + at + i) : 0.f;
   }
   // Lists never leave the buffers, whatever the row says.
   const uint32_t h0 = min(r.history_at, a.n_history), hn = min(r.history_len, a.n_history - h0);
@@ -109,7 +110,7 @@ __global__ __launch_bounds__(THREADS) void k_logits_edit(EditArgs a) {
     if (i >= len) continue;
     const uint32_t t = base + i;
     const bool allowed = !masked || (known && (mask[t / 32] >> (t % 32) & 1));
-    a.out[at + i] = allowed ? x[j] : -INFINITY;
+    __builtin_nontemporal_store(allowed ? x[j] : -INFINITY, a.out + at + i);
   }
 }
 
@@ -146,8 +147,8 @@ extern "C" int bch_logits_edit(bch_ctx *ctx, bch_view logits, bch_view out, uint
   // Slices of 4,096 logits for long histories, of which each slice reads all, and
   // of 2,048 for short ones, whose rows make more workgroups: 96 rows of 151,936
   // with 2,000 tokens on average 29 us and 32, with 1 token 22 and 22; one row of
-  // 65,536 with 600 tokens 6.4 and 5.8 (16 logits a thread instead of eight: 39
-  // to 42 of the 29 and 32).
+  // 65,536 with 600 tokens 6.4 and 5.8.  (The same inputs each time; 16 logits a
+  // thread instead of eight: 39 and 42 instead of 29 and 32.)
   const bool long_history = n_rows && a.n_history / n_rows > 1024;
   const uint32_t threads = long_history ? 512 : 256;
   a.slices = div_ceil(n_vocab, threads * kEditPer);

@@ -391,8 +391,9 @@ int bch_kv_load(bch_ctx *ctx, const bch_kv_plan *plan, bch_view cache, uint32_t 
  * n_heads·head_dim floats, q_stride and out_stride floats apart (16-byte
  * aligned, strides a multiple of 4); query head h reads KV head
  * h / (n_heads / n_kv_heads).  `out` may not lie over `q`.  What a query does
- * not see has no part in its output, whatever it holds; a value that it sees
- * and that is infinite or NaN makes that element of its output NaN.  The queries and the
+ * not see has no part in its output, whatever it holds.  A value that it sees
+ * and that is infinite or NaN makes that element of its output NaN; such a key
+ * makes all of it NaN (or, where q·k is -inf, may have no weight).  The queries and the
  * probabilities enter the products with ~22 bits, as in
  * bch_attention_prefill. */
 int bch_attention_paged(bch_ctx *ctx, const bch_kv_plan *plan, bch_view cache, bch_view q, uint32_t q_stride,

@@ -10,8 +10,8 @@ import pytest
 
 from _paged import Batch, Pool, attention, attention_bound, dequantise, quantise, random_rows
 from bobcat_amd import BobcatError
-from bobcat_amd._lib import STATUS
-from bobcat_amd.backend import Hip, kv_page_bytes
+from bobcat_amd._lib import STATUS, Sampling
+from bobcat_amd.backend import LOGIT_ROW, NO_MASK, Format, Hip, kv_page_bytes
 
 pytestmark = pytest.mark.gpu
 
@@ -403,6 +403,49 @@ def test_store_then_attend_over_steps(hip, fmt):
         past = [a + n for a, n in zip(past, new)]
     assert past == total
     assert np.array_equal(hip.read(cache.at(0), np.empty_like(pool.bytes)), pool.bytes)
+
+
+def test_a_serving_step(hip):
+    """Two sequences' step in one recording: rows stored, attended to, projected to logits, ruled and sampled greedily."""
+    rng = np.random.default_rng(41)
+    heads, kv, hd, page, vocab = 4, 2, 64, 16, 1000
+    pool, batch, q = case(rng, "i8", heads, kv, hd, page, [(50, 1), (7, 1)])
+    rows = np.stack([random_rows(rng, kv, hd) for _ in range(2)], 1)
+    head = (rng.standard_normal((vocab, heads * hd)) / 16).astype(np.float32)
+    cache, plan = hip.buffer_from(pool.bytes), plan_of(hip, pool, batch, heads)
+    kb, vb, qb, wb = (hip.buffer_from(x) for x in (rows[0], rows[1], q, head))
+    out, logits, tokens = hip.new_buffer(q.nbytes), hip.new_buffer(2 * vocab * 4), hip.new_buffer(8)
+    state = hip.buffer_from(np.zeros(1, np.uint64))
+    batch.put(pool, rows[0], rows[1])
+    attended = [attention(q[s:s + 1], *batch.gather(pool, s), batch.past[s]).reshape(-1) for s in range(2)]
+    want = np.stack(attended) @ head.astype(np.float64).T
+    best = want.argmax(1)
+    # The first row's best token is forbidden, the second's is in its history.
+    mask = np.full((vocab + 31) // 32, 0xFFFFFFFF, np.uint32)
+    mask[best[0] // 32] &= ~np.uint32(1 << int(best[0] % 32))
+    table = np.zeros(2, LOGIT_ROW)
+    table["mask"], table["repeat"], table["history_len"] = [0, NO_MASK], 1.0, [0, 1]
+    table["presence"] = 100.0
+    tb, hb, mb = hip.buffer_from(table), hip.buffer_from(best[1:].astype(np.uint32)), hip.buffer_from(mask)
+
+    def step():
+        hip.kv_store(plan, cache.at(0), kb.at(0), kv * hd, vb.at(0), kv * hd)
+        hip.attention_paged(plan, cache.at(0), qb.at(0), heads * hd, out.at(0), heads * hd)
+        for s in range(2):
+            hip.matvec(Format.F32, wb.at(0), vocab, heads * hd, out.at(4 * s * heads * hd), logits.at(4 * s * vocab))
+        hip.logits_edit(logits.at(0), logits.at(0), 2, vocab, tb.at(0), history=hb.at(0), n_history=1, masks=mb.at(0),
+                        n_masks=1)
+        for s in range(2):
+            hip.sample(logits.at(4 * s * vocab), vocab, hb.at(0), 0, Sampling(0.0, 0, 1.0, 0.0, 1.0), state.at(0),
+                       tokens.at(4 * s))
+
+    run(hip, step)
+    assert np.array_equal(hip.read(cache.at(0), np.empty_like(pool.bytes)), pool.bytes)
+    want[[0, 1], best] = -np.inf
+    got = hip.read(tokens.at(0), np.empty(2, np.uint32))
+    gap = np.sort(want, axis=1)
+    assert (gap[:, -1] - gap[:, -2]).min() > 1e-3  # (the choice is not one of rounding)
+    assert got.tolist() == want.argmax(1).tolist()
 
 
 # --- refusals -------------------------------------------------------------------------
