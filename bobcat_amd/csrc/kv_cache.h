@@ -89,7 +89,8 @@ struct KvJoinItem {
   uint32_t row, first, rows, splits, part;
 };
 // Items dealt to workgroups: workgroup w of a KV head takes items starts[w] ..
-// starts[w + 1].
+// starts[w + 1].  (Where each has one, the kernels get no starts and save a
+// load that the item's own load would wait for.)
 struct KvWork {
   std::vector<KvAttnItem> items;
   std::vector<uint32_t> starts;

@@ -175,7 +175,10 @@ static int plan_set(bch_kv_plan *plan, uint32_t n_seqs, const uint32_t *n_past, 
   bch_kv_plan::Work *const kept[] = {&plan->tiles8, &plan->tiles16, &plan->chunks};
   for (int i = 0; i < 3; i++)
     *kept[i] = {reinterpret_cast<const KvAttnItem *>(plan->memory + at_items[i]),
-                reinterpret_cast<const uint32_t *>(plan->memory + at_starts[i]), (uint32_t)works[i]->starts.size() - 1};
+                works[i]->items.size() < works[i]->starts.size()
+                    ? nullptr
+                    : reinterpret_cast<const uint32_t *>(plan->memory + at_starts[i]),
+                (uint32_t)works[i]->starts.size() - 1};
   plan->d_join = reinterpret_cast<const KvJoinItem *>(plan->memory + at_join);
   plan->n_join = (uint32_t)work.join.size();
   plan->join_rows = plan->join_splits = 0;
