@@ -48,6 +48,11 @@ typedef uint32_t au4_t __attribute__((ext_vector_type(4)));
 // passes 2^kLazy: high in f16's range, so that the low parts of much smaller
 // ones are still normal numbers, with room for scale_log's error.
 constexpr float kPeak = 8.f, kLazy = 14.f;
+// A reference that moves further than kCoarse takes u with it only to its own last
+// place, so it moves again by what is left, up or down.  (O and l are 0 then.  From
+// 2^33 on the first move is the largest u itself; below, the second one's last
+// place is 2^-11.)
+constexpr float kCoarse = 262144.f;
 constexpr float kUnset = -INFINITY;      // in its place, of a row that has seen no key yet
 
 // Four elements of 8 bits as f16, exactly.
@@ -87,11 +92,13 @@ __device__ __forceinline__ bool not_finite(_Float16 x) { return (__builtin_bit_c
 // The lowest n bytes (0 to 4, clamped).
 __device__ __forceinline__ uint32_t bytes_below(int n) { return n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1; }
 
-// A query's factor to and from f16's range: 1 unless its largest element
-// (times scale·log2 e) passes 2^15.
-__device__ __forceinline__ float query_down(float largest) {
-  if (!(largest > 32768.f) || !(largest <= 3.402823466e38f)) return 1.f;
-  return __int_as_float((127 + 14 - ((__float_as_int(largest) >> 23) - 127)) << 23);
+// A query's factor into f16's range, a power of two: 1 while its largest element
+// (times scale·log2 e) lies in 2^-4 .. 2^15, where two f16 parts keep every element
+// to 2^-21 of the largest (their step ends at 2^-24) at no cost; else the one that
+// brings the largest to 2^14, and each score is taken back.
+__device__ __forceinline__ float query_factor(float largest) {
+  if ((largest >= 0.0625f && largest <= 32768.f) || largest == 0.f || !(largest <= 3.402823466e38f)) return 1.f;
+  return ldexpf(1.f, min(14 - ilogbf(largest), 126));
 }
 
 struct AttnOut {
@@ -194,13 +201,13 @@ __global__ __launch_bounds__(256, token_groups(FORMAT, HD)) void k_attn_tokens(
       }
       largest = fmaxf(largest, __shfl_xor(largest, 16, 64));
       largest = fmaxf(largest, __shfl_xor(largest, 32, 64));
-      const float down = query_down(largest);
-      back = 1.f / down;
+      const float factor = query_factor(largest);
+      back = 1.f / factor;
 #pragma unroll
       for (uint32_t s = 0; s < KS; s++)
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-          const float v = in_f32(x[s][j] * down);
+          const float v = in_f32(x[s][j] * factor);
           const _Float16 hi = (_Float16)v, lo = (_Float16)(v - (float)hi);
           if constexpr (PACK) {
             qh[s][j] = col < 8 ? hi : lo;
@@ -261,15 +268,21 @@ __global__ __launch_bounds__(256, token_groups(FORMAT, HD)) void k_attn_tokens(
             if constexpr (QUANT) vs[t][i] = seen ? vs[t][i] : 0.f;
           }
       }
-      float top = -INFINITY;
+      auto highest = [&]() __attribute__((always_inline)) {
+        float top = -INFINITY;
 #pragma unroll
-      for (int t = 0; t < 2; t++)
+        for (int t = 0; t < 2; t++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) top = fmaxf(top, QUANT ? u[t][i] + scale_log(vs[t][i]) : u[t][i]);
-      if constexpr (QUANT) top -= 127.f;
+          for (int i = 0; i < 4; i++) top = fmaxf(top, QUANT ? u[t][i] + scale_log(vs[t][i]) : u[t][i]);
+        return QUANT ? top - 127.f : top;
+      };
+      float top = highest();
       if (__builtin_amdgcn_ballot_w64(top > lazy)) {
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        auto of_row = [](float x) {
+          x = fmaxf(x, __shfl_xor(x, 16, 64));
+          return fmaxf(x, __shfl_xor(x, 32, 64));
+        };
+        top = of_row(top);
         const bool move = top > lazy;  // the same in the four lanes of a row
         const float d = move ? top - kPeak : 0.f, corr = !move || lazy == kUnset ? 1.f : __builtin_amdgcn_exp2f(-d);
         m += d;
@@ -281,6 +294,16 @@ __global__ __launch_bounds__(256, token_groups(FORMAT, HD)) void k_attn_tokens(
         for (int t = 0; t < 2; t++)
 #pragma unroll
           for (int i = 0; i < 4; i++) u[t][i] -= d;
+        const bool coarse = fabsf(d) > kCoarse;
+        if (__builtin_amdgcn_ballot_w64(coarse)) {
+          top = of_row(highest());
+          const float rest = coarse ? top - kPeak : 0.f;
+          m += rest;
+#pragma unroll
+          for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) u[t][i] -= rest;
+        }
       }
       ah8_t ph, pl;
       float sum = 0.f;  // of the step, so that l takes one rounding from it
@@ -522,10 +545,10 @@ __global__ __launch_bounds__(256, chunk_groups(FORMAT, HD)) void k_attn_chunk(
         }
         return fmaxf(largest, __shfl_xor(largest, 32, 64));
       };
-      const float down = query_down(take(1.f));
-      if (__builtin_amdgcn_ballot_w64(down != 1.f)) {
-        take(down);
-        back = 1.f / down;
+      const float factor = query_factor(take(1.f));
+      if (__builtin_amdgcn_ballot_w64(factor != 1.f)) {
+        take(factor);
+        back = 1.f / factor;
       }
     }
     const bool far = __builtin_amdgcn_ballot_w64(back != 1.f) != 0;
@@ -566,9 +589,6 @@ __global__ __launch_bounds__(256, chunk_groups(FORMAT, HD)) void k_attn_chunk(
 #pragma unroll
         for (int r = 0; r < 16; r++) u[r] *= back;
       }
-      // The largest u + log2 b: key by key where some are not seen (those must
-      // change nothing), else from the largest of both.
-      float top = -INFINITY;
       auto scales = [&](const float *from, int q4) __attribute__((always_inline)) {
         const float4 a = *reinterpret_cast<const float4 *>(from + k0 + 8 * q4 + 4 * half_id);
         return af4_t{a.x, a.y, a.z, a.w};
@@ -576,18 +596,30 @@ __global__ __launch_bounds__(256, chunk_groups(FORMAT, HD)) void k_attn_chunk(
       auto seen = [&](int r) __attribute__((always_inline)) { return kb + 8 * (r / 4) + 4 * half_id + r % 4 <= pos; };
 #pragma unroll
       for (int q4 = 0; q4 < 4; q4++) {
-        af4_t a, b;
+        af4_t a;
         if constexpr (QUANT) a = scales(s_s[buf][0], q4);
-        if constexpr (QUANT && masked) b = scales(s_s[buf][1], q4);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           const int r = 4 * q4 + i;
           u[r] = QUANT ? fmaf(u[r], a[i], -m) : u[r] - m;
           if constexpr (masked) u[r] = seen(r) ? u[r] : -INFINITY;
-          top = fmaxf(top, QUANT && masked ? u[r] + scale_log(b[i]) : u[r]);
         }
       }
-      if constexpr (QUANT) top += masked ? -127.f : fmaxf(top_s[buf][k0 / 16], top_s[buf][k0 / 16 + 1]);
+      // The largest u + log2 b: key by key where some are not seen (those must
+      // change nothing), else from the largest of both.
+      auto highest = [&]() __attribute__((always_inline)) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int q4 = 0; q4 < 4; q4++) {
+          af4_t b;
+          if constexpr (QUANT && masked) b = scales(s_s[buf][1], q4);
+#pragma unroll
+          for (int i = 0; i < 4; i++) top = fmaxf(top, QUANT && masked ? u[4 * q4 + i] + scale_log(b[i]) : u[4 * q4 + i]);
+        }
+        if constexpr (QUANT) top += masked ? -127.f : fmaxf(top_s[buf][k0 / 16], top_s[buf][k0 / 16 + 1]);
+        return top;
+      };
+      float top = highest();
       if (__builtin_amdgcn_ballot_w64(top > lazy)) {
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         const bool move = top > lazy;  // the same in both lanes of a row
@@ -601,6 +633,15 @@ __global__ __launch_bounds__(256, chunk_groups(FORMAT, HD)) void k_attn_chunk(
           for (int i = 0; i < 16; i++) o[b][i] *= corr;
 #pragma unroll
         for (int r = 0; r < 16; r++) u[r] -= d;
+        const bool coarse = fabsf(d) > kCoarse;
+        if (__builtin_amdgcn_ballot_w64(coarse)) {
+          top = highest();
+          top = fmaxf(top, __shfl_xor(top, 32, 64));
+          const float rest = coarse ? top - kPeak : 0.f;
+          m += rest;
+#pragma unroll
+          for (int r = 0; r < 16; r++) u[r] -= rest;
+        }
       }
       ah8_t ph[2], pl[2];
       float sum = 0.f;  // of the tile, so that l takes one rounding from it

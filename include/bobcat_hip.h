@@ -393,9 +393,10 @@ int bch_kv_load(bch_ctx *ctx, const bch_kv_plan *plan, bch_view cache, uint32_t 
  * h / (n_heads / n_kv_heads).  `out` may not lie over `q`.  What a query does
  * not see has no part in its output, whatever it holds.  A value that it sees
  * and that is infinite or NaN makes that element of its output NaN; such a key
- * makes all of it NaN (or, where q·k is -inf, may have no weight).  The queries and the
- * probabilities enter the products with ~22 bits, as in
- * bch_attention_prefill. */
+ * makes all of it NaN (or, where q·k is -inf, may have no weight).  The
+ * queries and the probabilities enter the products with ~22 bits, as in
+ * bch_attention_prefill; scores are f32, so that of keys whose scores agree to
+ * f32's precision, far beyond 10^4, any may have the weight. */
 int bch_attention_paged(bch_ctx *ctx, const bch_kv_plan *plan, bch_view cache, bch_view q, uint32_t q_stride,
                         bch_view out, uint32_t out_stride);
 

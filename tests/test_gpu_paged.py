@@ -257,6 +257,43 @@ def test_attention_of_large_and_small_queries(hip, size, new):
     assert worst <= (attention_bound(q * size, k, v) if size < 1 else np.abs(v).max() * 2.0 ** -20), worst
 
 
+@pytest.mark.parametrize("fmt", ["i8", "f8"])
+@pytest.mark.parametrize("scale", [1e5, 1e8, 1e15])
+@pytest.mark.parametrize("new", [1, 36])
+def test_attention_of_small_queries_and_large_keys(hip, fmt, scale, new):
+    """Queries below f16's numbers, whose scores are ordinary ones; between them rows of zeros and of ordinary size
+    (whose softmax picks one key, or two that tie)."""
+    say("attention_paged small queries", fmt, scale, new)
+    rng = np.random.default_rng(10)
+    pool, batch, heads, q = case_args(rng, fmt, 4, 2, 64, 16, [(150, new)], scale)
+    q = (q / scale).astype(np.float32)
+    q[:, 1] = 0.0
+    q[::3, 2] *= np.float32(scale)
+    got = attend(hip, pool, batch, heads, q)
+    k, v = batch.gather(pool, 0)
+    want = attention(q, k, v, batch.past[0])
+    small = np.ones(q.shape[:2], bool)
+    small[::3, 2] = False
+    bound = attention_bound(np.where(small[..., None], q, 0), k, v)
+    assert np.abs(got - want)[small].max() <= bound
+    assert np.abs(got - want)[~small].max() <= np.abs(v).max() * 2.0 ** -20
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("size", [1e6, 3e7, 1e9, 1e15])
+@pytest.mark.parametrize("new", [1, 36])
+def test_attention_of_large_scores_and_values(hip, fmt, size, new):
+    """Scores whose last place in f32 is more than the room that the probabilities have, with values far above 1: each
+    query picks its best key (the next is millions below)."""
+    say("attention_paged large scores", fmt, size, new)
+    rng = np.random.default_rng(13)
+    pool, batch, heads, q = case_args(rng, fmt, 4, 2, 64, 16, [(150, new)], 100.0)
+    q *= np.float32(size)
+    got = attend(hip, pool, batch, heads, q)
+    k, v = batch.gather(pool, 0)
+    assert np.abs(got - attention(q, k, v, batch.past[0])).max() <= np.abs(v).max() * 2.0 ** -20
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("seqs", [[(20, 40)], [(100, 1), (37, 1)], [(0, 5), (64, 3)], [(10, 140)]])
 @pytest.mark.parametrize("what", ["nan", "inf"])
