@@ -14,8 +14,10 @@
 
 namespace bch {
 
-constexpr uint32_t kKvMaxPositions = (1u << 30) - 1;  // of a sequence (KvGeometry::block)
-constexpr uint32_t kKvMaxTokens = 1u << 26;  // of a batch: packed rows and workgroups then stay below 2^31
+// Positions of a sequence and new tokens of a batch: a launch has fewer than 2^32
+// threads, and kv_load and kv_store have 256 for every 16 positions and for
+// every block that receives tokens.
+constexpr uint32_t kKvMaxPositions = 1u << 27, kKvMaxTokens = 1u << 23;
 
 static int check_shape(const char *kernel, const bch_kv_shape *s) {
   if (!s) return fail(BCH_ERR_ARGUMENT, "%s: no shape", kernel);
@@ -52,7 +54,7 @@ static int check_batch(const char *kernel, const bch_kv_shape *s, uint32_t n_seq
   if (want != n_pages)
     return fail(BCH_ERR_ARGUMENT, "%s: the sequences need %llu pages, got %llu", kernel, (unsigned long long)want,
                 (unsigned long long)n_pages);
-  if (tokens > kKvMaxTokens) return fail(BCH_ERR_ARGUMENT, "%s: more than 2^26 new tokens", kernel);
+  if (tokens > kKvMaxTokens) return fail(BCH_ERR_ARGUMENT, "%s: more than 2^23 new tokens", kernel);
   uint32_t last = 0;
   for (uint64_t i = 0; i < n_pages; i++) {
     if (pages[i] >= s->n_pages)

@@ -361,8 +361,9 @@ uint64_t bch_kv_page_bytes(const bch_kv_shape *shape);
  * heads in groups of at most 32 per KV head.  BCH_ERR_UNSUPPORTED_FORMAT and
  * BCH_ERR_ATTENTION_LIMITS for the shape; BCH_ERR_OUT_OF_BOUNDS for a page
  * past the cache's; BCH_ERR_ARGUMENT for a list of another length, a sequence
- * of 2^30 positions, more than 2^26 new tokens, or a page that receives tokens and is named twice in the
- * batch (pages that are only read may be shared by sequences). */
+ * of more than 2^27 positions, more than 2^23 new tokens, or a page that
+ * receives tokens and is named twice in the batch (pages that are only read
+ * may be shared by sequences). */
 int bch_kv_plan_check(const bch_kv_shape *shape, uint32_t n_heads, uint32_t n_seqs, const uint32_t *n_past,
                       const uint32_t *n_new, const uint32_t *pages, uint64_t n_pages);
 /* A plan without a batch yet; to be freed before its context is closed. */

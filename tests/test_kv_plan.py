@@ -54,6 +54,14 @@ def test_batches_that_are_refused():
     refused("Argument", past=(40, 32), new=(3, 0), pages=((4, 7), (7,)))
 
 
+def test_batches_that_no_launch_could_take():
+    shape = kv_shape("i8", 2, 64, 512, 1 << 20)
+    kv_plan_check(shape, 8, [1 << 27], [0], [range(1 << 18)])
+    kv_plan_check(shape, 8, [0], [1 << 23], [range(1 << 14)])
+    refused("Argument", shape, 8, [1 << 27], [1], [range((1 << 18) + 1)])
+    refused("Argument", shape, 8, [0, 0], [1 << 23, 1], [range(1 << 14), [1 << 14]])
+
+
 def test_batches_that_are_allowed():
     kv_plan_check(SHAPE, 8, [], [], [])
     kv_plan_check(SHAPE, 64, [0], [0], [[]])
