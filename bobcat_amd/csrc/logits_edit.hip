@@ -81,7 +81,7 @@ __global__ __launch_bounds__(THREADS) void k_logits_edit(EditArgs a) {
       owner_s[tid + THREADS * j] = ~0u;
     }
     __syncthreads();
-    // 256 biases at a time, each in turn added by the lowest thread that has
+    // THREADS biases at a time, each in turn added by the lowest thread that has
     // one for its token: one round, or as many as a token is named.
     for (uint32_t i0 = 0; i0 < bn; i0 += THREADS) {
       const uint32_t i = i0 + tid;
@@ -122,7 +122,23 @@ extern "C" int bch_logits_edit(bch_ctx *ctx, bch_view logits, bch_view out, uint
                                const bch_logit_rules *rules) {
   if (!rules) return fail(BCH_ERR_ARGUMENT, "logits_edit: no rules");
   if (!n_vocab || n_vocab > 1u << 30) return fail(BCH_ERR_ARGUMENT, "logits_edit: rows of %u logits", n_vocab);
+  // (The kernel's places in a list and a step behind them are 32 bits.)
+  if (rules->n_history > 1u << 30 || rules->n_bias > 1u << 30)
+    return fail(BCH_ERR_ARGUMENT, "logits_edit: lists of more than 2^30 entries");
+  // Slices of 4,096 logits for long histories, of which each slice reads all, and
+  // of 2,048 for short ones, whose rows make more workgroups: 96 rows of 151,936
+  // with 2,000 tokens on average 29 us and 32, with 1 token 22 and 22; one row of
+  // 65,536 with 600 tokens 6.4 and 5.8.  (The same inputs each time; 16 logits a
+  // thread instead of eight: 39 and 42 instead of 29 and 32.)
+  const bool long_history = n_rows && rules->n_history / n_rows > 1024;
+  const uint32_t threads = long_history ? 512 : 256, slices = div_ceil(n_vocab, threads * kEditPer);
+  if ((uint64_t)n_rows * slices >= 1u << 23) return fail(BCH_ERR_ARGUMENT, "logits_edit: too many logits");
   EditArgs a{};
+  a.n_vocab = n_vocab;
+  a.n_history = rules->n_history;
+  a.n_bias = rules->n_bias;
+  a.n_masks = rules->n_masks;
+  a.slices = slices;
   const uint64_t bytes = (uint64_t)n_rows * n_vocab * 4;
   BCH_TRY(view_ptr(ctx, "logits_edit", logits, bytes, &a.logits));
   BCH_TRY(view_ptr(ctx, "logits_edit", out, bytes, &a.out));
@@ -138,21 +154,17 @@ extern "C" int bch_logits_edit(bch_ctx *ctx, bch_view logits, bch_view out, uint
                         (const void *)a.bias_tokens, (const void *)a.bias_values, (const void *)a.masks})
     if (reinterpret_cast<uintptr_t>(p) % 4) return fail(BCH_ERR_ARGUMENT, "logits_edit: operands must be 4-byte aligned");
   const uintptr_t from = reinterpret_cast<uintptr_t>(a.logits), to = reinterpret_cast<uintptr_t>(a.out);
-  if (from != to && from < to + bytes && to < from + bytes)
+  auto over = [&](const void *list, uint64_t list_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(list);
+    return x < to + bytes && to < x + list_bytes;
+  };
+  if (from != to && over(a.logits, bytes))
     return fail(BCH_ERR_ARGUMENT, "logits_edit: the outputs lie over the logits (the same place or another is wanted)");
-  a.n_vocab = n_vocab;
-  a.n_history = rules->n_history;
-  a.n_bias = rules->n_bias;
-  a.n_masks = rules->n_masks;
-  // Slices of 4,096 logits for long histories, of which each slice reads all, and
-  // of 2,048 for short ones, whose rows make more workgroups: 96 rows of 151,936
-  // with 2,000 tokens on average 29 us and 32, with 1 token 22 and 22; one row of
-  // 65,536 with 600 tokens 6.4 and 5.8.  (The same inputs each time; 16 logits a
-  // thread instead of eight: 39 and 42 instead of 29 and 32.)
-  const bool long_history = n_rows && a.n_history / n_rows > 1024;
-  const uint32_t threads = long_history ? 512 : 256;
-  a.slices = div_ceil(n_vocab, threads * kEditPer);
-  if ((uint64_t)n_rows * a.slices > 0x7fffffffu) return fail(BCH_ERR_ARGUMENT, "logits_edit: too many logits");
+  // (Slices read the lists while others write.)
+  if (over(a.rows, (uint64_t)n_rows * sizeof(bch_logit_row)) || over(a.history, (uint64_t)a.n_history * 4) ||
+      over(a.bias_tokens, (uint64_t)a.n_bias * 4) || over(a.bias_values, (uint64_t)a.n_bias * 4) ||
+      over(a.masks, (uint64_t)a.n_masks * ((n_vocab + 31) / 32) * 4))
+    return fail(BCH_ERR_ARGUMENT, "logits_edit: the outputs lie over the rules");
   return launch(ctx, {"logits_edit", n_rows, n_vocab, 0}, [&](hipStream_t s) {
     if (!n_rows) return;
     if (long_history)

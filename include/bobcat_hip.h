@@ -467,7 +467,10 @@ typedef struct bch_logit_rules {
  * occurs; bch_sample's penalty takes the last 64 tokens and no counts.
  * Tokens that are not below n_vocab change nothing, lists end where their
  * buffers' entries do, and a mask that is not below n_masks (other than
- * BCH_NO_MASK) allows nothing.  No counterpart in the reference. */
+ * BCH_NO_MASK) allows nothing.  `out` may not lie over the rules; lists of at
+ * most 2^30 entries, and fewer than 2^23 pieces of 2,048 logits (4,096 where
+ * the rows have more than 1,024 tokens of history on average).  No counterpart
+ * in the reference. */
 int bch_logits_edit(bch_ctx *ctx, bch_view logits, bch_view out, uint32_t n_rows, uint32_t n_vocab,
                     const bch_logit_rules *rules);
 

@@ -145,6 +145,16 @@ def test_refusals(hip):
     refused("OutOfBounds", b.at(0), b.at(2048), 1, 33, rows.at(0), masks=b.at(4092), n_masks=1)
     refused("Argument", b.at(0), b.at(2048), 1, 33, rows.at(0), n_history=4)  # a list without a view
     refused("Argument", b.at(0), b.at(2048), 1, 33, rows.at(0), n_bias=4, bias_tokens=b.at(0))
+    refused("Argument", b.at(0), b.at(2048), 1, 33, rows.at(0), n_history=(1 << 30) + 1, history=b.at(0))
+    refused("Argument", b.at(0), b.at(2048), 1, 33, rows.at(0), n_bias=(1 << 30) + 1, bias_tokens=b.at(0), bias_values=b.at(0))
+    refused("Argument", b.at(0), b.at(0), 1 << 23, 33, rows.at(0))
+    # The outputs over each of the rules.
+    refused("Argument", b.at(0), rows.at(64), 1, 10, rows.at(64))
+    for at in (2048, 2048 + 4 * 32):
+        refused("Argument", b.at(0), b.at(2048), 1, 33, rows.at(0), n_history=4, history=b.at(at))
+        refused("Argument", b.at(0), b.at(2048), 1, 33, rows.at(0), n_bias=4, bias_tokens=b.at(at), bias_values=b.at(0))
+        refused("Argument", b.at(0), b.at(2048), 1, 33, rows.at(0), n_bias=4, bias_tokens=b.at(0), bias_values=b.at(at))
+        refused("Argument", b.at(0), b.at(2048), 1, 33, rows.at(0), n_masks=1, masks=b.at(at))
     hip.begin()
     hip.logits_edit(b.at(0), b.at(0), 0, 33, rows.at(0))
     hip.end()
