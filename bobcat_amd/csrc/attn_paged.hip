@@ -754,11 +754,14 @@ __global__ __launch_bounds__(256, chunk_groups(FORMAT, HD)) void k_attn_chunk(
 
 // The rows of tiles whose keys were split, from the splits' records.  HD / 4
 // threads read a record; `parts` (a power of two) such groups have every
-// parts-th of a row's records each, eight in flight, and meet in LDS.
+// parts-th of a row's records each and meet in LDS.  Bound by latency (the item,
+// then its records): 4.3 us for rows of up to 16 pieces.  Eight records in flight
+// each, three where there are no more: 50 wide and some narrow tiles of heads of
+// 128, 58 MB of records, 28 us instead of 32.
 template <uint32_t HD>
 __global__ __launch_bounds__(256) void k_attn_join(const KvJoinItem *__restrict__ items, uint32_t n_kv, uint32_t group,
                                                    uint32_t parts, AttnOut to) {
-  constexpr uint32_t N = 8, WIDE = HD / 4, GROUPS = 256 / WIDE;
+  constexpr uint32_t WIDE = HD / 4, GROUPS = 256 / WIDE;
   __shared__ float4 acc_s[GROUPS][WIDE];
   __shared__ float2 ml_s[GROUPS];
   const KvJoinItem it = items[blockIdx.x];
@@ -775,28 +778,35 @@ __global__ __launch_bounds__(256) void k_attn_join(const KvJoinItem *__restrict_
     acc.x = fmaf(x.x, f, acc.x), acc.y = fmaf(x.y, f, acc.y), acc.z = fmaf(x.z, f, acc.z), acc.w = fmaf(x.w, f, acc.w);
     sum = fmaf(l, f, sum);
   };
-  for (uint32_t s0 = part; s0 < it.splits; s0 += N * parts) {
-    float2 ml[N];
-    float4 x[N];
+  auto take = [&](auto in_flight) __attribute__((always_inline)) {
+    constexpr uint32_t N = decltype(in_flight)::value;
+    for (uint32_t s0 = part; s0 < it.splits; s0 += N * parts) {
+      float2 ml[N];
+      float4 x[N];
 #pragma unroll
-    for (uint32_t j = 0; j < N; j++) {
-      const float *r = p + min(s0 + j * parts, it.splits - 1) * apart;
-      ml[j] = *reinterpret_cast<const float2 *>(r + HD);
-      x[j] = *reinterpret_cast<const float4 *>(r + d);
+      for (uint32_t j = 0; j < N; j++) {
+        const float *r = p + min(s0 + j * parts, it.splits - 1) * apart;
+        ml[j] = *reinterpret_cast<const float2 *>(r + HD);
+        x[j] = *reinterpret_cast<const float4 *>(r + d);
+      }
+      float next = top;
+#pragma unroll
+      for (uint32_t j = 0; j < N; j++) next = fmaxf(next, ml[j].x);
+      const float f0 = weight(top, next);
+      top = next;
+      sum *= f0;
+      acc.x *= f0, acc.y *= f0, acc.z *= f0, acc.w *= f0;
+#pragma unroll
+      for (uint32_t j = 0; j < N; j++) {
+        if (s0 + j * parts >= it.splits) break;
+        add(weight(ml[j].x, top), x[j], ml[j].y);
+      }
     }
-    float next = top;
-#pragma unroll
-    for (uint32_t j = 0; j < N; j++) next = fmaxf(next, ml[j].x);
-    const float f0 = weight(top, next);
-    top = next;
-    sum *= f0;
-    acc.x *= f0, acc.y *= f0, acc.z *= f0, acc.w *= f0;
-#pragma unroll
-    for (uint32_t j = 0; j < N; j++) {
-      if (s0 + j * parts >= it.splits) break;
-      add(weight(ml[j].x, top), x[j], ml[j].y);
-    }
-  }
+  };
+  if (it.splits <= 3 * parts)
+    take(std::integral_constant<uint32_t, 3>{});
+  else
+    take(std::integral_constant<uint32_t, 8>{});
   if (parts > 1) {
     acc_s[mine][lane] = acc;
     if (lane == 0) ml_s[mine] = {top, sum};
