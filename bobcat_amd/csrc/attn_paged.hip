@@ -6,14 +6,19 @@
 // The query heads of a KV head's group and a sequence's tokens are one list of
 // packed rows, row = token·group + head: every row of a tile reads the same
 // keys, whatever the group.  Two kernels share the mathematics:
-//   k_attn_tokens: sequences of at most 16 packed rows (decoding, drafts).  A
-//     wave takes 32 keys at a time from memory straight into the operands of
-//     16x16x32 MFMAs; the waves of a workgroup, and the splits of a sequence,
-//     have keys of their own and are joined.  Bound by the cache's bytes.
+//   k_attn_tokens: tiles of at most 16 packed rows (decoding, drafts, short
+//     chunks).  A wave takes 32 keys at a time from memory straight into the
+//     operands of 16x16x32 MFMAs, with no barrier in its loop; the waves of a
+//     workgroup, and the pieces of a tile, have keys of their own and are joined.
+//     Bound by the cache's bytes: 64 sequences of up to 16,384 int8 positions, 8
+//     KV heads of 64, 97 us (5.5 TB/s; with the join 103), 16 of up to 32,768 in
+//     f16 86 us; one short sequence by latency (600 positions 6.9 us).
 //   k_attn_chunk: tiles of 128 packed rows, 32 a wave, that share the keys
-//     through LDS.  Bound by the matrix cores and the softmax's instructions.
-// (The rule: with 16 rows or fewer the narrow tile wastes no matrix work and
-// needs no barrier; above, the wide one reads the cache once for 128 rows.)
+//     through LDS.  Bound by the clock that the matrix cores' work leaves and by
+//     what they wait for between the softmax's instructions: 965 TFLOP/s with
+//     heads of 128 (both parts counted; a large library product reaches 1,222),
+//     the matrix cores busy 48% of the cycles.
+// kv_schedule says which of a batch's sequences take which.
 //
 // Scores come as S^T = K·Q^T (keys x rows), so that a lane holds scores of one
 // row, and as probabilities they are in place as an operand of O^T = V^T·P^T.
@@ -130,7 +135,7 @@ constexpr uint32_t chunk_groups(uint32_t format, uint32_t hd) {
   return hd == 64 ? (format == BCH_KV_F16 ? 2 : 3) : hd == 128 ? 2 : 1;
 }
 
-// --- at most 16 packed rows ---------------------------------------------------
+// --- tiles of at most 16 packed rows ---------------------------------------------------
 
 // ROWS 8: the high parts of the queries and probabilities are the operands'
 // columns 0..7, the low parts columns 8..15, so one MFMA does both and the
@@ -161,7 +166,8 @@ __global__ __launch_bounds__(256, token_groups(FORMAT, HD)) void k_attn_tokens(
       float4 s[2];
     } kr, vr;
     auto block = [&](uint32_t step, int t) {
-      return g.block<BYTES>(g.page(it.table, min(2 * step + t, last)), min(2 * step + t, last), kv);  // (past the end: the last block, masked)
+      const uint32_t b = min(2 * step + t, last);  // (past the end: the last block, masked)
+      return g.block<BYTES>(g.page(it.table, b), b, kv);
     };
     auto load = [&](Raw &raw, uint32_t step, uint32_t part) __attribute__((always_inline)) {
 #pragma unroll
@@ -410,7 +416,7 @@ __global__ __launch_bounds__(256, token_groups(FORMAT, HD)) void k_attn_tokens(
   }
 }
 
-// --- more rows ------------------------------------------------------------------
+// --- tiles of 128 packed rows ------------------------------------------------------------------
 
 // Keys of a step: what the registers that bring the next step's hold.
 constexpr uint32_t chunk_keys(uint32_t format, uint32_t hd) { return hd == 256 || (hd == 128 && format == BCH_KV_F16) ? 32 : 64; }
@@ -1007,9 +1013,9 @@ KvSchedule kv_schedule(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t 
   deal(w, w.tiles8, narrow, few_groups, 8, longest <= unsplit, 4, n_kv, 1, records);
   deal(w, w.tiles16, tokens, few_groups, 8, longest <= unsplit, 4, n_kv, 1, records);
   const uint32_t keys = chunk_keys(format, head_dim);
-  // Wide tiles: four trips of the loop at least.  What starting one costs showed in prompts without a past, 2,048
-  // tokens in 64 tiles of 1 to 64 steps (heads of 128): 156 us counted as 4
-  // steps, 114 as 10.
+  // Wide tiles: four trips of the loop at least.  What starting one costs showed
+  // in prompts without a past, 2,048 tokens in 64 tiles of 1 to 64 steps (heads of
+  // 128): 156 us counted as 4 steps, 114 as 10.
   deal(w, w.chunks, chunks, (uint64_t)n_cus * chunk_groups(format, head_dim) / n_kv, keys / 8, false, 10, n_kv,
        keys / 32, records);
   return w;
