@@ -33,6 +33,7 @@
 // nothing.
 #include <algorithm>
 #include <cmath>
+#include <numeric>
 
 #include "device.h"
 #include "kernels.h"
@@ -891,6 +892,39 @@ struct Dealer {
   }
 };
 
+// Workgroups go to the eight XCDs in turn, so those of a KV head to
+// 8 / gcd(8, n_kv) of them.  Puts the pieces of a sequence's tiles that read the
+// same keys on one XCD, whose L2 then has them for all but the first.
+static void keep_together(std::vector<KvAttnItem> &items, uint32_t n_kv) {
+  const uint32_t xcds = 8 / std::gcd(8u, n_kv);
+  if (xcds == 1) return;
+  struct Piece {
+    uint32_t row, number;
+    KvAttnItem it;
+  };
+  std::vector<Piece> pieces;
+  pieces.reserve(items.size());
+  for (const KvAttnItem &it : items) {
+    const bool same = !pieces.empty() && pieces.back().row == it.row && pieces.back().it.first == it.first;
+    pieces.push_back({it.row, same ? pieces.back().number + 1 : 0, it});
+  }
+  auto before = [](const Piece &a, const Piece &b) { return a.row != b.row ? a.row < b.row : a.number < b.number; };
+  std::stable_sort(pieces.begin(), pieces.end(), before);
+  std::vector<KvAttnItem> of[8];
+  uint32_t to = 0;
+  for (size_t i = 0; i < pieces.size(); i++) {
+    if (!i || before(pieces[i - 1], pieces[i])) {
+      for (uint32_t x = to = 0; x < xcds; x++)
+        if (of[x].size() < of[to].size()) to = x;
+    }
+    of[to].push_back(pieces[i].it);
+  }
+  items.clear();
+  for (size_t i = 0; items.size() < pieces.size(); i++)
+    for (uint32_t x = 0; x < xcds; x++)
+      if (i < of[x].size()) items.push_back(of[x][i]);
+}
+
 static void deal(KvSchedule &w, KvWork &work, const std::vector<Tile> &tiles, uint64_t most, uint32_t least, bool whole,
                  uint64_t start, uint32_t n_kv, uint32_t granule, uint64_t records) {
   work.starts.push_back(0);
@@ -1012,6 +1046,13 @@ KvSchedule kv_schedule(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t 
   const uint64_t few_groups = (uint64_t)n_cus * (head_dim == 256 ? 1 : token_groups(format, head_dim)) / n_kv;
   deal(w, w.tiles8, narrow, few_groups, 8, longest <= unsplit, 4, n_kv, 1, records);
   deal(w, w.tiles16, tokens, few_groups, 8, longest <= unsplit, 4, n_kv, 1, records);
+  // Where a workgroup has one item, the order is free.  (Heads of 256, 12 sequences
+  // of 20 rows and 4,096 keys: 18.1 us instead of 19.5, of 64 rows and 2,000 keys
+  // 18.7 instead of 19.8.  Smaller heads take fewer bytes a CU at a time and gain
+  // nothing: of 128, 20 rows, 15.5 instead of 15.0, of 64 12.3 and 12.3.)
+  if (head_dim == 256)
+    for (KvWork *work : {&w.tiles8, &w.tiles16})
+      if (work->items.size() < work->starts.size()) keep_together(work->items, n_kv);
   const uint32_t keys = chunk_keys(format, head_dim);
   // Wide tiles: four trips of the loop at least.  What starting one costs showed
   // in prompts without a past, 2,048 tokens in 64 tiles of 1 to 64 steps (heads of
