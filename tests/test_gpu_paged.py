@@ -349,6 +349,38 @@ def test_attention_probabilities(hip, fmt, new):
         row += new
 
 
+@pytest.mark.parametrize("fmt,hd", [("i8", 64), ("f16", 128), ("f8", 256)])
+@pytest.mark.parametrize("many", ["tokens", "chunks"])
+def test_attention_of_many_sequences(hip, fmt, hd, many):
+    """More tiles than workgroups run at once: a workgroup has several, and pieces of some."""
+    say("attention_paged many", fmt, hd, many)
+    rng = np.random.default_rng(14)
+    if many == "tokens":
+        seqs = [(int(n), 1) for n in rng.integers(0, 40, 260)] + [(1500, 1)]
+        pool, batch, heads, q = case_args(rng, fmt, 16, 8, hd, 16, seqs)
+    else:
+        seqs = [(int(n), 17) for n in rng.integers(0, 60, 66)] + [(900, 20)]
+        pool, batch, heads, q = case_args(rng, fmt, 64, 8, hd, 32, seqs)
+    check_attention(hip, pool, batch, heads, q)
+
+
+@pytest.mark.parametrize("seqs", [[], [(0, 0)], [(40, 0), (0, 0), (16, 0)]])
+def test_batches_without_tokens(hip, seqs):
+    rng = np.random.default_rng(15)
+    batch = Batch(rng, seqs, 16)
+    pool = Pool("i8", 2, 64, 16, batch.n_pages)
+    batch.fill(rng, pool)
+    cache, plan, b = hip.buffer_from(pool.bytes), plan_of(hip, pool, batch, 4), hip.buffer_from(np.full(1024, 7.0, np.float32))
+
+    def step():
+        hip.kv_store(plan, cache.at(0), b.at(0), 128, b.at(0), 128)
+        hip.attention_paged(plan, cache.at(0), b.at(0), 256, b.at(2048), 256)
+
+    run(hip, step)
+    assert np.array_equal(hip.read(cache.at(0), np.empty_like(pool.bytes)), pool.bytes)
+    assert (hip.read(b.at(0), np.empty(1024, np.float32)) == 7.0).all()
+
+
 def test_attention_shared_prefix_and_changed_batches(hip):
     """Sequences that share pages, a plan that is given another batch, and batches without tokens."""
     rng = np.random.default_rng(13)
