@@ -113,14 +113,18 @@ struct AttnOut {
   float *partials;  // records of hd + 4 floats: O, the reference m, l
 };
 
-// One record or output quad: elements d .. d + 3 of a row with O, m and l.
+// One record or output quad: elements d .. d + 3 of a row with O, m and l.  An
+// infinite f16 value times a probability's two parts is an infinity or, where
+// the low part is 0 or of the other sign, NaN: outputs that see one are NaN
+// either way.  (Nothing else makes O infinite: values are below 2^68.)
 template <uint32_t HD>
 __device__ __forceinline__ void put_row(const AttnOut &o, uint32_t part, uint32_t record, uint64_t row, uint32_t head, uint32_t d,
                                         float4 acc, float m, float l) {
   if (part == ~0u) {
     const float inv = 1.f / l;
+    auto finite = [](float x) { return fabsf(x) <= 3.402823466e38f ? x : NAN; };
     *reinterpret_cast<float4 *>(o.out + row * o.stride + (uint64_t)head * HD + d) =
-        float4{acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+        float4{finite(acc.x * inv), finite(acc.y * inv), finite(acc.z * inv), finite(acc.w * inv)};
   } else {
     float *p = o.partials + ((uint64_t)part + record) * (HD + 4);
     *reinterpret_cast<float4 *>(p + d) = acc;
