@@ -1104,6 +1104,7 @@ extern "C" int bch_attention_paged(bch_ctx *ctx, const bch_kv_plan *plan, bch_vi
   }
   return launch(ctx, {"attention_paged", plan->n_tokens, width, 0}, [&](hipStream_t st) {
     if (!plan->n_tokens) return;
+    kv_plan_use(ctx, plan);
     const KvGeometry geo = plan->geometry(cp);
     const AttnOut to{op, out_stride, ctx->attn_partials};
     const uint32_t n_kv = s.n_kv_heads, group = plan->n_heads / n_kv;

@@ -133,8 +133,7 @@ struct bch_kv_plan {
   bch_kv_shape shape;
   uint32_t n_heads;
   bool ready = false;  // bch_kv_plan_set has succeeded
-  // The ticket of the last recording that used the plan (the open one's
-  // next): its launches read the plan's memory until it has been waited for.
+  // The last recording whose launches read the plan's memory (bch_ctx::begun).
   mutable uint64_t last_use = 0;
   uint32_t n_seqs = 0, n_tokens = 0;
   std::vector<bch::KvSeq> seqs;
@@ -161,8 +160,10 @@ struct bch_kv_plan {
 
 namespace bch {
 // The plan of a recorded op: BCH_OK if it belongs to ctx, is ready, and the
-// view `cache` holds its pages, whose address goes to *ptr; notes the use.
+// view `cache` holds its pages, whose address goes to *ptr.
 int kv_plan_cache(bch_ctx *ctx, const char *kernel, const bch_kv_plan *plan, bch_view cache, void **ptr);
+// Notes that the open recording has launches that read the plan's memory.
+void kv_plan_use(const bch_ctx *ctx, const bch_kv_plan *plan);
 // Rows of `width` floats, `stride` apart, one for each of the plan's tokens.
 int kv_plan_rows(bch_ctx *ctx, const char *kernel, const bch_kv_plan *plan, bch_view view, uint32_t width,
                  uint32_t stride, float **ptr);

@@ -87,9 +87,10 @@ int kv_plan_cache(bch_ctx *ctx, const char *kernel, const bch_kv_plan *plan, bch
   if (!plan->ready) return fail(BCH_ERR_ARGUMENT, "%s: the plan has no batch", kernel);
   BCH_TRY(check_view(ctx, kernel, cache, bch_kv_page_bytes(&plan->shape) * plan->shape.n_pages, ptr));
   if (reinterpret_cast<uintptr_t>(*ptr) % 16) return fail(BCH_ERR_ARGUMENT, "%s: the cache must be 16-byte aligned", kernel);
-  plan->last_use = ctx->committed + 1;
   return BCH_OK;
 }
+
+void kv_plan_use(const bch_ctx *ctx, const bch_kv_plan *plan) { plan->last_use = ctx->begun; }
 
 int kv_plan_rows(bch_ctx *ctx, const char *kernel, const bch_kv_plan *plan, bch_view view, uint32_t width,
                  uint32_t stride, float **ptr) {
@@ -145,8 +146,8 @@ static int plan_set(bch_kv_plan *plan, uint32_t n_seqs, const uint32_t *n_past, 
 
   plan->ready = false;
   // Launches of a recording that was discarded have no ticket and may still
-  // read the last batch.
-  if (plan->last_use > plan->ctx->committed && hipStreamSynchronize(plan->ctx->stream) != hipSuccess)
+  // read the last batch.  (Where a later one was waited for they have run.)
+  if (plan->last_use > plan->ctx->finished && hipStreamSynchronize(plan->ctx->stream) != hipSuccess)
     return fail(BCH_ERR_EXECUTION, "kv_plan_set: the stream failed");
   plan->last_use = 0;
   if (all.bytes.size() > plan->memory_bytes) {
@@ -243,7 +244,9 @@ int bch_kv_plan_set(bch_kv_plan *plan, uint32_t n_seqs, const uint32_t *n_past, 
   if (!plan) return fail(BCH_ERR_ARGUMENT, "kv_plan_set: no plan");
   // In the open recording, or in one that has not been waited for.
   const bch_ctx *ctx = plan->ctx;
-  if (plan->last_use > ctx->waited && (plan->last_use <= ctx->committed || ctx->recording))
+  bool busy = ctx->recording && plan->last_use == ctx->begun;
+  for (const bch_ctx::Pending &p : ctx->pending) busy |= plan->last_use == p.recording;
+  if (busy)
     return fail(BCH_ERR_BUSY, "kv_plan_set: the batch cannot change while work that uses it is in flight");
   BCH_TRY(bch_kv_plan_check(&plan->shape, plan->n_heads, n_seqs, n_past, n_new, pages, n_pages));
   try {

@@ -201,6 +201,7 @@ extern "C" int bch_kv_store(bch_ctx *ctx, const bch_kv_plan *plan, bch_view cach
     return fail(BCH_ERR_ARGUMENT, "kv_store: the rows lie over the cache");
   return launch(ctx, {"kv_store", plan->n_tokens, width, 0}, [&](hipStream_t st) {
     if (!plan->n_store) return;
+    kv_plan_use(ctx, plan);
     kv_dispatch(s.format, s.head_dim, [&](auto format, auto hd) {
       k_kv_store<decltype(format)::value, decltype(hd)::value><<<dim3(plan->n_store, s.n_kv_heads), kStoreThreads, 0, st>>>(
           plan->d_store, static_cast<uint8_t *>(cp), s.page_size / kKvBlock, s.n_kv_heads, kp, k_stride, vp, v_stride);
@@ -229,6 +230,7 @@ extern "C" int bch_kv_load(bch_ctx *ctx, const bch_kv_plan *plan, bch_view cache
     return fail(BCH_ERR_ARGUMENT, "kv_load: the keys, the values and the cache lie over each other");
   return launch(ctx, {"kv_load", n, s.n_kv_heads * s.head_dim, 0}, [&](hipStream_t st) {
     if (!n) return;
+    kv_plan_use(ctx, plan);
     const uint32_t blocks = (first + n - 1) / kKvBlock - first / kKvBlock + 1;
     kv_dispatch(s.format, s.head_dim, [&](auto format, auto hd) {
       k_kv_load<decltype(format)::value, decltype(hd)::value><<<dim3(blocks, s.n_kv_heads), kStoreThreads, 0, st>>>(

@@ -25,9 +25,14 @@ struct bch_ctx {
   // Tickets: commit k records events[k-1-first_event]; wait drains them.
   uint64_t committed = 0;
   uint64_t waited = 0;
+  // Recordings begun, the open one's number among them, and the last of which
+  // the host knows that all work up to it has run.
+  uint64_t begun = 0;
+  uint64_t finished = 0;
   hipEvent_t begin_event = nullptr;  // recorded at bch_begin
   struct Pending {
     uint64_t ticket;
+    uint64_t recording;
     hipEvent_t begin;
     hipEvent_t end;
   };

@@ -220,6 +220,7 @@ int bch_begin(bch_ctx *ctx) {
   if (!ctx->begin_event) hipEventCreate(&ctx->begin_event);
   hipEventRecord(ctx->begin_event, ctx->stream);
   ctx->recording = true;
+  ctx->begun++;
   return BCH_OK;
 }
 
@@ -233,6 +234,7 @@ int bch_commit(bch_ctx *ctx, uint64_t *ticket) {
   if (!ctx->recording) return fail(BCH_ERR_NOT_RECORDING, "no recording is open");
   bch_ctx::Pending p;
   p.ticket = ++ctx->committed;
+  p.recording = ctx->begun;
   hipEventCreate(&p.begin);
   hipEventCreate(&p.end);
   // The event recorded at bch_begin marks this ticket's start; the fresh
@@ -259,6 +261,7 @@ int bch_wait(bch_ctx *ctx, uint64_t ticket, double *gpu_seconds) {
     hipEventDestroy(p.begin);
     hipEventDestroy(p.end);
     if (p.ticket > ctx->waited) ctx->waited = p.ticket;
+    if (p.recording > ctx->finished) ctx->finished = p.recording;
   }
   if (ticket > ctx->waited && ticket <= ctx->committed) ctx->waited = ticket;
   if (gpu_seconds) *gpu_seconds = total;
