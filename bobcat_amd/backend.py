@@ -10,12 +10,13 @@ from __future__ import annotations
 
 import ctypes as C
 import weakref
+from array import array
 from dataclasses import dataclass
 from enum import IntEnum
 
 import numpy as np
 
-from ._lib import BobcatError, KvShape, LogitRules, Norm as _Norm, ProfileEntry, View as _View, check, lib
+from ._lib import BobcatError, KvShape, LogitRules, Norm as _Norm, ProfileEntry, STATUS, View as _View, check, lib
 
 
 class Format(IntEnum):
@@ -114,18 +115,37 @@ def kv_page_bytes(shape: KvShape) -> int:
     return lib().bch_kv_page_bytes(C.byref(shape))
 
 
-def _batch(n_past, n_new, pages):
+def _u32(lists, what: str) -> np.ndarray:
+    """The whole numbers below 2^32 of lists or arrays, one behind the other, as the library takes them."""
+    out = array("I")  # (refuses others)
+    try:
+        for numbers in lists:
+            out.extend(numbers.tolist() if isinstance(numbers, np.ndarray) else numbers)
+    except (TypeError, OverflowError) as e:
+        raise ValueError(f"{what} are whole numbers below 2^32") from e
+    return np.frombuffer(out, np.uint32) if out else np.empty(0, np.uint32)
+
+
+def _batch(shape: KvShape, n_past, n_new, pages):
     """A batch's arguments: lengths, and each sequence's pages one list after the other."""
-    past, new = np.ascontiguousarray(n_past, np.uint32), np.ascontiguousarray(n_new, np.uint32)
-    if past.shape != new.shape or past.ndim != 1:
+    past, new = _u32([n_past], "lengths"), _u32([n_new], "lengths")
+    if past.shape != new.shape:
         raise ValueError("n_past and n_new hold one number for each sequence")
-    flat = np.ascontiguousarray([p for seq in pages for p in seq], np.uint32)
+    # (The library sees one list and would deal it out anew.)
+    page = max(shape.page_size, 1)
+    need, have = [-(-(p + n) // page) for p, n in zip(past.tolist(), new.tolist())], [len(seq) for seq in pages]
+    if need != have:
+        if len(need) != len(have):
+            raise BobcatError(STATUS["Argument"], f"{len(have)} lists of pages for {len(need)} sequences")
+        at = next(i for i in range(len(need)) if need[i] != have[i])
+        raise BobcatError(STATUS["Argument"], f"sequence {at} needs {need[at]} pages, got {have[at]}")
+    flat = _u32(pages, "pages")
     return past, new, flat, (past.size, past.ctypes.data, new.ctypes.data, flat.ctypes.data, flat.size)
 
 
 def kv_plan_check(shape: KvShape, n_heads: int, n_past, n_new, pages) -> None:
     """Raise what KvPlan and its set() would, without a device."""
-    *_keep, args = _batch(n_past, n_new, pages)
+    *_keep, args = _batch(shape, n_past, n_new, pages)
     check(lib().bch_kv_plan_check(C.byref(shape), n_heads, *args))
 
 
@@ -139,8 +159,9 @@ class KvPlan:
         hip._dependents.add(self)
 
     def set(self, n_past, n_new, pages) -> None:
-        """The batch: past positions and new tokens of each sequence, and each sequence's list of pages."""
-        *_keep, args = _batch(n_past, n_new, pages)
+        """The batch: past positions and new tokens of each sequence, and each sequence's list of pages
+        (ceil((past + new) / page_size) of them)."""
+        *_keep, args = _batch(self.shape, n_past, n_new, pages)
         check(lib().bch_kv_plan_set(self.handle, *args))
 
     def close(self) -> None:
