@@ -330,8 +330,9 @@ int bch_moe_combine(bch_ctx *ctx, bch_view x, bch_view route, bch_view y, uint32
 /* The rows x of a position and head are kept as f16, or with a scale of */
 /* their own: s = clamp(max|x|·(1/top), 2^-40, 2^60), y = x / s rounded  */
 /* to the nearest int8 (top 127) or e4m3 (top 448), ties to even, and    */
-/* read back as s·y (1/top, s and x / s are f32).  A row with a NaN or   */
-/* an infinity reads back as NaN.                                        */
+/* read back as s·y (1/top, s and x / s are f32).  In the 8-bit formats  */
+/* a row with a NaN or an infinity reads back as NaN, all of it; in f16  */
+/* each element reads back as its own f16 (from 65,520 on an infinity).  */
 /*                                                                      */
 /* Layout, for programs that move pages: a page is [head][16 positions], */
 /* a block of 16 positions of a head its keys, its values and (8-bit     */
@@ -397,7 +398,9 @@ int bch_kv_load(bch_ctx *ctx, const bch_kv_plan *plan, bch_view cache, uint32_t 
  * makes all of it NaN (or, where q·k is -inf, may have no weight).  The
  * queries and the probabilities enter the products with ~22 bits, as in
  * bch_attention_prefill; scores are f32, so that of keys whose scores agree to
- * f32's precision, far beyond 10^4, any may have the weight. */
+ * f32's precision, far beyond 10^4, any may have the weight.  A probability
+ * (times its value row's scale) ends at 2^-33 of the query's largest: what n keys
+ * below that add to an output, up to n·2^-33 of the largest value, is lost. */
 int bch_attention_paged(bch_ctx *ctx, const bch_kv_plan *plan, bch_view cache, bch_view q, uint32_t q_stride,
                         bch_view out, uint32_t out_stride);
 
@@ -448,7 +451,8 @@ typedef struct bch_logit_row {
 } bch_logit_row;
 
 /* The lists that the rows share, in device memory; a list of no entries
- * needs no view. */
+ * needs no view.  (bch_write is refused while work is in flight: a program with
+ * steps queued writes the next step's rows and lists from the device, or waits.) */
 typedef struct bch_logit_rules {
   bch_view rows;                     /* n_rows bch_logit_row */
   bch_view history;                  /* u32 tokens */

@@ -1,12 +1,14 @@
-"""Infinities in f16 value rows: an element that a query sees makes that element
-of its output NaN wherever it lies among the steps, and changes no other."""
+"""Infinities in f16 rows: each is its element's alone in the cache, and one that
+a query sees among its values makes that element of its output NaN, wherever it
+lies among the steps, and changes no other."""
 from __future__ import annotations
 
 import numpy as np
 import pytest
 
+from _paged import Batch, Pool
 from _paged_bounds import case
-from test_gpu_paged import attend, say
+from test_gpu_paged import attend, plan_of, say
 
 pytestmark = pytest.mark.gpu
 
@@ -30,3 +32,24 @@ def test_an_infinite_value_makes_its_element_nan(hip, hd, past, new, value):
     spoilt = np.broadcast_to(spoilt[:, None], after.shape)
     assert np.isnan(after[spoilt]).all()
     assert np.array_equal(after[~spoilt], before[~spoilt])
+
+
+def test_f16_rows_read_back_element_by_element(hip):
+    """A NaN or an infinity is that element's alone, also one that comes from a finite number past f16's end."""
+    rng = np.random.default_rng(6)
+    kv, hd, page = 2, 64, 16
+    batch = Batch(rng, [(0, 20)], page)
+    pool = Pool("f16", kv, hd, page, batch.n_pages)
+    x = rng.standard_normal((20, kv, hd)).astype(np.float32)
+    x[3, 0, 5], x[4, 1, 6], x[5, 0, 7], x[6, 1, 8], x[7, 0, 9] = np.nan, np.inf, -np.inf, 65520.0, 65519.0
+    cache, plan, xb = hip.buffer_from(pool.bytes), plan_of(hip, pool, batch, kv), hip.buffer_from(x)
+    out = [hip.new_buffer(x.nbytes) for _ in range(2)]
+    hip.begin()
+    hip.kv_store(plan, cache.at(0), xb.at(0), kv * hd, xb.at(0), kv * hd)
+    hip.kv_load(plan, cache.at(0), 0, 0, 20, out[0].at(0), out[1].at(0))
+    hip.end()
+    with np.errstate(over="ignore"):
+        want = x.astype(np.float16).astype(np.float32)
+    assert np.isinf(want).sum() == 3 and np.isnan(want).sum() == 1
+    for buffer in out:
+        assert np.array_equal(hip.read(buffer.at(0), np.empty_like(x)), want, equal_nan=True)
