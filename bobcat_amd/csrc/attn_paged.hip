@@ -11,13 +11,14 @@
 //     operands of 16x16x32 MFMAs, with no barrier in its loop; the waves of a
 //     workgroup, and the pieces of a tile, have keys of their own and are joined.
 //     Bound by the cache's bytes: 64 sequences of up to 16,384 int8 positions, 8
-//     KV heads of 64, 97 us (5.5 TB/s; with the join 103), 16 of up to 32,768 in
-//     f16 86 us; one short sequence by latency (600 positions 6.9 us).
+//     KV heads of 64, 99 us (5.4 TB/s; with the join 103), 16 of up to 32,768 in
+//     f16 86 us; one short sequence by latency (600 positions 7.0 us).
 //   k_attn_chunk: tiles of 128 packed rows, 32 a wave, that share the keys
 //     through LDS.  Bound by the clock that the matrix cores' work leaves and by
-//     what they wait for between the softmax's instructions: 965 TFLOP/s with
-//     heads of 128 (both parts counted; a large library product reaches 1,222),
-//     the matrix cores busy 48% of the cycles.
+//     what they wait for between the softmax's instructions: two prompts of up to
+//     1,024 tokens over 16,384 int8 keys, 32 heads of 128, 780-800 us, 950-975
+//     TFLOP/s (both parts counted; a large library product reaches 1,200), the
+//     matrix cores busy 46% of the cycles.
 // kv_schedule says which of a batch's sequences take which.
 //
 // Scores come as S^T = K·Q^T (keys x rows), so that a lane holds scores of one
@@ -29,7 +30,7 @@
 //   u = a·s − m,  p = 2^u,  l += p,  O += (p·b)·v,
 // where m follows the largest u + log2 b: p·b then stays inside f16's range,
 // whatever the scales, and p needs no bound of its own (scales lie in 2^-40 ..
-// 2^60).  m moves only when p·b would leave its range, so most steps rescale
+// 2^60).  m moves only when p·b could leave its range, so most steps rescale
 // nothing.
 #include <algorithm>
 #include <cmath>
@@ -132,7 +133,9 @@ __device__ __forceinline__ void put_row(const AttnOut &o, uint32_t part, uint32_
   }
 }
 
-// Workgroups of a CU that the registers let run at once.
+// Workgroups of a CU that the registers let run at once.  (Up to 17 registers of
+// the wide tiles and four of the narrow ones are spilled for it, where an item
+// begins and in the staging; no block with matrix instructions reloads one.)
 constexpr uint32_t token_groups(uint32_t format, uint32_t hd) {
   return format == BCH_KV_F16 ? (hd == 64 ? 4 : hd == 128 ? 2 : 1) : (hd == 64 ? 4 : hd == 128 ? 3 : 2);
 }
@@ -1059,15 +1062,21 @@ KvSchedule kv_schedule(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t 
   // a join (about 2.5 us) pays from 24 steps on with heads of 64, 19 of 128, 16
   // of 256 (300 keys of 64: 5.6 us whole, 7.6 cut; 2,000: 14.2 and 9.0).
   const uint32_t unsplit = 14 + 640 / head_dim;
-  // What the registers let run at once; of heads of 256 one a CU (twelve
-  // sequences of drafts of 256: 19 us, with two 22).
+  // What the registers let run at once; of heads of 256 one a CU: twelve
+  // sequences of five drafts in int8 19.6 us, with two 23.4, in e4m3 18.1 and 23.0.
+  // (Where a sequence has one tile it goes both ways: single tokens of 64
+  // sequences of 4,000 int8 keys, two KV heads, 29.8 and 27.9; of eight, eight KV
+  // heads, 24.4 and 22.2, in e4m3 16.2 and 17.9; of one with 32,000 keys 29.4 and
+  // 30.6.)
   const uint64_t few_groups = (uint64_t)n_cus * (head_dim == 256 ? 1 : token_groups(format, head_dim)) / n_kv;
   deal(w, w.tiles8, narrow, few_groups, 8, longest <= unsplit, 4, n_kv, 1, records);
   deal(w, w.tiles16, tokens, few_groups, 8, longest <= unsplit, 4, n_kv, 1, records);
   // Where a workgroup has one item, the order is free.  (Heads of 256, 12 sequences
-  // of 20 rows and 4,096 keys: 18.1 us instead of 19.5, of 64 rows and 2,000 keys
-  // 18.7 instead of 19.8.  Smaller heads take fewer bytes a CU at a time and gain
-  // nothing: of 128, 20 rows, 15.5 instead of 15.0, of 64 12.3 and 12.3.)
+  // of 20 rows and 4,096 keys: 18.1 us instead of 20.4 in e4m3, 23.4 instead of
+  // 26.2 in f16, of 64 rows and 2,000 keys 18.7 instead of 19.8; single tokens,
+  // whose tiles share no keys, the same either way.  Smaller heads take fewer bytes
+  // a CU at a time and gain nothing: of 128, 20 rows, 15.5 instead of 15.0, of 64
+  // 12.3 and 12.3.)
   if (head_dim == 256)
     for (KvWork *work : {&w.tiles8, &w.tiles16})
       if (work->items.size() < work->starts.size()) keep_together(work->items, n_kv);
