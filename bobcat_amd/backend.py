@@ -128,11 +128,11 @@ def _u32(lists, what: str) -> np.ndarray:
 
 def _batch(shape: KvShape, n_past, n_new, pages):
     """A batch's arguments: lengths, and each sequence's pages one list after the other."""
-    past, new = _u32([n_past], "lengths"), _u32([n_new], "lengths")
+    past, new = (_u32([[n] if isinstance(n, (int, np.integer)) else n], "lengths") for n in (n_past, n_new))
     if past.shape != new.shape:
         raise ValueError("n_past and n_new hold one number for each sequence")
     # (The library sees one list and would deal it out anew.)
-    page = max(shape.page_size, 1)
+    page, pages = max(shape.page_size, 1), [seq if hasattr(seq, "__len__") else list(seq) for seq in pages]
     need, have = [-(-(p + n) // page) for p, n in zip(past.tolist(), new.tolist())], [len(seq) for seq in pages]
     if need != have:
         if len(need) != len(have):

@@ -44,3 +44,14 @@ def test_numbers_that_are_refused(number):
 def test_arrays():
     kv_plan_check(SHAPE, 8, np.asarray([20, 40]), np.asarray([3, 1], np.uint8), [np.asarray([4]), np.asarray([7, 1], np.int32)])
     kv_plan_check(SHAPE, 8, np.empty(0, np.uint32), [], [])
+
+
+def test_iterators_and_single_numbers():
+    """Lists that can be gone through once, rows of an array, and a single sequence's lengths."""
+    kv_plan_check(SHAPE, 8, [20, 40], [3, 1], iter([[4], [7, 1]]))
+    kv_plan_check(SHAPE, 8, [20, 40], [3, 1], (iter(p) for p in ([4], [7, 1])))
+    kv_plan_check(SHAPE, 8, (33, 34), (1, 1), np.asarray([[1, 2], [3, 4]]))
+    kv_plan_check(SHAPE, 8, 20, 3, [[4]])
+    kv_plan_check(SHAPE, 8, np.uint32(20), np.int64(3), [[4]])
+    with pytest.raises(ValueError):
+        kv_plan_check(SHAPE, 8, np.asarray([[20]]), np.asarray([[3]]), [[4]])
