@@ -43,6 +43,26 @@ class KvShape(C.Structure):
                 ("page_size", C.c_uint32), ("n_pages", C.c_uint32)]
 
 
+class RopeSpec(C.Structure):
+    _fields_ = [("layout", C.c_uint32), ("n_rot", C.c_uint32), ("scaling", C.c_uint32), ("n_original", C.c_uint32),
+                ("theta", C.c_double), ("factor", C.c_double), ("slow", C.c_double), ("fast", C.c_double),
+                ("magnitude", C.c_double)]
+
+
+class RopeRowsC(C.Structure):
+    _fields_ = [("from", View), ("to", View), ("norm", View), ("n_heads", C.c_uint32), ("head_stride", C.c_uint32),
+                ("from_stride", C.c_uint32), ("to_stride", C.c_uint32), ("eps", C.c_float)]
+
+
+class Drafts(C.Structure):
+    _fields_ = [("logits", View), ("draft", View), ("tokens", View), ("uniforms", View), ("temperatures", View),
+                ("distinct", C.c_uint32)]
+
+
+class Verdict(C.Structure):
+    _fields_ = [("kept", View), ("path", View), ("next", View), ("chances", View)]
+
+
 class LogitRules(C.Structure):
     _fields_ = [("rows", View), ("history", View), ("bias_tokens", View), ("bias_values", View), ("masks", View),
                 ("n_history", C.c_uint32), ("n_bias", C.c_uint32), ("n_masks", C.c_uint32)]
@@ -210,9 +230,17 @@ PROTOTYPES = {
     "bch_kv_plan_new": (_int, [_vp, C.POINTER(KvShape), _u32, C.POINTER(_vp)]),
     "bch_kv_plan_free": (None, [_vp]),
     "bch_kv_plan_set": (_int, [_vp, _u32, _vp, _vp, _vp, _u64]),
+    "bch_kv_plan_check_trees": (_int, [C.POINTER(KvShape), _u32, _u32, _vp, _vp, _vp, _u64, _vp, _u64]),
+    "bch_kv_plan_set_trees": (_int, [_vp, _u32, _vp, _vp, _vp, _u64, _vp, _u64]),
     "bch_kv_store": (_int, [_vp, _vp, View, View, _u32, View, _u32]),
     "bch_kv_load": (_int, [_vp, _vp, View, _u32, _u32, _u32, View, View]),
     "bch_attention_paged": (_int, [_vp, _vp, View, View, _u32, View, _u32]),
+    "bch_rope_frequencies": (_int, [C.POINTER(RopeSpec), _vp]),
+    "bch_rope_new": (_int, [_vp, C.POINTER(RopeSpec), _vp, C.POINTER(_vp)]),
+    "bch_rope_free": (None, [_vp]),
+    "bch_rope_paged": (_int, [_vp, _vp, _vp, C.POINTER(RopeRowsC), C.POINTER(RopeRowsC)]),
+    "bch_kv_keep": (_int, [_vp, _vp, _u32, _u32, View, _u32, _u64, View, View]),
+    "bch_verify_drafts": (_int, [_vp, _vp, _u32, _u32, _u32, C.POINTER(Drafts), C.POINTER(Verdict)]),
     "bch_logits_edit": (_int, [_vp, View, View, _u32, _u32, C.POINTER(LogitRules)]),
     "bch_lfm2_new": (_int, [_vp, C.POINTER(Lfm2Model), _u32, _int, C.POINTER(_vp)]),
     "bch_lfm2_free": (None, [_vp]),

@@ -16,7 +16,8 @@ from enum import IntEnum
 
 import numpy as np
 
-from ._lib import BobcatError, KvShape, LogitRules, Norm as _Norm, ProfileEntry, STATUS, View as _View, check, lib
+from ._lib import (BobcatError, Drafts, KvShape, LogitRules, Norm as _Norm, ProfileEntry, RopeRowsC, RopeSpec, STATUS,
+                   Verdict, View as _View, check, lib)
 
 
 class Format(IntEnum):
@@ -103,6 +104,8 @@ class KvFormat(IntEnum):
 LOGIT_ROW = np.dtype([("history_at", "<u4"), ("history_len", "<u4"), ("bias_at", "<u4"), ("bias_len", "<u4"),
                       ("mask", "<u4"), ("repeat", "<f4"), ("presence", "<f4"), ("frequency", "<f4")])
 NO_MASK = 0xFFFFFFFF
+NO_PARENT = 0xFFFFFFFF  # of a new token that follows the past
+NO_TOKEN = 0xFFFFFFFF   # in a path behind the kept tokens, and where no token can be drawn
 
 
 def kv_shape(fmt, n_kv_heads: int, head_dim: int, page_size: int, n_pages: int) -> KvShape:
@@ -143,10 +146,27 @@ def _batch(shape: KvShape, n_past, n_new, pages):
     return past, new, flat, (past.size, past.ctypes.data, new.ctypes.data, flat.ctypes.data, flat.size)
 
 
-def kv_plan_check(shape: KvShape, n_heads: int, n_past, n_new, pages) -> None:
+def _parents(new: np.ndarray, parents):
+    """The parents of all new tokens, one list after the other; None for a sequence is a chain."""
+    parents = [seq if seq is None or hasattr(seq, "__len__") else list(seq) for seq in parents]
+    if len(parents) != new.size:
+        raise BobcatError(STATUS["Argument"], f"{len(parents)} lists of parents for {new.size} sequences")
+    for at, (seq, n) in enumerate(zip(parents, new.tolist())):
+        if seq is not None and len(seq) != n:
+            raise BobcatError(STATUS["Argument"], f"sequence {at} has {n} new tokens and {len(seq)} parents")
+    chain = lambda n: [NO_PARENT, *range(n - 1)][:n]  # noqa: E731
+    flat = _u32([chain(n) if seq is None else seq for seq, n in zip(parents, new.tolist())], "parents")
+    return flat, (flat.ctypes.data, flat.size)
+
+
+def kv_plan_check(shape: KvShape, n_heads: int, n_past, n_new, pages, parents=None) -> None:
     """Raise what KvPlan and its set() would, without a device."""
-    *_keep, args = _batch(shape, n_past, n_new, pages)
-    check(lib().bch_kv_plan_check(C.byref(shape), n_heads, *args))
+    past, new, *_keep, args = _batch(shape, n_past, n_new, pages)
+    if parents is None:
+        check(lib().bch_kv_plan_check(C.byref(shape), n_heads, *args))
+    else:
+        _kept, more = _parents(new, parents)
+        check(lib().bch_kv_plan_check_trees(C.byref(shape), n_heads, *args, *more))
 
 
 class KvPlan:
@@ -158,11 +178,16 @@ class KvPlan:
         self.handle, self.shape, self.n_heads = h.value, shape, n_heads
         hip._dependents.add(self)
 
-    def set(self, n_past, n_new, pages) -> None:
+    def set(self, n_past, n_new, pages, parents=None) -> None:
         """The batch: past positions and new tokens of each sequence, and each sequence's list of pages
-        (ceil((past + new) / page_size) of them)."""
-        *_keep, args = _batch(self.shape, n_past, n_new, pages)
-        check(lib().bch_kv_plan_set(self.handle, *args))
+        (ceil((past + new) / page_size) of them).  `parents` makes trees of the new tokens: each sequence's list of
+        the places that its tokens follow (NO_PARENT: the past), or None where each follows the one before."""
+        past, new, *_keep, args = _batch(self.shape, n_past, n_new, pages)
+        if parents is None:
+            check(lib().bch_kv_plan_set(self.handle, *args))
+        else:
+            _kept, more = _parents(new, parents)
+            check(lib().bch_kv_plan_set_trees(self.handle, *args, *more))
 
     def close(self) -> None:
         if self.handle:
@@ -174,6 +199,67 @@ class KvPlan:
             self.close()
         except Exception:
             pass
+
+
+_LAYOUTS = dict(halves=0, pairs=1)
+_SCALINGS = dict(none=0, linear=1, parts=2)
+
+
+def rope_spec(n_rot: int, theta: float, *, layout="halves", scaling="none", factor=1.0, n_original=0, slow=1.0, fast=32.0,
+              magnitude=1.0) -> RopeSpec:
+    """Rotary positions (bch_rope_spec): `layout` halves or pairs, `scaling` none, linear or parts."""
+    pick = lambda x, names: names[x] if isinstance(x, str) else int(x)  # noqa: E731
+    return RopeSpec(pick(layout, _LAYOUTS), n_rot, pick(scaling, _SCALINGS), n_original, theta, factor, slow, fast, magnitude)
+
+
+def rope_frequencies(spec: RopeSpec) -> np.ndarray:
+    """The radians a position of a spec's pairs; no device is needed."""
+    out = np.empty(min(spec.n_rot, 256) // 2, np.float64)
+    check(lib().bch_rope_frequencies(C.byref(spec), out.ctypes.data))
+    return out
+
+
+class Rope:
+    """Rotary positions for launches (bch_rope)."""
+
+    def __init__(self, hip: "Hip", spec: RopeSpec, frequencies=None):
+        h, given = C.c_void_p(), None
+        if frequencies is not None:
+            given = np.ascontiguousarray(frequencies, np.float64)
+            if given.shape != (spec.n_rot // 2,):
+                raise BobcatError(STATUS["Argument"], f"{spec.n_rot // 2} frequencies are wanted, got {given.shape}")
+        check(lib().bch_rope_new(hip.handle, C.byref(spec), None if given is None else given.ctypes.data, C.byref(h)))
+        self.handle, self.spec = h.value, spec
+        hip._dependents.add(self)
+
+    def close(self) -> None:
+        if self.handle:
+            lib().bch_rope_free(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+@dataclass(frozen=True)
+class RopeRows:
+    """A batch's heads for rope_paged (bch_rope_rows): head_stride None is heads one after the other."""
+    src: ViewRef
+    src_stride: int
+    dst: ViewRef
+    dst_stride: int
+    n_heads: int
+    head_stride: int | None = None
+    norm: NormSpec | None = None
+
+    def c(self, head_dim: int) -> RopeRowsC:
+        norm = _View() if self.norm is None else _view(self.norm.weight)
+        return RopeRowsC(_view(self.src), _view(self.dst), norm, self.n_heads,
+                         head_dim if self.head_stride is None else self.head_stride, self.src_stride, self.dst_stride,
+                         0.0 if self.norm is None else self.norm.eps)
 
 
 class Hip:
@@ -348,6 +434,25 @@ class Hip:
         check(lib().bch_attention_paged(self.handle, plan.handle, _view(cache), _view(q), q_stride, _view(out),
                                         out_stride))
 
+    def rope(self, n_rot, theta, *, frequencies=None, **spec) -> Rope:
+        return Rope(self, rope_spec(n_rot, theta, **spec), frequencies)
+
+    def rope_paged(self, rope: Rope, plan: KvPlan, q: RopeRows | None, k: RopeRows | None):
+        rows = lambda r: None if r is None else C.byref(r.c(plan.shape.head_dim))  # noqa: E731
+        check(lib().bch_rope_paged(self.handle, rope.handle, plan.handle, rows(q), rows(k)))
+
+    def kv_keep(self, plan: KvPlan, first, n_seqs, cache, n_layers, layer_bytes, kept, path):
+        check(lib().bch_kv_keep(self.handle, plan.handle, first, n_seqs, _view(cache), n_layers, layer_bytes, _view(kept),
+                                _view(path)))
+
+    def verify_drafts(self, plan: KvPlan, first, n_seqs, n_vocab, logits, tokens, uniforms, temperatures, kept, path, next,
+                      *, chances=None, draft=None, distinct=False):
+        """`draft` None: the tokens were chosen without chance."""
+        view = lambda v: _View() if v is None else _view(v)  # noqa: E731
+        drafts = Drafts(view(logits), view(draft), view(tokens), view(uniforms), view(temperatures), int(bool(distinct)))
+        verdict = Verdict(view(kept), view(path), view(next), view(chances))
+        check(lib().bch_verify_drafts(self.handle, plan.handle, first, n_seqs, n_vocab, C.byref(drafts), C.byref(verdict)))
+
     def logits_edit(self, logits, out, n_rows, n_vocab, rows, *, history=None, n_history=0, bias_tokens=None,
                     bias_values=None, n_bias=0, masks=None, n_masks=0):
         """`rows` holds n_rows LOGIT_ROW; a list of no entries needs no view."""
@@ -415,6 +520,7 @@ def row_bytes(fmt: int, n_cols: int) -> int:
     return lib().bch_row_bytes(int(fmt), n_cols)
 
 
-__all__ = ["Hip", "Buffer", "KvFormat", "KvPlan", "LOGIT_ROW", "NO_MASK", "ViewRef", "NormSpec", "Format", "Store",
-           "BobcatError", "attention_scratch_floats", "attention_decode_scratch_floats", "kv_page_bytes",
-           "kv_plan_check", "kv_shape", "row_bytes"]
+__all__ = ["Hip", "Buffer", "KvFormat", "KvPlan", "LOGIT_ROW", "NO_MASK", "NO_PARENT", "NO_TOKEN", "Rope", "RopeRows",
+           "ViewRef", "NormSpec", "Format", "Store", "BobcatError", "attention_scratch_floats",
+           "attention_decode_scratch_floats", "kv_page_bytes", "kv_plan_check", "kv_shape", "rope_frequencies",
+           "rope_spec", "row_bytes"]

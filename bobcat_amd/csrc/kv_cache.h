@@ -70,12 +70,23 @@ struct KvSeq {
   uint32_t row;          // of the first token among the batch's
   uint32_t table;        // of the first page among the batch's pages
 };
-// One block that receives tokens: positions lo .. lo + n of block `block` of
-// page `page` from the batch's rows row ...
+// New tokens that go into one block: their rows in the batch, and the place of
+// the first among its sequence's positions.
 struct KvStoreItem {
-  uint32_t page, block, row;
-  uint16_t lo, n;
+  uint32_t page, pos, row, n;
 };
+constexpr uint32_t kKvNone = ~0u;
+// A new token of a batch with trees: the places of its parent, its first child
+// and its parent's next child among its sequence's new tokens (kKvNone: none), its
+// position, and where its mask begins (kKvNone: its sequence is a chain).
+struct KvNode {
+  uint32_t parent, child, sibling, position, mask;
+};
+// The mask of a tree's token: a bit for each key that it sees from key
+// past / 32·32 on, 32 keys a word, to the word with the sequence's last.
+__host__ __device__ constexpr uint32_t kv_mask_words(uint32_t past, uint32_t n_new) {
+  return (past + n_new - 1) / 32 - past / 32 + 1;
+}
 // A tile of packed rows (row = token·group + head of the group) of a sequence
 // and a part of its keys.
 struct KvAttnItem {
@@ -118,9 +129,10 @@ struct KvGeometry {
     using Constant = const __attribute__((address_space(4))) uint32_t;
     return ((Constant *)pages)[table + __umulhi(2 * b, page_magic)];
   }
+  __device__ __forceinline__ uint32_t in_page(uint32_t b) const { return b - __umulhi(2 * b, page_magic) * page_blocks; }
   template <uint32_t BYTES>
   __device__ __forceinline__ uint8_t *block(uint32_t page, uint32_t b, uint32_t head) const {
-    const uint32_t in_page = b - __umulhi(2 * b, page_magic) * page_blocks;
+    const uint32_t in_page = this->in_page(b);
     return cache + (((uint64_t)page * n_kv + head) * page_blocks + in_page) * BYTES;
   }
 };
@@ -137,12 +149,17 @@ struct bch_kv_plan {
   mutable uint64_t last_use = 0;
   uint32_t n_seqs = 0, n_tokens = 0;
   std::vector<bch::KvSeq> seqs;
+  std::vector<uint8_t> rooted;  // sequences whose first new token is all others' ancestor; none: all of them
+  const bch::KvSeq *d_seqs = nullptr;
   // One device allocation with all of the below, grown on demand.
   uint8_t *memory = nullptr;
   uint64_t memory_bytes = 0;
   const uint32_t *d_pages = nullptr;
   const bch::KvStoreItem *d_store = nullptr;
   uint32_t n_store = 0;
+  // A batch with trees (else null): a node for each new token, and the masks.
+  const bch::KvNode *d_nodes = nullptr;
+  const uint32_t *d_masks = nullptr;
   struct Work {
     const bch::KvAttnItem *items = nullptr;
     const uint32_t *starts = nullptr;
@@ -159,8 +176,9 @@ struct bch_kv_plan {
 };
 
 namespace bch {
-// The plan of a recorded op: BCH_OK if it belongs to ctx, is ready, and the
-// view `cache` holds its pages, whose address goes to *ptr.
+// The plan of a recorded op: BCH_OK if it belongs to ctx and is ready.
+int kv_plan_ready(bch_ctx *ctx, const char *kernel, const bch_kv_plan *plan);
+// The same, and the view `cache` holds its pages, whose address goes to *ptr.
 int kv_plan_cache(bch_ctx *ctx, const char *kernel, const bch_kv_plan *plan, bch_view cache, void **ptr);
 // Notes that the open recording has launches that read the plan's memory.
 void kv_plan_use(const bch_ctx *ctx, const bch_kv_plan *plan);
@@ -171,6 +189,8 @@ int kv_plan_rows(bch_ctx *ctx, const char *kernel, const bch_kv_plan *plan, bch_
 inline uint64_t kv_rows_bytes(const bch_kv_plan *plan, uint32_t width, uint32_t stride) {
   return plan->n_tokens ? ((uint64_t)(plan->n_tokens - 1) * stride + width) * 4 : 0;
 }
+// Sequences first .. first + n of a plan that has a batch, and their new tokens.
+int kv_plan_range(const char *kernel, const bch_kv_plan *plan, uint32_t first, uint32_t n, uint32_t *row, uint32_t *tokens);
 inline bool kv_overlap(const void *a, uint64_t a_bytes, const void *b, uint64_t b_bytes) {
   const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
   return x < y + b_bytes && y < x + a_bytes;

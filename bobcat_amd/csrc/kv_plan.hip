@@ -81,10 +81,50 @@ static int check_batch(const char *kernel, const bch_kv_shape *s, uint32_t n_seq
   return BCH_OK;
 }
 
-int kv_plan_cache(bch_ctx *ctx, const char *kernel, const bch_kv_plan *plan, bch_view cache, void **ptr) {
+// The tokens' parents: each before its child, and trees of a size that masks are made for.
+static bool is_chain(const uint32_t *parents, uint32_t n) {
+  for (uint32_t i = 0; i < n; i++)
+    if (parents[i] != (i ? i - 1 : BCH_NO_PARENT)) return false;
+  return true;
+}
+
+static int check_trees(const char *kernel, uint32_t n_seqs, const uint32_t *n_new, const uint32_t *parents, uint64_t n_parents) {
+  uint64_t tokens = 0;
+  for (uint32_t i = 0; i < n_seqs; i++) tokens += n_new[i];
+  if (n_parents != tokens)
+    return fail(BCH_ERR_ARGUMENT, "%s: %llu parents for %llu new tokens", kernel, (unsigned long long)n_parents,
+                (unsigned long long)tokens);
+  if (tokens && !parents) return fail(BCH_ERR_ARGUMENT, "%s: no parents", kernel);
+  for (uint32_t i = 0; i < n_seqs; parents += n_new[i++]) {
+    if (is_chain(parents, n_new[i])) continue;
+    if (n_new[i] > BCH_MAX_TREE)
+      return fail(BCH_ERR_ARGUMENT, "%s: the tree of sequence %u has %u tokens, at most %u are wanted", kernel, i, n_new[i],
+                  BCH_MAX_TREE);
+    for (uint32_t t = 0; t < n_new[i]; t++)
+      if (parents[t] != BCH_NO_PARENT && parents[t] >= t)
+        return fail(BCH_ERR_ARGUMENT, "%s: token %u of sequence %u follows token %u", kernel, t, i, parents[t]);
+  }
+  return BCH_OK;
+}
+
+int kv_plan_ready(bch_ctx *ctx, const char *kernel, const bch_kv_plan *plan) {
   if (!plan) return fail(BCH_ERR_ARGUMENT, "%s: no plan", kernel);
   if (plan->ctx != ctx) return fail(BCH_ERR_FOREIGN_BUFFER, "%s: the plan belongs to another backend", kernel);
   if (!plan->ready) return fail(BCH_ERR_ARGUMENT, "%s: the plan has no batch", kernel);
+  return BCH_OK;
+}
+
+int kv_plan_range(const char *kernel, const bch_kv_plan *plan, uint32_t first, uint32_t n, uint32_t *row, uint32_t *tokens) {
+  if (first > plan->n_seqs || n > plan->n_seqs - first)
+    return fail(BCH_ERR_ARGUMENT, "%s: sequences %u to %llu of %u", kernel, first, (unsigned long long)first + n, plan->n_seqs);
+  auto at = [&](uint32_t seq) { return seq < plan->n_seqs ? plan->seqs[seq].row : plan->n_tokens; };
+  *row = at(first);
+  *tokens = at(first + n) - *row;
+  return BCH_OK;
+}
+
+int kv_plan_cache(bch_ctx *ctx, const char *kernel, const bch_kv_plan *plan, bch_view cache, void **ptr) {
+  BCH_TRY(kv_plan_ready(ctx, kernel, plan));
   BCH_TRY(check_view(ctx, kernel, cache, bch_kv_page_bytes(&plan->shape) * plan->shape.n_pages, ptr));
   if (reinterpret_cast<uintptr_t>(*ptr) % 16) return fail(BCH_ERR_ARGUMENT, "%s: the cache must be 16-byte aligned", kernel);
   return BCH_OK;
@@ -114,8 +154,40 @@ struct Layout {
   }
 };
 
+// The nodes and masks of a batch's trees; `rooted` as the plan's.
+static void lay_trees(const std::vector<KvSeq> &seqs, const uint32_t *parents, std::vector<KvNode> &nodes,
+                      std::vector<uint32_t> &masks, std::vector<uint8_t> &rooted) {
+  for (const KvSeq &q : seqs) {
+    const uint32_t *up = parents + q.row;
+    const bool chain = is_chain(up, q.n_new);
+    const uint32_t words = q.n_new && !chain ? kv_mask_words(q.past, q.n_new) : 0, skip = q.past % 32;
+    KvNode *const of = nodes.data() + q.row;
+    uint32_t roots = 0;
+    std::vector<uint32_t> last(q.n_new, kKvNone);  // of a token's children so far
+    for (uint32_t i = 0; i < q.n_new; i++) {
+      const uint32_t a = up[i];
+      of[i] = {a, kKvNone, kKvNone, a == BCH_NO_PARENT ? q.past : of[a].position + 1, words ? (uint32_t)masks.size() : kKvNone};
+      if (a == BCH_NO_PARENT) {
+        roots++;
+      } else {
+        (last[a] == kKvNone ? of[a].child : of[last[a]].sibling) = i;
+        last[a] = i;
+      }
+      if (!words) continue;
+      const size_t at = masks.size();
+      masks.resize(at + words);
+      if (a == BCH_NO_PARENT)
+        masks[at] = (1u << skip) - 1;  // the past's keys of the first word
+      else
+        std::copy_n(masks.begin() + of[a].mask, words, masks.begin() + at);
+      masks[at + (skip + i) / 32] |= 1u << (skip + i) % 32;
+    }
+    rooted.push_back(roots <= 1);
+  }
+}
+
 static int plan_set(bch_kv_plan *plan, uint32_t n_seqs, const uint32_t *n_past, const uint32_t *n_new,
-                    const uint32_t *pages, uint64_t n_pages) {
+                    const uint32_t *pages, uint64_t n_pages, const uint32_t *parents) {
   const uint32_t page_blocks = plan->shape.page_size / kKvBlock;
   std::vector<KvSeq> seqs(n_seqs);
   std::vector<KvStoreItem> store;
@@ -124,8 +196,8 @@ static int plan_set(bch_kv_plan *plan, uint32_t n_seqs, const uint32_t *n_past, 
     const uint32_t end = n_past[i] + n_new[i];
     seqs[i] = {n_past[i], n_new[i], row, table};
     for (uint32_t p = n_past[i]; p < end;) {
-      const uint32_t b = p / kKvBlock, lo = p % kKvBlock, n = std::min(kKvBlock - lo, end - p);
-      store.push_back({pages[table + b / page_blocks], b % page_blocks, row + (p - n_past[i]), (uint16_t)lo, (uint16_t)n});
+      const uint32_t n = std::min(kKvBlock - p % kKvBlock, end - p);
+      store.push_back({pages[table + p / kKvBlock / page_blocks], p, row + (p - n_past[i]), n});
       p += n;
     }
     row += n_new[i];
@@ -133,7 +205,20 @@ static int plan_set(bch_kv_plan *plan, uint32_t n_seqs, const uint32_t *n_past, 
   }
   const KvSchedule work = kv_schedule(seqs, plan->n_heads / plan->shape.n_kv_heads, plan->shape.n_kv_heads,
                                       plan->shape.format, plan->shape.head_dim, plan->ctx->n_cus, plan->ctx->attn_partials ? kAttnPartialFloats : 0);
+  // (Parents that make chains of all sequences are no trees.)
+  std::vector<KvNode> nodes;
+  std::vector<uint32_t> masks;
+  std::vector<uint8_t> rooted;
+  bool trees = false;
+  for (uint32_t i = 0; parents && i < n_seqs; i++) trees |= !is_chain(parents + seqs[i].row, seqs[i].n_new);
+  if (trees) {
+    nodes.resize(row);
+    lay_trees(seqs, parents, nodes, masks, rooted);
+  }
   Layout all;
+  const uint64_t at_seqs = all.add(seqs.data(), seqs.size());
+  const uint64_t at_nodes = all.add(nodes.data(), nodes.size());
+  const uint64_t at_masks = all.add(masks.data(), masks.size());
   const uint64_t at_pages = all.add(pages, n_pages);
   const uint64_t at_store = all.add(store.data(), store.size());
   const KvWork *const works[] = {&work.tiles8, &work.tiles16, &work.chunks};
@@ -170,6 +255,10 @@ static int plan_set(bch_kv_plan *plan, uint32_t n_seqs, const uint32_t *n_past, 
        hipStreamSynchronize(nullptr) != hipSuccess))
     return fail(BCH_ERR_EXECUTION, "kv_plan_set: host-to-device copy failed");
   plan->seqs.swap(seqs);
+  plan->rooted.swap(rooted);
+  plan->d_seqs = reinterpret_cast<const KvSeq *>(plan->memory + at_seqs);
+  plan->d_nodes = trees ? reinterpret_cast<const KvNode *>(plan->memory + at_nodes) : nullptr;
+  plan->d_masks = reinterpret_cast<const uint32_t *>(plan->memory + at_masks);
   plan->n_seqs = n_seqs;
   plan->n_tokens = row;
   plan->d_pages = reinterpret_cast<const uint32_t *>(plan->memory + at_pages);
@@ -204,15 +293,28 @@ uint64_t bch_kv_page_bytes(const bch_kv_shape *shape) {
   return (uint64_t)shape->n_kv_heads * (shape->page_size / kKvBlock) * kv_block_bytes(shape->format, shape->head_dim);
 }
 
-int bch_kv_plan_check(const bch_kv_shape *shape, uint32_t n_heads, uint32_t n_seqs, const uint32_t *n_past,
-                      const uint32_t *n_new, const uint32_t *pages, uint64_t n_pages) {
+static int plan_check(const bch_kv_shape *shape, uint32_t n_heads, uint32_t n_seqs, const uint32_t *n_past,
+                      const uint32_t *n_new, const uint32_t *pages, uint64_t n_pages, bool trees, const uint32_t *parents,
+                      uint64_t n_parents) {
   BCH_TRY(check_shape("kv_plan", shape));
   BCH_TRY(check_heads("kv_plan", shape, n_heads));
   try {
-    return check_batch("kv_plan", shape, n_seqs, n_past, n_new, pages, n_pages);
+    BCH_TRY(check_batch("kv_plan", shape, n_seqs, n_past, n_new, pages, n_pages));
   } catch (const std::bad_alloc &) {
     return fail(BCH_ERR_ALLOCATION, "kv_plan: out of host memory");
   }
+  return trees ? check_trees("kv_plan", n_seqs, n_new, parents, n_parents) : BCH_OK;
+}
+
+int bch_kv_plan_check(const bch_kv_shape *shape, uint32_t n_heads, uint32_t n_seqs, const uint32_t *n_past,
+                      const uint32_t *n_new, const uint32_t *pages, uint64_t n_pages) {
+  return plan_check(shape, n_heads, n_seqs, n_past, n_new, pages, n_pages, false, nullptr, 0);
+}
+
+int bch_kv_plan_check_trees(const bch_kv_shape *shape, uint32_t n_heads, uint32_t n_seqs, const uint32_t *n_past,
+                            const uint32_t *n_new, const uint32_t *pages, uint64_t n_pages, const uint32_t *parents,
+                            uint64_t n_parents) {
+  return plan_check(shape, n_heads, n_seqs, n_past, n_new, pages, n_pages, true, parents, n_parents);
 }
 
 int bch_kv_plan_new(bch_ctx *ctx, const bch_kv_shape *shape, uint32_t n_heads, bch_kv_plan **out) {
@@ -239,8 +341,8 @@ void bch_kv_plan_free(bch_kv_plan *plan) {
   delete plan;
 }
 
-int bch_kv_plan_set(bch_kv_plan *plan, uint32_t n_seqs, const uint32_t *n_past, const uint32_t *n_new,
-                    const uint32_t *pages, uint64_t n_pages) {
+static int plan_take(bch_kv_plan *plan, uint32_t n_seqs, const uint32_t *n_past, const uint32_t *n_new,
+                     const uint32_t *pages, uint64_t n_pages, bool trees, const uint32_t *parents, uint64_t n_parents) {
   if (!plan) return fail(BCH_ERR_ARGUMENT, "kv_plan_set: no plan");
   // In the open recording, or in one that has not been waited for.
   const bch_ctx *ctx = plan->ctx;
@@ -248,12 +350,22 @@ int bch_kv_plan_set(bch_kv_plan *plan, uint32_t n_seqs, const uint32_t *n_past, 
   for (const bch_ctx::Pending &p : ctx->pending) busy |= plan->last_use == p.recording;
   if (busy)
     return fail(BCH_ERR_BUSY, "kv_plan_set: the batch cannot change while work that uses it is in flight");
-  BCH_TRY(bch_kv_plan_check(&plan->shape, plan->n_heads, n_seqs, n_past, n_new, pages, n_pages));
+  BCH_TRY(plan_check(&plan->shape, plan->n_heads, n_seqs, n_past, n_new, pages, n_pages, trees, parents, n_parents));
   try {
-    return plan_set(plan, n_seqs, n_past, n_new, pages, n_pages);
+    return plan_set(plan, n_seqs, n_past, n_new, pages, n_pages, trees ? parents : nullptr);
   } catch (const std::bad_alloc &) {
     return fail(BCH_ERR_ALLOCATION, "kv_plan_set: out of host memory");
   }
+}
+
+int bch_kv_plan_set(bch_kv_plan *plan, uint32_t n_seqs, const uint32_t *n_past, const uint32_t *n_new,
+                    const uint32_t *pages, uint64_t n_pages) {
+  return plan_take(plan, n_seqs, n_past, n_new, pages, n_pages, false, nullptr, 0);
+}
+
+int bch_kv_plan_set_trees(bch_kv_plan *plan, uint32_t n_seqs, const uint32_t *n_past, const uint32_t *n_new,
+                          const uint32_t *pages, uint64_t n_pages, const uint32_t *parents, uint64_t n_parents) {
+  return plan_take(plan, n_seqs, n_past, n_new, pages, n_pages, true, parents, n_parents);
 }
 
 }  // extern "C"

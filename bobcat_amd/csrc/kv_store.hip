@@ -66,16 +66,15 @@ __device__ __forceinline__ uint32_t kv_element(uint2 w, int i) {
 }
 
 template <uint32_t FORMAT, uint32_t HD>
-__global__ __launch_bounds__(kStoreThreads) void k_kv_store(const KvStoreItem *__restrict__ items, uint8_t *cache,
-                                                            uint32_t page_blocks, uint32_t n_kv,
+__global__ __launch_bounds__(kStoreThreads) void k_kv_store(const KvStoreItem *__restrict__ items, KvGeometry g,
                                                             const float *__restrict__ k, uint32_t k_stride,
                                                             const float *__restrict__ v, uint32_t v_stride) {
   using Elem = std::conditional_t<FORMAT == BCH_KV_F16, uint16_t, uint8_t>;
   constexpr uint32_t J = HD / 64, BYTES = kv_block_bytes(FORMAT, HD), PART = kKvBlock * HD * sizeof(Elem);
   __shared__ __align__(16) Elem v_s[kKvBlock * HD];
   const KvStoreItem it = items[blockIdx.x];
-  const uint32_t head = blockIdx.y, r = threadIdx.x / 16, c = threadIdx.x % 16, pos = it.lo + r;
-  uint8_t *const block = cache + (((uint64_t)it.page * n_kv + head) * page_blocks + it.block) * BYTES;
+  const uint32_t head = blockIdx.y, r = threadIdx.x / 16, c = threadIdx.x % 16, pos = it.pos % kKvBlock + r;
+  uint8_t *const block = g.block<BYTES>(it.page, it.pos / kKvBlock, head);
   const bool mine = r < it.n;
   const uint64_t row = it.row + (mine ? r : 0);
   float4 x[2][J];
@@ -204,7 +203,7 @@ extern "C" int bch_kv_store(bch_ctx *ctx, const bch_kv_plan *plan, bch_view cach
     kv_plan_use(ctx, plan);
     kv_dispatch(s.format, s.head_dim, [&](auto format, auto hd) {
       k_kv_store<decltype(format)::value, decltype(hd)::value><<<dim3(plan->n_store, s.n_kv_heads), kStoreThreads, 0, st>>>(
-          plan->d_store, static_cast<uint8_t *>(cp), s.page_size / kKvBlock, s.n_kv_heads, kp, k_stride, vp, v_stride);
+          plan->d_store, plan->geometry(cp), kp, k_stride, vp, v_stride);
     });
   });
 }

@@ -377,6 +377,22 @@ void bch_kv_plan_free(bch_kv_plan *plan);
 int bch_kv_plan_set(bch_kv_plan *plan, uint32_t n_seqs, const uint32_t *n_past, const uint32_t *n_new,
                     const uint32_t *pages, uint64_t n_pages);
 
+/* The same with the sequences' new tokens as trees, as drafts of the next tokens
+ * are: parents[t] is the place, among its sequence's new tokens, of the one that
+ * token t follows, or BCH_NO_PARENT where it follows the past; n_parents is the
+ * number of all new tokens.  Parents come before their children.  A token sees
+ * the past, its ancestors and itself, and its position is n_past + its depth (0
+ * without a parent); its row in the cache is at n_past + its place.  Sequences
+ * whose tokens each follow the one before are what they are without parents,
+ * others have at most BCH_MAX_TREE new tokens (else BCH_ERR_ARGUMENT). */
+#define BCH_NO_PARENT 0xffffffffu
+#define BCH_MAX_TREE 1024u
+int bch_kv_plan_check_trees(const bch_kv_shape *shape, uint32_t n_heads, uint32_t n_seqs, const uint32_t *n_past,
+                            const uint32_t *n_new, const uint32_t *pages, uint64_t n_pages, const uint32_t *parents,
+                            uint64_t n_parents);
+int bch_kv_plan_set_trees(bch_kv_plan *plan, uint32_t n_seqs, const uint32_t *n_past, const uint32_t *n_new,
+                          const uint32_t *pages, uint64_t n_pages, const uint32_t *parents, uint64_t n_parents);
+
 /* Quantise the new tokens' keys and values, rows of n_kv_heads·head_dim
  * floats k_stride and v_stride floats apart (16-byte aligned, strides a
  * multiple of 4), into their pages; every other byte of the cache keeps its
@@ -389,7 +405,8 @@ int bch_kv_load(bch_ctx *ctx, const bch_kv_plan *plan, bch_view cache, uint32_t 
                 bch_view k, bch_view v);
 /* Causal attention of the new tokens, whose keys and values bch_kv_store has
  * put into the pages before: token i of a sequence attends to its positions
- * 0 .. n_past + i, softmax(q·k/√head_dim)·v.  Query and output rows of
+ * 0 .. n_past + i (of a tree: to 0 .. n_past - 1 and to the rows of its ancestors
+ * and its own), softmax(q·k/√head_dim)·v.  Query and output rows of
  * n_heads·head_dim floats, q_stride and out_stride floats apart (16-byte
  * aligned, strides a multiple of 4); query head h reads KV head
  * h / (n_heads / n_kv_heads).  `out` may not lie over `q`.  What a query does
@@ -403,6 +420,69 @@ int bch_kv_load(bch_ctx *ctx, const bch_kv_plan *plan, bch_view cache, uint32_t 
  * below that add to an output, up to n·2^-33 of the largest value, is lost. */
 int bch_attention_paged(bch_ctx *ctx, const bch_kv_plan *plan, bch_view cache, bch_view q, uint32_t q_stride,
                         bch_view out, uint32_t out_stride);
+
+/* Rotary positions for batches.  Of each head the first n_rot elements (even)
+ * are pairs, pair j elements j and j + n_rot/2 (BCH_ROPE_HALVES) or 2j and 2j + 1
+ * (BCH_ROPE_PAIRS), and (a, b) at position t becomes
+ *   magnitude·(a·cos t·f_j - b·sin t·f_j, a·sin t·f_j + b·cos t·f_j)
+ * with f_j = theta^(-2j / n_rot) radians a position, divided by `factor`
+ * (BCH_ROPE_LINEAR), or with r = n_original·f_j / 2π, the turns over the positions
+ * of the training, and w = clamp((r - slow) / (fast - slow), 0, 1) times
+ * w + (1 - w) / factor (BCH_ROPE_BY_PARTS: fast pairs as they are, slow ones
+ * divided).  Other elements stay as they are.  Frequencies are doubles and angles
+ * are reduced as integers, so that a far position costs no precision. */
+typedef enum bch_rope_layout { BCH_ROPE_HALVES = 0, BCH_ROPE_PAIRS = 1 } bch_rope_layout;
+typedef enum bch_rope_scaling { BCH_ROPE_PLAIN = 0, BCH_ROPE_LINEAR = 1, BCH_ROPE_BY_PARTS = 2 } bch_rope_scaling;
+typedef struct bch_rope_spec {
+  uint32_t layout;     /* bch_rope_layout */
+  uint32_t n_rot;      /* 2 to 256, even */
+  uint32_t scaling;    /* bch_rope_scaling */
+  uint32_t n_original; /* BY_PARTS, as slow < fast */
+  double theta;        /* above 0 */
+  double factor;       /* LINEAR and BY_PARTS, above 0 */
+  double slow, fast;
+  double magnitude;    /* 1 changes nothing */
+} bch_rope_spec;
+typedef struct bch_rope bch_rope;
+/* The n_rot / 2 frequencies of a spec; no device is needed. */
+int bch_rope_frequencies(const bch_rope_spec *spec, double *out);
+/* A spec for launches, to be freed before its context is closed.  With
+ * `frequencies` (nullable, n_rot / 2 finite numbers) those take the place of the
+ * spec's. */
+int bch_rope_new(bch_ctx *ctx, const bch_rope_spec *spec, const double *frequencies, bch_rope **out);
+void bch_rope_free(bch_rope *rope);
+
+/* The rows of a batch's tokens: n_heads heads of the plan's head_dim, in `from`
+ * head_stride floats apart (at least head_dim, as where each query head has its
+ * gate beside it), in `to` one after the other; rows from_stride and to_stride
+ * floats apart.  With a buffer in `norm` (head_dim weights) every head is first
+ * RMS-normalised as by bch_rms_norm.  All 16-byte aligned, strides a multiple of 4. */
+typedef struct bch_rope_rows {
+  bch_view from, to, norm;
+  uint32_t n_heads, head_stride, from_stride, to_stride;
+  float eps;
+} bch_rope_rows;
+/* Turn the queries and the keys (either may be NULL) of a plan's new tokens,
+ * each for its position: n_past + its place, in a tree n_past + its depth.
+ * Rows may be turned where they are (`to` as `from`, head_stride head_dim), and
+ * rows side by side at one stride may be read and written by one call; else what is
+ * written may not lie over what is read, nor over other rows that are written. */
+int bch_rope_paged(bch_ctx *ctx, const bch_rope *rope, const bch_kv_plan *plan, const bch_rope_rows *q,
+                   const bch_rope_rows *k);
+
+/* Move what a step keeps of its drafts together, once bch_verify_drafts has said
+ * which: for sequences first .. first + n_seqs of the plan, place j of the path of
+ * kept[s] tokens is the place path[j] among the new tokens, and position n_past + j
+ * of the cache gets the row (keys, values and scales, bit for bit) of position
+ * n_past + path[j]; all other bytes keep their values.  `kept` has n_seqs u32, `path`
+ * one for each new token of these sequences, sequence after sequence.  The next
+ * batch then has n_past + kept[s] positions.  A path goes up (path[j + 1] > path[j]);
+ * entries that do not, or are not below n_new, and counts above n_new move nothing
+ * outside the sequence's new tokens.  One launch for the caches of n_layers layers, layer l's
+ * layer_bytes·l bytes behind `cache` (a multiple of 16, at least a cache's bytes where
+ * there are several). */
+int bch_kv_keep(bch_ctx *ctx, const bch_kv_plan *plan, uint32_t first, uint32_t n_seqs, bch_view cache,
+                uint32_t n_layers, uint64_t layer_bytes, bch_view kept, bch_view path);
 
 /* ------------------------------------------------------------------ */
 /* Sampling                                                            */
@@ -477,6 +557,49 @@ typedef struct bch_logit_rules {
  * in the reference. */
 int bch_logits_edit(bch_ctx *ctx, bch_view logits, bch_view out, uint32_t n_rows, uint32_t n_vocab,
                     const bch_logit_rules *rules);
+
+/* Drafted tokens and what decides about them, in device memory; the rows of the
+ * sequences' new tokens one after the other. */
+typedef struct bch_drafts {
+  bch_view logits;       /* the target's, after each token: [tokens][n_vocab] floats */
+  bch_view draft;        /* what each token's children were drawn from: [tokens][n_vocab] probabilities, or a
+                            null buffer where they were chosen without chance */
+  bch_view tokens;       /* u32 */
+  bch_view uniforms;     /* a float in [0, 1) for each token: its own test's, the first token's for the draw */
+  bch_view temperatures; /* a float for each sequence; not above 0: the likeliest token */
+  uint32_t distinct;     /* a token's children were drawn without replacement */
+} bch_drafts;
+typedef struct bch_verdict {
+  bch_view kept;         /* u32 a sequence: the tokens that stay, its first one among them */
+  bch_view path;         /* u32 a token: their places in order, then BCH_NO_TOKEN */
+  bch_view next;         /* u32 a sequence: the token after them */
+  bch_view chances;      /* or a null buffer: a float a token, its probability by the target after its parent; in the
+                            first one's place that of `next` */
+} bch_verdict;
+#define BCH_NO_TOKEN 0xffffffffu
+
+/* Which of the drafted tokens of sequences first .. first + n_seqs of the plan
+ * stay, and the token after them, so that it and they are distributed as if the target had
+ * drawn each (speculative sampling on a tree).  A sequence's first new token is the step's
+ * own (no draft), and all others descend from it: BCH_ERR_ARGUMENT for a tree with another
+ * root, or for more than BCH_MAX_TREE tokens.  From the first token on: with p = softmax(logits /
+ * temperature) after the current token and q its draft row, the first child x in order
+ * with u·q(x) < p(x) stays and becomes the current token; for each child that does not,
+ *   p <- max(p - q, 0), normalised,
+ * before the next is looked at, and with `distinct` q <- q without x, divided by 1 - Σ q
+ * of those looked at.  Children chosen without chance have q = 1 each for themselves.
+ * Where no child stays, the next token is the first in token order up to which p sums to
+ * more than the first token's uniform times the whole.  At a temperature not above 0
+ * (or NaN) p is 1 for the first of the largest logits and `draft` is not looked at.
+ * A logit that is NaN counts as -inf, +inf as the largest float; tokens from n_vocab on
+ * have no probability.  If nothing is left of p (p and q agree to rounding) the
+ * draw is from p itself; a row without any logit above -inf gives BCH_NO_TOKEN and the
+ * chance 0.  (Tokens that bch_logits_edit leaves out are not drawn, whatever the
+ * draft says of them.)  Sequences without new tokens get 0 kept and BCH_NO_TOKEN.  Sums over the vocabulary are
+ * f64 of f32 terms: a test or a draw within about 2^-22 of its border may go either way, always
+ * the same way.  No counterpart in the reference. */
+int bch_verify_drafts(bch_ctx *ctx, const bch_kv_plan *plan, uint32_t first, uint32_t n_seqs, uint32_t n_vocab,
+                      const bch_drafts *drafts, const bch_verdict *verdict);
 
 /* ------------------------------------------------------------------ */
 /* Gated DeltaNet and gated attention (Qwen3.5)                        */
