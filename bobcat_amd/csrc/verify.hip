@@ -13,11 +13,15 @@
 // vocabulary.  For children chosen without chance (q is 1 for each in its turn) what is left
 // is p without them, and a rejection costs nothing.
 //
-// k_verify_rows reads every token's logits once: the largest, the first place of it,
-// and the sum of the exponentials, for pieces of the vocabulary.  k_verify_walk has a workgroup
-// for each sequence: it joins the pieces of its rows and takes the probabilities of all
-// drafted tokens at once, walks down (every thread the same way, out of LDS), and
-// draws.
+// Three steps, each a launch, so that none waits for another inside a kernel.
+//   k_verify_rows reads every token's logits once, in pieces of the vocabulary: the
+//     largest, the first place of it, and the sum of the exponentials.
+//   k_verify_rest (where there is a draft) sums pieces of (p - c·q)+ for one rejection of each
+//     sequence.  All its workgroups walk down the tree for themselves, out of LDS, up to where a sum
+//     is missing: a few microseconds of latency, where one workgroup's sum over the vocabulary takes
+//     70 us.
+//   k_verify_walk, a workgroup for each sequence, walks to the end (summing by itself what further
+//     rejections need) and draws: the piece in which the sum passes its goal, then the token in it.
 #include <algorithm>
 #include <cmath>
 
@@ -28,8 +32,9 @@
 
 namespace bch {
 
-constexpr uint32_t kRowThreads = 256, kRowPer = 16, kRowPiece = kRowThreads * kRowPer;
-constexpr uint32_t kWalkThreads = 1024, kWalkWaves = kWalkThreads / 64;
+constexpr uint32_t kRowThreads = 256, kRowPer = 16, kPiece = kRowThreads * kRowPer;
+constexpr uint32_t kWalkThreads = 1024;
+constexpr uint32_t kRounds = 3;  // of k_verify_rest for trees (for chains one is all)
 constexpr float kLargest = 3.402823466e38f;
 
 // One piece of a row: its largest logit, where it is first, and the sum of
@@ -47,8 +52,10 @@ struct VerifyArgs {
   float *chances;               // or null
   const KvSeq *seqs;            // of the first sequence on
   const KvNode *nodes;          // from the first token on, or null: chains
-  VerifyPiece *pieces;
+  VerifyPiece *pieces;          // [row][piece]
+  double *rest;                 // [round][sequence][piece], one round more than `rounds`
   uint32_t n_seqs, row0, n_rows, n_vocab, n_pieces, distinct;
+  uint32_t rounds, most;        // rejections that k_verify_rest sums; the most tokens of a sequence
 };
 
 // A logit as it counts: NaN as -inf, +inf as the largest float.
@@ -77,38 +84,67 @@ __device__ __forceinline__ double wave_sum_f64(double x) {
   return x;
 }
 
-// The sequence of a row (rows of a sequence are consecutive).
+// Over a workgroup; `scratch` holds a double a wave and is free again afterwards.
+template <uint32_t THREADS>
+__device__ __forceinline__ double block_sum_f64(double x, double *scratch) {
+  x = wave_sum_f64(x);
+  if (threadIdx.x % 64 == 0) scratch[threadIdx.x / 64] = x;
+  __syncthreads();
+  double all = 0;
+#pragma unroll
+  for (uint32_t w = 0; w < THREADS / 64; w++) all += scratch[w];
+  __syncthreads();
+  return all;
+}
+
+// The sequence of a row (rows of a sequence are consecutive): the last that
+// begins at or before it, 64 at a time.
 __device__ __forceinline__ uint32_t seq_of_row(const VerifyArgs &a, uint32_t row) {
-  uint32_t lo = 0, hi = a.n_seqs;  // the last with a first row <= row that has rows
-  while (hi - lo > 1) {
-    const uint32_t mid = (lo + hi) / 2;
-    if (a.seqs[mid].row - a.row0 <= row) lo = mid; else hi = mid;
+  uint32_t lo = 0, count = a.n_seqs;
+  while (count > 1) {
+    const uint32_t step = (count + 63) / 64, i = threadIdx.x % 64 * step;
+    const bool before = i < count && a.seqs[lo + min(i, count - 1)].row - a.row0 <= row;
+    const uint32_t n = __popcll(__builtin_amdgcn_ballot_w64(before));
+    lo += (n - 1) * step;
+    count = min(step, count - (n - 1) * step);
   }
   return lo;
 }
 
+// VEC: rows are 16-byte aligned.
+template <bool VEC>
 __global__ __launch_bounds__(kRowThreads) void k_verify_rows(VerifyArgs a) {
   __shared__ float top_s[4], sum_s[4];
   __shared__ uint32_t at_s[4];
   const uint32_t row = blockIdx.x / a.n_pieces, piece = blockIdx.x % a.n_pieces, tid = threadIdx.x;
-  const uint32_t base = piece * kRowPiece, len = min(kRowPiece, a.n_vocab - base);
+  const uint32_t base = piece * kPiece, len = min(kPiece, a.n_vocab - base);
   const float *p = a.logits + (uint64_t)row * a.n_vocab + base;
   float x[kRowPer];
+  // Element j of a thread is at place(j).
+  auto place = [&](uint32_t j) { return VEC ? 4 * (tid + kRowThreads * (j / 4)) + j % 4 : tid + kRowThreads * j; };
+  if constexpr (VEC) {
 #pragma unroll
-  for (uint32_t j = 0; j < kRowPer; j++) {
-    const uint32_t i = tid + kRowThreads * j;
-    x[j] = i < len ? logit(p[i]) : -INFINITY;
+    for (uint32_t j = 0; j < kRowPer; j += 4) {
+      const float4 v = *reinterpret_cast<const float4 *>(p + min(place(j), len - 4));
+      x[j] = v.x, x[j + 1] = v.y, x[j + 2] = v.z, x[j + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < kRowPer; j++) x[j] = p[min(place(j), len - 1)];
   }
   const float temperature = a.temperatures[seq_of_row(a, row)];
   float top = -INFINITY;
 #pragma unroll
-  for (uint32_t j = 0; j < kRowPer; j++) top = fmaxf(top, x[j]);
+  for (uint32_t j = 0; j < kRowPer; j++) {
+    x[j] = place(j) < len ? logit(x[j]) : -INFINITY;
+    top = fmaxf(top, x[j]);
+  }
   top = block_max<kRowThreads>(top, top_s);
   // The first place of the largest.
   uint32_t at = ~0u;
 #pragma unroll
   for (int j = kRowPer - 1; j >= 0; j--)
-    if (x[j] == top) at = base + tid + kRowThreads * j;
+    if (x[j] == top) at = base + place(j);
 #pragma unroll
   for (int i = 1; i < 64; i *= 2) at = min(at, (uint32_t)__shfl_xor((int)at, i, 64));
   float sum = 0.f;
@@ -123,202 +159,341 @@ __global__ __launch_bounds__(kRowThreads) void k_verify_rows(VerifyArgs a) {
   if (tid == 0) a.pieces[blockIdx.x] = {top, sum, min(min(at_s[0], at_s[1]), min(at_s[2], at_s[3])), 0};
 }
 
+// What a workgroup knows of its sequence, in LDS: of each token its row's largest
+// logit, sum and first largest's place, its own probabilities (after its parent), and the tree.
+struct WalkMemory {
+  double *sum, *p, *q;
+  float *top, *u;
+  uint32_t *best, *token, *child, *sibling, *path;
+  __device__ WalkMemory(double *at, uint32_t n) {
+    sum = at, p = sum + n, q = p + n;
+    top = reinterpret_cast<float *>(q + n), u = top + n;
+    best = reinterpret_cast<uint32_t *>(u + n), token = best + n, child = token + n, sibling = child + n, path = sibling + n;
+  }
+};
+constexpr uint32_t kWalkBytes = 3 * 8 + 7 * 4;  // a token
+
+template <uint32_t THREADS>
+struct Walk {
+  const VerifyArgs &a;
+  const uint32_t seq_at;
+  const KvSeq seq;
+  const uint32_t n, row0;
+  const float temperature;
+  const bool greedy, drawn;
+  const Heat heat;
+  const double heat64;
+  WalkMemory m;
+  // The current token and the kept ones, and what is left of p: (p - c·q)+ with the sum of `round`.
+  uint32_t t = 0, kept = 1, round = 0;
+  double c = 0;
+
+  __device__ Walk(const VerifyArgs &args, uint32_t which, double *memory)
+      : a(args), seq_at(which), seq(args.seqs[which]), n(seq.n_new), row0(seq.row - args.row0),
+        temperature(args.temperatures[which]), greedy(!(temperature > 0.f)), drawn(args.draft && !greedy),
+        heat(greedy ? 1.f : temperature), heat64((double)heat.hi + (double)heat.lo), m(memory, args.most) {}
+
+  // The target's probability of token x after token i.
+  __device__ double chance(uint32_t i, uint32_t x) const {
+    if (x >= a.n_vocab || m.best[i] == BCH_NO_TOKEN) return 0.0;
+    if (greedy) return x == m.best[i] ? 1.0 : 0.0;
+    const float l = logit(a.logits[(uint64_t)(row0 + i) * a.n_vocab + x]);
+    return l > -INFINITY ? exp2(((double)l - m.top[i]) * heat64) / m.sum[i] : 0.0;
+  }
+
+  // The rows' pieces joined, 16 lanes a row, and every drafted token's probabilities.
+  __device__ void load(bool chances) {
+    const uint32_t tid = threadIdx.x, lane = tid % 16;
+    const KvNode *nodes = a.nodes ? a.nodes + row0 : nullptr;
+    for (uint32_t i = tid; i < n; i += THREADS) {
+      m.token[i] = a.tokens[row0 + i];
+      m.u[i] = a.uniforms[row0 + i];
+      m.child[i] = nodes ? nodes[i].child : i + 1 < n ? i + 1 : kKvNone;
+      m.sibling[i] = nodes ? nodes[i].sibling : kKvNone;
+      m.path[i] = i ? BCH_NO_TOKEN : 0;
+    }
+    for (uint32_t i0 = 0; i0 < n; i0 += THREADS / 16) {
+      const uint32_t i = min(i0 + tid / 16, n - 1);
+      const VerifyPiece *p = a.pieces + (uint64_t)(row0 + i) * a.n_pieces;
+      // (A running sum: rows of up to 64 pieces, 262,144 tokens, in one round of loads.)
+      float top = -INFINITY;
+      double sum = 0;
+      uint32_t best = ~0u;
+      for (uint32_t j0 = 0; j0 < a.n_pieces; j0 += 64) {
+        VerifyPiece x[4];
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) x[k] = p[min(j0 + 16 * k + lane, a.n_pieces - 1)];
+        const float before = top;
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) {
+          if (j0 + 16 * k + lane >= a.n_pieces) x[k] = {-INFINITY, 0.f, ~0u, 0};
+          best = x[k].top > top ? x[k].at : best;  // (pieces go up, and so do the places)
+          top = fmaxf(top, x[k].top);
+        }
+        if (before > -INFINITY) sum *= exp2(((double)before - top) * heat64);
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++)
+          if (x[k].top > -INFINITY) sum += (double)x[k].sum * exp2(((double)x[k].top - top) * heat64);
+      }
+      float all = top;
+#pragma unroll
+      for (int k = 1; k < 16; k *= 2) all = fmaxf(all, __shfl_xor(all, k, 64));
+      if (top > -INFINITY) sum *= exp2(((double)top - all) * heat64);
+      if (top != all) best = ~0u;
+#pragma unroll
+      for (int k = 1; k < 16; k *= 2) {
+        sum += __shfl_xor(sum, k, 64);
+        best = min(best, (uint32_t)__shfl_xor((int)best, k, 64));
+      }
+      if (lane == 0) m.top[i] = all, m.sum[i] = sum, m.best[i] = all > -INFINITY ? best : BCH_NO_TOKEN;
+    }
+    __syncthreads();
+    for (uint32_t i = tid; i < n; i += THREADS) {
+      if (!i) continue;
+      const uint32_t up = nodes ? nodes[i].parent : i - 1, x = m.token[i];
+      const double p = chance(up, x);
+      m.p[i] = p;
+      m.q[i] = !drawn ? 1.0 : x < a.n_vocab ? (double)a.draft[(uint64_t)(row0 + up) * a.n_vocab + x] : 0.0;
+      if (chances) a.chances[row0 + i] = (float)p;
+    }
+    __syncthreads();
+  }
+
+  // Whether a sibling before s is the same token.
+  __device__ bool again(uint32_t s) const {
+    for (uint32_t b = m.child[t]; b != s; b = m.sibling[b])
+      if (m.token[b] == m.token[s]) return true;
+    return false;
+  }
+
+  // Down the tree; total(round) is the sum of (p - c·q)+, or below 0 where it is not known yet: false then.
+  template <class Total>
+  __device__ bool down(Total &&total_of) {
+    for (;;) {
+      double left = 1, total = 1;
+      c = 0;
+      uint32_t s = m.child[t];
+      for (; s != kKvNone; s = m.sibling[s]) {
+        const double u = (double)m.u[s], p = m.p[s], q = m.q[s];
+        if (p > 0 && (greedy ? true : drawn ? u * q * total < (p - c * q) * left : u * total < p && !again(s))) break;
+        if (drawn) {
+          if (left > 0) c += total / left;
+          if (a.distinct) left -= q;
+          total = total_of(round);
+          if (total < 0) return false;
+          round++;
+        } else if (!greedy && !again(s)) {
+          total -= p;
+        }
+      }
+      if (s == kKvNone) return true;
+      if (threadIdx.x == 0) m.path[kept] = s;
+      kept++;
+      t = s;
+    }
+  }
+
+  // Element i of (p - c·q)+, or of p in units of its largest; 0 behind the vocabulary.
+  struct Row {
+    const float *logits, *draft;
+    float top, inv, c;
+    uint32_t n_vocab;
+    __device__ float at(const Heat &heat, uint32_t i) const {
+      if (i >= n_vocab) return 0.f;
+      const float p = heat.weight(logit(logits[i]), top) * inv;
+      // (What the target does not have stays at 0, whatever the draft says.)
+      return draft && p > 0.f ? fmaxf(fmaf(-c, draft[i], p), 0.f) : p;
+    }
+  };
+  __device__ Row row() const {
+    const uint64_t at = (uint64_t)(row0 + t) * a.n_vocab;
+    return {a.logits + at, c > 0 ? a.draft + at : nullptr, fmaxf(m.top[t], -kLargest), c > 0 ? (float)(1.0 / m.sum[t]) : 1.f,
+            (float)c, a.n_vocab};
+  }
+  __device__ double *rest(uint32_t which) const { return a.rest + ((uint64_t)which * a.n_seqs + seq_at) * a.n_pieces; }
+  // The sum of a round's pieces (never below 0).
+  __device__ double total_of_pieces(uint32_t which, double *scratch) const {
+    const double *p = rest(which);
+    double sum = 0;
+    for (uint32_t i = threadIdx.x; i < a.n_pieces; i += THREADS) sum += p[i];
+    return block_sum_f64<THREADS>(sum, scratch);
+  }
+};
+
+__global__ __launch_bounds__(kRowThreads) void k_verify_rest(VerifyArgs a, uint32_t round) {
+  extern __shared__ double memory[];
+  __shared__ double scratch[kRowThreads / 64];
+  Walk<kRowThreads> w(a, blockIdx.x / a.n_pieces, memory);
+  const uint32_t piece = blockIdx.x % a.n_pieces;
+  if (!w.n || !w.drawn) return;
+  w.load(false);
+  if (w.down([&](uint32_t which) { return which < round ? w.total_of_pieces(which, scratch) : -1.0; })) return;
+  const auto row = w.row();
+  float sum = 0.f;
+#pragma unroll
+  for (uint32_t j = 0; j < kRowPer; j++) sum += row.at(w.heat, piece * kPiece + threadIdx.x + kRowThreads * j);
+  const double all = block_sum_f64<kRowThreads>((double)sum, scratch);
+  if (threadIdx.x == 0) w.rest(round)[piece] = all;
+}
+
 __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(VerifyArgs a) {
-  __shared__ float top_s[BCH_MAX_TREE];                      // of each token's row
-  __shared__ double sum_s[BCH_MAX_TREE];                     // its sum; greedy: unused
-  __shared__ uint32_t best_s[BCH_MAX_TREE];                  // the first place of its largest
-  __shared__ double p_s[BCH_MAX_TREE], q_s[BCH_MAX_TREE];    // of each drafted token after its parent
-  __shared__ uint32_t token_s[BCH_MAX_TREE], path_s[BCH_MAX_TREE];
-  __shared__ bool again_s[BCH_MAX_TREE];                     // a sibling before it is the same token
-  __shared__ double span_s[kWalkThreads];
-  __shared__ double part_s[kWalkWaves];
-  __shared__ uint32_t next_s;
-  const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
-  const KvSeq seq = a.seqs[blockIdx.x];
-  const uint32_t n = seq.n_new, row0 = seq.row - a.row0;
-  if (!n) {
+  constexpr uint32_t WAVES = kWalkThreads / 64, PER = kPiece / kWalkThreads;
+  extern __shared__ double memory[];
+  __shared__ double scratch[WAVES], before_s[WAVES];
+  __shared__ uint32_t pick_s[WAVES], some_s[WAVES];
+  const uint32_t tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
+  Walk<kWalkThreads> w(a, blockIdx.x, memory);
+  if (!w.n) {
     if (tid == 0) a.kept[blockIdx.x] = 0, a.next[blockIdx.x] = BCH_NO_TOKEN;
     return;
   }
-  const float temperature = a.temperatures[blockIdx.x];
-  const bool greedy = !(temperature > 0.f), drawn = a.draft && !greedy;
-  const Heat heat(greedy ? 1.f : temperature);
-  const double heat64 = (double)heat.hi + (double)heat.lo;
-  const KvNode *nodes = a.nodes ? a.nodes + row0 : nullptr;
-  auto parent_of = [&](uint32_t t) { return nodes ? nodes[t].parent : t - 1; };
-  auto child_of = [&](uint32_t t) { return nodes ? nodes[t].child : t + 1 < n ? t + 1 : kKvNone; };
-  auto sibling_of = [&](uint32_t t) { return nodes ? nodes[t].sibling : kKvNone; };
-
-  // The rows' pieces joined, a wave a row.
-  for (uint32_t t = wave; t < n; t += kWalkWaves) {
-    const VerifyPiece *p = a.pieces + (uint64_t)(row0 + t) * a.n_pieces;
-    float top = -INFINITY;
-    for (uint32_t i = lane; i < a.n_pieces; i += 64) top = fmaxf(top, p[i].top);
-    top = wave_max(top);
-    uint32_t best = ~0u;
-    double sum = 0;
-    for (uint32_t i = lane; i < a.n_pieces; i += 64) {
-      if (p[i].top == top) best = min(best, p[i].at);
-      if (p[i].top > -INFINITY) sum += (double)p[i].sum * exp2(((double)p[i].top - top) * heat64);
-    }
-#pragma unroll
-    for (int i = 1; i < 64; i *= 2) best = min(best, (uint32_t)__shfl_xor((int)best, i, 64));
-    sum = wave_sum_f64(sum);
-    if (lane == 0) top_s[t] = top, sum_s[t] = sum, best_s[t] = top > -INFINITY ? best : BCH_NO_TOKEN;
-  }
-  if (tid < n) token_s[tid] = a.tokens[row0 + tid];
-  __syncthreads();
-  // The target's probability of token x after token t.
-  auto chance = [&](uint32_t t, uint32_t x) {
-    if (x >= a.n_vocab || best_s[t] == BCH_NO_TOKEN) return 0.0;
-    if (greedy) return x == best_s[t] ? 1.0 : 0.0;
-    const float l = logit(a.logits[(uint64_t)(row0 + t) * a.n_vocab + x]);
-    return l > -INFINITY ? exp2(((double)l - top_s[t]) * heat64) / sum_s[t] : 0.0;
-  };
-  if (tid && tid < n) {
-    const uint32_t t = parent_of(tid), x = token_s[tid];
-    const double p = chance(t, x);
-    p_s[tid] = p;
-    q_s[tid] = drawn && x < a.n_vocab ? (double)a.draft[(uint64_t)(row0 + t) * a.n_vocab + x] : drawn ? 0.0 : 1.0;
-    if (a.chances) a.chances[row0 + tid] = (float)p;
-    bool again = false;
-    for (uint32_t s = child_of(t); s < tid; s = sibling_of(s)) again |= token_s[s] == x;
-    again_s[tid] = again;
-  }
-  if (tid < n) path_s[tid] = BCH_NO_TOKEN;
-  __syncthreads();
-
-  // What is left of p after token t: elements from `from` on, 64 at a time, of the
-  // row as weights (times the whole sum where children were drawn, which p - c·q needs
-  // normalised; otherwise as they are).  `fallen`: the rejected children.
-  uint32_t t = 0, kept = 1;
-  double c = 0, left = 1, total = 1;
-  auto weight = [&](uint32_t i, float top, float inv) {
-    if (i >= a.n_vocab) return 0.f;
-    const uint64_t at = (uint64_t)(row0 + t) * a.n_vocab + i;
-    const float p = heat.weight(logit(a.logits[at]), top) * inv;
-    // (What the target does not have stays at 0, whatever the draft says.)
-    return c > 0 && p > 0.f ? fmaxf(fmaf((float)-c, a.draft[at], p), 0.f) : p;
-  };
-  // The vocabulary in spans of whole 64s, at most kWalkThreads of them; a wave
-  // sums every kWalkWaves-th.  Their sums to span_s, the whole's is returned.
-  const uint32_t span = (a.n_vocab + kWalkThreads * 64 - 1) / (kWalkThreads * 64) * 64, spans = (a.n_vocab + span - 1) / span;
-  auto fallen = [&](uint32_t i) {  // whether element i is a rejected child's token (without a draft)
-    for (uint32_t s = child_of(t); s != kKvNone; s = sibling_of(s))
-      if (token_s[s] == i) return true;
-    return false;
-  };
-  auto sums = [&](bool without) {
-    const float top = fmaxf(top_s[t], -kLargest), inv = (float)(1.0 / sum_s[t]);
-    double all = 0;
-    for (uint32_t s = wave; s < spans; s += kWalkWaves) {
-      double sum = 0;
-      for (uint32_t i = s * span + lane; i < (s + 1) * span; i += 64) {
-        const float w = weight(i, top, inv);
-        sum += without && w > 0.f && fallen(i) ? 0.0 : (double)w;
+  w.load(a.chances != nullptr);
+  uint32_t latest = 0;  // the round whose pieces are those of the last c
+  w.down([&](uint32_t which) {
+    latest = min(which, a.rounds);
+    if (which >= a.rounds) {
+      // Further rejections: a wave sums every WAVES-th piece.
+      const auto row = w.row();
+      __syncthreads();
+      for (uint32_t piece = wave; piece < a.n_pieces; piece += WAVES) {
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (uint32_t j = 0; j < kPiece / 64; j++) sum[j % 4] += row.at(w.heat, piece * kPiece + 64 * j + lane);
+        const double all = wave_sum_f64(((double)sum[0] + sum[1]) + ((double)sum[2] + sum[3]));
+        if (lane == 0) w.rest(latest)[piece] = all;
       }
-      sum = wave_sum_f64(sum);
-      if (lane == 0) span_s[s] = sum;
-      all += sum;
+      __syncthreads();
     }
-    __syncthreads();
-    if (lane == 0) part_s[wave] = all;
-    __syncthreads();
-    all = 0;
-    for (uint32_t w = 0; w < kWalkWaves; w++) all += part_s[w];
-    return all;
-  };
-
-  if (tid == 0) path_s[0] = 0;
-  for (;;) {
-    c = 0, left = 1, total = 1;
-    uint32_t s = child_of(t);
-    for (; s != kKvNone; s = sibling_of(s)) {
-      const double u = (double)a.uniforms[row0 + s], p = p_s[s], q = q_s[s];
-      if (p > 0 && (greedy ? true : drawn ? u * q * total < (p - c * q) * left : u * total < (again_s[s] ? 0.0 : p))) break;
-      if (drawn) {
-        if (left > 0) c += total / left;
-        if (a.distinct) left -= q;
-        total = sums(false);
-      } else if (!greedy && !again_s[s]) {
-        total -= p;
-      }
-    }
-    if (s == kKvNone) break;
-    if (tid == 0) path_s[kept] = s;
-    kept++;
-    t = s;
-  }
+    return w.total_of_pieces(latest, scratch);
+  });
 
   // The next token.
-  if (tid == 0) next_s = greedy ? best_s[t] : BCH_NO_TOKEN;
-  __syncthreads();
-  if (!greedy && best_s[t] != BCH_NO_TOKEN) {
-    const bool without = !drawn && child_of(t) != kKvNone;
-    total = sums(without);
-    bool all = false;  // p itself
-    if (!(total > 0)) {
-      c = 0;
-      all = true;
-      total = sums(false);
-    }
-    // The span in which the sum passes the goal: a thread a span.
-    const double goal = (double)a.uniforms[row0] * total;
-    double mine = tid < spans ? span_s[tid] : 0, up = mine;
-#pragma unroll
-    for (int i = 1; i < 64; i *= 2) {
-      const double x = __shfl_up(up, i, 64);
-      if (lane >= (uint32_t)i) up += x;
-    }
-    __syncthreads();
-    if (lane == 63) part_s[wave] = up;
-    __syncthreads();
-    double before = 0;
-    for (uint32_t w = 0; w < wave; w++) before += part_s[w];
-    up += before;
-    span_s[tid] = up;  // the sum up to the span's end
-    __syncthreads();
-    // The first span whose end lies past the goal and that has any weight, or the last
-    // that has any.
-    uint32_t pick = tid < spans && mine > 0 && up > goal ? tid : ~0u, last = tid < spans && mine > 0 ? tid : 0;
-#pragma unroll
-    for (int i = 1; i < 64; i *= 2) {
-      pick = min(pick, (uint32_t)__shfl_xor((int)pick, i, 64));
-      last = max(last, (uint32_t)__shfl_xor((int)last, i, 64));
-    }
-    __shared__ uint32_t pick_s[kWalkWaves], last_s[kWalkWaves];
-    if (lane == 0) pick_s[wave] = pick, last_s[wave] = last;
-    __syncthreads();
-    if (wave == 0) {
-      for (uint32_t w = 0; w < kWalkWaves; w++) pick = min(pick, pick_s[w]), last = max(last, last_s[w]);
-      const uint32_t s = pick == ~0u ? last : pick;
-      double sum = s ? span_s[s - 1] : 0;
-      const float top = fmaxf(top_s[t], -kLargest), inv = (float)(1.0 / sum_s[t]);
-      uint32_t found = BCH_NO_TOKEN, some = BCH_NO_TOKEN;
-      for (uint32_t i0 = s * span; i0 < (s + 1) * span && found == BCH_NO_TOKEN; i0 += 64) {
-        const uint32_t i = i0 + lane;
-        const float w = weight(i, top, inv);
-        const double x = without && !all && w > 0.f && fallen(i) ? 0.0 : (double)w;
-        double run = x;
-#pragma unroll
-        for (int k = 1; k < 64; k *= 2) {
-          const double y = __shfl_up(run, k, 64);
-          if (lane >= (uint32_t)k) run += y;
+  uint32_t next = w.greedy ? w.m.best[w.t] : BCH_NO_TOKEN;
+  if (!w.greedy && w.m.best[w.t] != BCH_NO_TOKEN) {
+    bool without = !w.drawn && w.m.child[w.t] != kKvNone;  // without the children that were chosen
+    auto fallen = [&](uint32_t i) {
+      for (uint32_t s = w.m.child[w.t]; s != kKvNone; s = w.m.sibling[s])
+        if (w.m.token[s] == i) return true;
+      return false;
+    };
+    // A thread's pieces are consecutive.
+    const uint32_t per = (a.n_pieces + kWalkThreads - 1) / kWalkThreads, first = min(tid * per, a.n_pieces),
+                   end = min(first + per, a.n_pieces);
+    auto mass = [&](uint32_t piece) {
+      if (w.c > 0) return w.rest(latest)[piece];
+      const VerifyPiece p = a.pieces[(uint64_t)(w.row0 + w.t) * a.n_pieces + piece];
+      double sum = p.top > -INFINITY ? (double)p.sum * exp2(((double)p.top - w.m.top[w.t]) * w.heat64) : 0.0;
+      if (without) {
+        const auto row = w.row();
+        for (uint32_t s = w.m.child[w.t]; s != kKvNone; s = w.m.sibling[s]) {
+          const uint32_t x = w.m.token[s];
+          if (x < a.n_vocab && x / kPiece == piece && !w.again(s)) sum -= (double)row.at(w.heat, x);
         }
-        const uint64_t past = __builtin_amdgcn_ballot_w64(x > 0 && sum + run > goal), any = __builtin_amdgcn_ballot_w64(x > 0);
-        if (past) found = i0 + __ffsll((unsigned long long)past) - 1;
-        if (any) some = i0 + 63 - __clzll((long long)any);
-        sum += __shfl(run, 63, 64);
       }
-      if (lane == 0) next_s = found != BCH_NO_TOKEN ? found : some;
+      return fmax(sum, 0.0);
+    };
+    double mine = 0, up, total;
+    for (;;) {
+      mine = 0;
+      for (uint32_t i = first; i < end; i++) mine += mass(i);
+      up = mine;
+#pragma unroll
+      for (int i = 1; i < 64; i *= 2) {
+        const double x = __shfl_up(up, i, 64);
+        if (lane >= (uint32_t)i) up += x;
+      }
+      if (lane == 63) before_s[wave] = up;
+      __syncthreads();
+      double before = 0;
+      total = 0;
+      for (uint32_t i = 0; i < WAVES; i++) {
+        before += i < wave ? before_s[i] : 0;
+        total += before_s[i];
+      }
+      up += before;
+      if (total > 0 || (w.c == 0 && !without)) break;
+      w.c = 0, without = false;  // nothing is left: p itself
+      __syncthreads();
     }
+    const double goal = (double)w.m.u[0] * total;
+    // The first piece whose end lies past the goal; the last with any mass where rounding leaves none.
+    uint32_t pick = ~0u, some = 0;
+    double start = up - mine;
+    if (mine > 0) {
+      double sum = start;
+      for (uint32_t i = first; i < end; i++) {
+        const double x = mass(i);
+        if (x > 0) some = i;
+        if (x > 0 && pick == ~0u && sum + x > goal) pick = i, start = sum;
+        sum += x;
+      }
+    }
+    uint32_t lowest = pick, highest = some;
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) {
+      lowest = min(lowest, (uint32_t)__shfl_xor((int)lowest, i, 64));
+      highest = max(highest, (uint32_t)__shfl_xor((int)highest, i, 64));
+    }
+    if (lane == 0) pick_s[wave] = lowest, some_s[wave] = highest;
     __syncthreads();
+    for (uint32_t i = 0; i < WAVES; i++) lowest = min(lowest, pick_s[i]), highest = max(highest, some_s[i]);
+    if (lowest != ~0u && pick == lowest) scratch[0] = start;
+    __syncthreads();
+    double sum = lowest == ~0u ? 2 * total : scratch[0];  // (past every goal: the piece's last token with any)
+    __syncthreads();
+    // The token in the piece.  Its own sum may end below the goal by rounding: the last token with any weight
+    // then, or where it has none (all of it was fallen children) the pieces behind it, then those before.
+    const auto row = w.row();
+    const uint32_t from = lowest == ~0u ? highest : lowest;
+    uint32_t found = BCH_NO_TOKEN;
+    for (uint32_t k = 0; k < a.n_pieces && found == BCH_NO_TOKEN; k++) {
+      const uint32_t piece = from + k < a.n_pieces ? from + k : a.n_pieces - 1 - k;
+      float x[PER];
+      double run = 0;
+#pragma unroll
+      for (uint32_t j = 0; j < PER; j++) {
+        const uint32_t i = piece * kPiece + PER * tid + j;
+        x[j] = row.at(w.heat, i);
+        if (without && x[j] > 0.f && fallen(i)) x[j] = 0.f;
+        run += (double)x[j];
+      }
+      double up = run;
+#pragma unroll
+      for (int i = 1; i < 64; i *= 2) {
+        const double y = __shfl_up(up, i, 64);
+        if (lane >= (uint32_t)i) up += y;
+      }
+      if (lane == 63) before_s[wave] = up;
+      __syncthreads();
+      double at = sum + up - run;
+      for (uint32_t i = 0; i < wave; i++) at += before_s[i];
+      uint32_t pick = BCH_NO_TOKEN, last = 0;
+#pragma unroll
+      for (uint32_t j = 0; j < PER; j++) {
+        at += (double)x[j];
+        const uint32_t i = piece * kPiece + PER * tid + j;
+        if (x[j] > 0.f) last = i + 1;
+        if (x[j] > 0.f && pick == BCH_NO_TOKEN && at > goal && lowest != ~0u) pick = i;
+      }
+#pragma unroll
+      for (int i = 1; i < 64; i *= 2) {
+        pick = min(pick, (uint32_t)__shfl_xor((int)pick, i, 64));
+        last = max(last, (uint32_t)__shfl_xor((int)last, i, 64));
+      }
+      if (lane == 0) pick_s[wave] = pick, some_s[wave] = last;
+      __syncthreads();
+      for (uint32_t i = 0; i < WAVES; i++) pick = min(pick, pick_s[i]), last = max(last, some_s[i]);
+      found = pick != BCH_NO_TOKEN ? pick : last ? last - 1 : BCH_NO_TOKEN;
+      __syncthreads();
+    }
+    next = found;
   }
-  if (tid < n) a.path[row0 + tid] = path_s[tid];
+  __syncthreads();  // (the path is thread 0's)
+  for (uint32_t i = tid; i < w.n; i += kWalkThreads) a.path[w.row0 + i] = w.m.path[i];
   if (tid == 0) {
-    a.kept[blockIdx.x] = kept;
-    a.next[blockIdx.x] = next_s;
-    if (a.chances) a.chances[row0] = next_s == BCH_NO_TOKEN ? 0.f : (float)chance(t, next_s);
+    a.kept[blockIdx.x] = w.kept;
+    a.next[blockIdx.x] = next;
+    if (a.chances) a.chances[w.row0] = next == BCH_NO_TOKEN ? 0.f : (float)w.chance(w.t, next);
   }
 }
 
@@ -342,7 +517,7 @@ extern "C" int bch_verify_drafts(bch_ctx *ctx, const bch_kv_plan *plan, uint32_t
   }
   a.n_seqs = n_seqs;
   a.n_vocab = n_vocab;
-  a.n_pieces = div_ceil(n_vocab, kRowPiece);
+  a.n_pieces = div_ceil(n_vocab, kPiece);
   a.distinct = drafts->distinct != 0;
   if ((uint64_t)a.n_rows * a.n_pieces >= 1u << 23) return fail(BCH_ERR_ARGUMENT, "verify_drafts: too many logits");
   const uint64_t rows = a.n_rows, bytes = rows * n_vocab * 4;
@@ -376,15 +551,26 @@ extern "C" int bch_verify_drafts(bch_ctx *ctx, const bch_kv_plan *plan, uint32_t
   for (const Part &x : out)
     if (reinterpret_cast<uintptr_t>(x.at) % 4) return fail(BCH_ERR_ARGUMENT, "verify_drafts: operands must be 4-byte aligned");
   if (!ctx->recording && !ctx->capturing) return fail(BCH_ERR_NOT_RECORDING, "no recording is open");
+  for (uint32_t i = first; i < first + n_seqs; i++) a.most = std::max(a.most, plan->seqs[i].n_new);
+  a.rounds = !a.draft || a.most < 2 ? 0 : plan->d_nodes ? std::min(kRounds, a.most - 1) : 1;
+  const uint64_t pieces = rows * a.n_pieces * sizeof(VerifyPiece), rest = (uint64_t)n_seqs * a.n_pieces * 8;
   void *scratch;
-  BCH_TRY(ctx_scratch(ctx, std::max<uint64_t>(rows * a.n_pieces * sizeof(VerifyPiece), 16), &scratch));
+  BCH_TRY(ctx_scratch(ctx, pieces + (a.rounds + 1) * rest + 16, &scratch));
   a.pieces = static_cast<VerifyPiece *>(scratch);
+  a.rest = reinterpret_cast<double *>(static_cast<char *>(scratch) + pieces);
   return launch(ctx, {"verify_drafts", a.n_rows, n_vocab, 0}, [&](hipStream_t st) {
     if (!n_seqs) return;
     kv_plan_use(ctx, plan);
     a.seqs = plan->d_seqs + first;
     a.nodes = plan->d_nodes ? plan->d_nodes + a.row0 : nullptr;
-    if (a.n_rows) k_verify_rows<<<a.n_rows * a.n_pieces, kRowThreads, 0, st>>>(a);
-    k_verify_walk<<<n_seqs, kWalkThreads, 0, st>>>(a);
+    const uint32_t memory = a.most * kWalkBytes;
+    if (a.n_rows) {
+      if (n_vocab % 4 == 0 && reinterpret_cast<uintptr_t>(a.logits) % 16 == 0)
+        k_verify_rows<true><<<a.n_rows * a.n_pieces, kRowThreads, 0, st>>>(a);
+      else
+        k_verify_rows<false><<<a.n_rows * a.n_pieces, kRowThreads, 0, st>>>(a);
+    }
+    for (uint32_t i = 0; i < a.rounds; i++) k_verify_rest<<<n_seqs * a.n_pieces, kRowThreads, memory, st>>>(a, i);
+    k_verify_walk<<<n_seqs, kWalkThreads, memory, st>>>(a);
   });
 }
