@@ -13,15 +13,14 @@
 // vocabulary.  For children chosen without chance (q is 1 for each in its turn) what is left
 // is p without them, and a rejection costs nothing.
 //
-// Three steps, each a launch, so that none waits for another inside a kernel.
 //   k_verify_rows reads every token's logits once, in pieces of the vocabulary: the
 //     largest, the first place of it, and the sum of the exponentials.
-//   k_verify_rest (where there is a draft) sums pieces of (p - c·q)+ for one rejection of each
-//     sequence.  All its workgroups walk down the tree for themselves, out of LDS, up to where a sum
-//     is missing: a few microseconds of latency, where one workgroup's sum over the vocabulary takes
-//     70 us.
-//   k_verify_walk, a workgroup for each sequence, walks to the end (summing by itself what further
-//     rejections need) and draws: the piece in which the sum passes its goal, then the token in it.
+//   k_verify_walk walks down each tree, out of LDS, and draws: the piece in which the sum passes
+//     its goal, then the token in it.  Without a draft a workgroup does a sequence.  With one
+//     (REST) a workgroup for each piece walks by itself to where the sum for a rejection is missing,
+//     adds its own piece to it, and the last one to do so goes on.  (One workgroup's sum
+//     over the whole vocabulary takes about 70 us.)  For trees there are launches before it that only add pieces,
+//     for the first rejections; what those do not cover the last workgroup sums alone.
 #include <algorithm>
 #include <cmath>
 
@@ -33,8 +32,8 @@
 namespace bch {
 
 constexpr uint32_t kRowThreads = 256, kRowPer = 16, kPiece = kRowThreads * kRowPer;
-constexpr uint32_t kWalkThreads = 1024;
-constexpr uint32_t kRounds = 3;  // of k_verify_rest for trees (for chains one is all)
+constexpr uint32_t kWalkThreads = 256;
+constexpr uint32_t kRounds = 3;  // rejections of trees that all workgroups sum (of chains there is one at most)
 constexpr float kLargest = 3.402823466e38f;
 
 // One piece of a row: its largest logit, where it is first, and the sum of
@@ -54,8 +53,9 @@ struct VerifyArgs {
   const KvNode *nodes;          // from the first token on, or null: chains
   VerifyPiece *pieces;          // [row][piece]
   double *rest;                 // [round][sequence][piece], one round more than `rounds`
+  uint32_t *arrived;            // [sequence]
   uint32_t n_seqs, row0, n_rows, n_vocab, n_pieces, distinct;
-  uint32_t rounds, most;        // rejections that k_verify_rest sums; the most tokens of a sequence
+  uint32_t rounds, most;        // rejections that are summed by all workgroups; the most tokens of a sequence
 };
 
 // A logit as it counts: NaN as -inf, +inf as the largest float.
@@ -84,17 +84,19 @@ __device__ __forceinline__ double wave_sum_f64(double x) {
   return x;
 }
 
-// Over a workgroup; `scratch` holds a double a wave and is free again afterwards.
-template <uint32_t THREADS>
-__device__ __forceinline__ double block_sum_f64(double x, double *scratch) {
-  x = wave_sum_f64(x);
-  if (threadIdx.x % 64 == 0) scratch[threadIdx.x / 64] = x;
-  __syncthreads();
-  double all = 0;
+// The sum of the lanes up to and with this one.
+__device__ __forceinline__ double wave_scan_f64(double x) {
 #pragma unroll
-  for (uint32_t w = 0; w < THREADS / 64; w++) all += scratch[w];
-  __syncthreads();
-  return all;
+  for (int i = 1; i < 64; i *= 2) {
+    const double y = __shfl_up(x, i, 64);
+    if (threadIdx.x % 64 >= (uint32_t)i) x += y;
+  }
+  return x;
+}
+__device__ __forceinline__ uint32_t wave_min_u32(uint32_t x) {
+#pragma unroll
+  for (int i = 1; i < 64; i *= 2) x = min(x, (uint32_t)__shfl_xor((int)x, i, 64));
+  return x;
 }
 
 // The sequence of a row (rows of a sequence are consecutive): the last that
@@ -132,7 +134,9 @@ __global__ __launch_bounds__(kRowThreads) void k_verify_rows(VerifyArgs a) {
 #pragma unroll
     for (uint32_t j = 0; j < kRowPer; j++) x[j] = p[min(place(j), len - 1)];
   }
-  const float temperature = a.temperatures[seq_of_row(a, row)];
+  const uint32_t seq = seq_of_row(a, row);
+  const float temperature = a.temperatures[seq];
+  if (piece == 0 && tid == 0 && a.seqs[seq].row - a.row0 == row) a.arrived[seq] = 0;
   float top = -INFINITY;
 #pragma unroll
   for (uint32_t j = 0; j < kRowPer; j++) {
@@ -145,8 +149,7 @@ __global__ __launch_bounds__(kRowThreads) void k_verify_rows(VerifyArgs a) {
 #pragma unroll
   for (int j = kRowPer - 1; j >= 0; j--)
     if (x[j] == top) at = base + place(j);
-#pragma unroll
-  for (int i = 1; i < 64; i *= 2) at = min(at, (uint32_t)__shfl_xor((int)at, i, 64));
+  at = wave_min_u32(at);
   float sum = 0.f;
   if (temperature > 0.f && top > -INFINITY) {
     const Heat heat(temperature);
@@ -173,7 +176,6 @@ struct WalkMemory {
 };
 constexpr uint32_t kWalkBytes = 3 * 8 + 7 * 4;  // a token
 
-template <uint32_t THREADS>
 struct Walk {
   const VerifyArgs &a;
   const uint32_t seq_at;
@@ -205,20 +207,21 @@ struct Walk {
   __device__ void load(bool chances) {
     const uint32_t tid = threadIdx.x, lane = tid % 16;
     const KvNode *nodes = a.nodes ? a.nodes + row0 : nullptr;
-    for (uint32_t i = tid; i < n; i += THREADS) {
+    for (uint32_t i = tid; i < n; i += kWalkThreads) {
       m.token[i] = a.tokens[row0 + i];
       m.u[i] = a.uniforms[row0 + i];
       m.child[i] = nodes ? nodes[i].child : i + 1 < n ? i + 1 : kKvNone;
       m.sibling[i] = nodes ? nodes[i].sibling : kKvNone;
-      m.path[i] = i ? BCH_NO_TOKEN : 0;
+      m.path[i] = nodes ? nodes[i].parent : i - 1;  // (until the probabilities are known)
     }
-    for (uint32_t i0 = 0; i0 < n; i0 += THREADS / 16) {
+    for (uint32_t i0 = 0; i0 < n; i0 += kWalkThreads / 16) {
       const uint32_t i = min(i0 + tid / 16, n - 1);
       const VerifyPiece *p = a.pieces + (uint64_t)(row0 + i) * a.n_pieces;
       // (A running sum: rows of up to 64 pieces, 262,144 tokens, in one round of loads.)
       float top = -INFINITY;
       double sum = 0;
       uint32_t best = ~0u;
+#pragma unroll 1
       for (uint32_t j0 = 0; j0 < a.n_pieces; j0 += 64) {
         VerifyPiece x[4];
 #pragma unroll
@@ -230,15 +233,15 @@ struct Walk {
           best = x[k].top > top ? x[k].at : best;  // (pieces go up, and so do the places)
           top = fmaxf(top, x[k].top);
         }
-        if (before > -INFINITY) sum *= exp2(((double)before - top) * heat64);
+        if (before > -INFINITY) sum *= heat.weight(before, top);
 #pragma unroll
         for (uint32_t k = 0; k < 4; k++)
-          if (x[k].top > -INFINITY) sum += (double)x[k].sum * exp2(((double)x[k].top - top) * heat64);
+          if (x[k].top > -INFINITY) sum += (double)x[k].sum * heat.weight(x[k].top, top);
       }
       float all = top;
 #pragma unroll
       for (int k = 1; k < 16; k *= 2) all = fmaxf(all, __shfl_xor(all, k, 64));
-      if (top > -INFINITY) sum *= exp2(((double)top - all) * heat64);
+      if (top > -INFINITY) sum *= heat.weight(top, all);
       if (top != all) best = ~0u;
 #pragma unroll
       for (int k = 1; k < 16; k *= 2) {
@@ -248,41 +251,44 @@ struct Walk {
       if (lane == 0) m.top[i] = all, m.sum[i] = sum, m.best[i] = all > -INFINITY ? best : BCH_NO_TOKEN;
     }
     __syncthreads();
-    for (uint32_t i = tid; i < n; i += THREADS) {
-      if (!i) continue;
-      const uint32_t up = nodes ? nodes[i].parent : i - 1, x = m.token[i];
+    for (uint32_t i = tid; i < n; i += kWalkThreads) {
+      if (!i) {
+        m.path[0] = 0;
+        continue;
+      }
+      const uint32_t up = m.path[i], x = m.token[i];
       const double p = chance(up, x);
-      m.p[i] = p;
+      // (Children chosen without chance that name a token again find nothing left of it.)
+      bool again = false;
+      if (!drawn)
+        for (uint32_t s = m.child[up]; s != i; s = m.sibling[s]) again |= m.token[s] == x;
+      m.p[i] = again ? 0.0 : p;
       m.q[i] = !drawn ? 1.0 : x < a.n_vocab ? (double)a.draft[(uint64_t)(row0 + up) * a.n_vocab + x] : 0.0;
+      m.path[i] = BCH_NO_TOKEN;
       if (chances) a.chances[row0 + i] = (float)p;
     }
     __syncthreads();
   }
 
-  // Whether a sibling before s is the same token.
-  __device__ bool again(uint32_t s) const {
-    for (uint32_t b = m.child[t]; b != s; b = m.sibling[b])
-      if (m.token[b] == m.token[s]) return true;
-    return false;
-  }
-
-  // Down the tree; total(round) is the sum of (p - c·q)+, or below 0 where it is not known yet: false then.
+  // Down the tree from its first token; total_of(round) is the sum of (p - c·q)+, or below 0 where it is not
+  // known yet: false then.
   template <class Total>
   __device__ bool down(Total &&total_of) {
+    t = 0, kept = 1, round = 0;
     for (;;) {
       double left = 1, total = 1;
       c = 0;
       uint32_t s = m.child[t];
       for (; s != kKvNone; s = m.sibling[s]) {
         const double u = (double)m.u[s], p = m.p[s], q = m.q[s];
-        if (p > 0 && (greedy ? true : drawn ? u * q * total < (p - c * q) * left : u * total < p && !again(s))) break;
+        if (p > 0 && (greedy ? true : drawn ? u * q * total < (p - c * q) * left : u * total < p)) break;
         if (drawn) {
           if (left > 0) c += total / left;
           if (a.distinct) left -= q;
           total = total_of(round);
           if (total < 0) return false;
           round++;
-        } else if (!greedy && !again(s)) {
+        } else if (!greedy) {
           total -= p;
         }
       }
@@ -293,206 +299,233 @@ struct Walk {
     }
   }
 
-  // Element i of (p - c·q)+, or of p in units of its largest; 0 behind the vocabulary.
-  struct Row {
+  // A piece of (p - c·q)+ after the current token, or of p in units of its largest; 0 behind the vocabulary.
+  struct Piece {
     const float *logits, *draft;
     float top, inv, c;
-    uint32_t n_vocab;
-    __device__ float at(const Heat &heat, uint32_t i) const {
-      if (i >= n_vocab) return 0.f;
-      const float p = heat.weight(logit(logits[i]), top) * inv;
-      // (What the target does not have stays at 0, whatever the draft says.)
-      return draft && p > 0.f ? fmaxf(fmaf(-c, draft[i], p), 0.f) : p;
+    uint32_t len;
+    // Elements `first` + STRIDE·j of it, all on their way before one is used.  (Buffer loads end at the
+    // piece by themselves: clamped places would take a register each.)
+    template <uint32_t STRIDE, uint32_t N>
+    __device__ __forceinline__ void load(const Heat &heat, float (&x)[N], uint32_t first) const {
+      float d[N];
+      auto bring = [&](float (&to)[N], const float *from) __attribute__((always_inline)) {
+        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(from), 0, len * 4, 0x00020000);
+#pragma unroll
+        for (uint32_t j = 0; j < N; j++)
+          to[j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsrc, 4 * first, 4 * STRIDE * j, 0));
+      };
+      bring(x, logits);
+      if (draft) bring(d, draft);
+#pragma unroll
+      for (uint32_t j = 0; j < N; j++) {
+        const float p = first + STRIDE * j < len ? heat.weight(logit(x[j]), top) * inv : 0.f;
+        // (What the target does not have stays at 0, whatever the draft says.)
+        x[j] = draft && p > 0.f ? fmaxf(fmaf(-c, d[j], p), 0.f) : p;
+      }
     }
   };
-  __device__ Row row() const {
-    const uint64_t at = (uint64_t)(row0 + t) * a.n_vocab;
+  __device__ Piece piece_of(uint32_t piece) const {  // (the same for a wave)
+    const uint32_t at_t = __builtin_amdgcn_readfirstlane(t), from = __builtin_amdgcn_readfirstlane(piece) * kPiece;
+    const uint64_t at = (uint64_t)(row0 + at_t) * a.n_vocab + from;
     return {a.logits + at, c > 0 ? a.draft + at : nullptr, fmaxf(m.top[t], -kLargest), c > 0 ? (float)(1.0 / m.sum[t]) : 1.f,
-            (float)c, a.n_vocab};
+            (float)c, min(kPiece, a.n_vocab - from)};
   }
   __device__ double *rest(uint32_t which) const { return a.rest + ((uint64_t)which * a.n_seqs + seq_at) * a.n_pieces; }
-  // The sum of a round's pieces (never below 0).
-  __device__ double total_of_pieces(uint32_t which, double *scratch) const {
+  // The sum of a round's pieces (never below 0), by each wave for itself.
+  double held = 0;  // of up to 64 pieces this lane's of the last round
+  __device__ double total_of_pieces(uint32_t which) {
     const double *p = rest(which);
     double sum = 0;
-    for (uint32_t i = threadIdx.x; i < a.n_pieces; i += THREADS) sum += p[i];
-    return block_sum_f64<THREADS>(sum, scratch);
+    for (uint32_t i = threadIdx.x % 64; i < a.n_pieces; i += 64) sum += coherent_load(p + i);
+    held = sum;
+    return wave_sum_f64(sum);
   }
-};
-
-__global__ __launch_bounds__(kRowThreads) void k_verify_rest(VerifyArgs a, uint32_t round) {
-  extern __shared__ double memory[];
-  __shared__ double scratch[kRowThreads / 64];
-  Walk<kRowThreads> w(a, blockIdx.x / a.n_pieces, memory);
-  const uint32_t piece = blockIdx.x % a.n_pieces;
-  if (!w.n || !w.drawn) return;
-  w.load(false);
-  if (w.down([&](uint32_t which) { return which < round ? w.total_of_pieces(which, scratch) : -1.0; })) return;
-  const auto row = w.row();
-  float sum = 0.f;
+  // A wave's sum of a piece of it.
+  __device__ double piece_by_wave(uint32_t piece) const {
+    const Piece part = piece_of(piece);
+    double sum = 0;
+#pragma unroll 1
+    for (uint32_t j0 = 0; j0 < kPiece / 64; j0 += 8) {
+      float x[8], all = 0.f;
+      part.load<64>(heat, x, 64 * j0 + threadIdx.x % 64);
 #pragma unroll
-  for (uint32_t j = 0; j < kRowPer; j++) sum += row.at(w.heat, piece * kPiece + threadIdx.x + kRowThreads * j);
-  const double all = block_sum_f64<kRowThreads>((double)sum, scratch);
-  if (threadIdx.x == 0) w.rest(round)[piece] = all;
-}
-
-__global__ __launch_bounds__(kWalkThreads) void k_verify_walk(VerifyArgs a) {
-  constexpr uint32_t WAVES = kWalkThreads / 64, PER = kPiece / kWalkThreads;
-  extern __shared__ double memory[];
-  __shared__ double scratch[WAVES], before_s[WAVES];
-  __shared__ uint32_t pick_s[WAVES], some_s[WAVES];
-  const uint32_t tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
-  Walk<kWalkThreads> w(a, blockIdx.x, memory);
-  if (!w.n) {
-    if (tid == 0) a.kept[blockIdx.x] = 0, a.next[blockIdx.x] = BCH_NO_TOKEN;
-    return;
-  }
-  w.load(a.chances != nullptr);
-  uint32_t latest = 0;  // the round whose pieces are those of the last c
-  w.down([&](uint32_t which) {
-    latest = min(which, a.rounds);
-    if (which >= a.rounds) {
-      // Further rejections: a wave sums every WAVES-th piece.
-      const auto row = w.row();
-      __syncthreads();
-      for (uint32_t piece = wave; piece < a.n_pieces; piece += WAVES) {
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-        for (uint32_t j = 0; j < kPiece / 64; j++) sum[j % 4] += row.at(w.heat, piece * kPiece + 64 * j + lane);
-        const double all = wave_sum_f64(((double)sum[0] + sum[1]) + ((double)sum[2] + sum[3]));
-        if (lane == 0) w.rest(latest)[piece] = all;
-      }
-      __syncthreads();
+      for (uint32_t j = 0; j < 8; j++) all += x[j];
+      sum += (double)all;
     }
-    return w.total_of_pieces(latest, scratch);
-  });
+    return wave_sum_f64(sum);
+  }
 
-  // The next token.
-  uint32_t next = w.greedy ? w.m.best[w.t] : BCH_NO_TOKEN;
-  if (!w.greedy && w.m.best[w.t] != BCH_NO_TOKEN) {
-    bool without = !w.drawn && w.m.child[w.t] != kKvNone;  // without the children that were chosen
-    auto fallen = [&](uint32_t i) {
-      for (uint32_t s = w.m.child[w.t]; s != kKvNone; s = w.m.sibling[s])
-        if (w.m.token[s] == i) return true;
-      return false;
-    };
-    // A thread's pieces are consecutive.
-    const uint32_t per = (a.n_pieces + kWalkThreads - 1) / kWalkThreads, first = min(tid * per, a.n_pieces),
-                   end = min(first + per, a.n_pieces);
+  // The next token; `latest` is the round of the last c.
+  __device__ uint32_t next(uint32_t latest) {
+    constexpr uint32_t WAVES = kWalkThreads / 64, PER = kPiece / kWalkThreads;
+    __shared__ double run_s[WAVES];
+    __shared__ uint32_t pick_s[WAVES], last_s[WAVES];
+    __shared__ float x_s[kWalkThreads * (PER + 1)];  // (a place in 17 is free: no bank is met twice)
+    const uint32_t tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
+    if (greedy || m.best[t] == BCH_NO_TOKEN) return m.best[t];
+    bool without = !drawn && m.child[t] != kKvNone;  // without the children that were chosen
     auto mass = [&](uint32_t piece) {
-      if (w.c > 0) return w.rest(latest)[piece];
-      const VerifyPiece p = a.pieces[(uint64_t)(w.row0 + w.t) * a.n_pieces + piece];
-      double sum = p.top > -INFINITY ? (double)p.sum * exp2(((double)p.top - w.m.top[w.t]) * w.heat64) : 0.0;
-      if (without) {
-        const auto row = w.row();
-        for (uint32_t s = w.m.child[w.t]; s != kKvNone; s = w.m.sibling[s]) {
-          const uint32_t x = w.m.token[s];
-          if (x < a.n_vocab && x / kPiece == piece && !w.again(s)) sum -= (double)row.at(w.heat, x);
-        }
-      }
+      if (c > 0) return a.n_pieces <= 64 ? held : coherent_load(rest(latest) + piece);
+      const VerifyPiece p = a.pieces[(uint64_t)(row0 + t) * a.n_pieces + piece];
+      double sum = p.top > -INFINITY ? (double)p.sum * heat.weight(p.top, m.top[t]) : 0.0;
+      if (without)
+        for (uint32_t s = m.child[t]; s != kKvNone; s = m.sibling[s])
+          if (m.token[s] / kPiece == piece) sum -= m.p[s] * m.sum[t];
       return fmax(sum, 0.0);
     };
-    double mine = 0, up, total;
+    // Every wave finds the piece for itself, a lane has `per` consecutive ones.
+    const uint32_t per = (a.n_pieces + 63) / 64, first = min(lane * per, a.n_pieces), end = min(first + per, a.n_pieces);
+    double mine, up, total;
     for (;;) {
       mine = 0;
       for (uint32_t i = first; i < end; i++) mine += mass(i);
-      up = mine;
-#pragma unroll
-      for (int i = 1; i < 64; i *= 2) {
-        const double x = __shfl_up(up, i, 64);
-        if (lane >= (uint32_t)i) up += x;
-      }
-      if (lane == 63) before_s[wave] = up;
-      __syncthreads();
-      double before = 0;
-      total = 0;
-      for (uint32_t i = 0; i < WAVES; i++) {
-        before += i < wave ? before_s[i] : 0;
-        total += before_s[i];
-      }
-      up += before;
-      if (total > 0 || (w.c == 0 && !without)) break;
-      w.c = 0, without = false;  // nothing is left: p itself
-      __syncthreads();
+      up = wave_scan_f64(mine);
+      total = __shfl(up, 63, 64);
+      if (total > 0 || (c == 0 && !without)) break;
+      c = 0, without = false;  // nothing is left: p itself
     }
-    const double goal = (double)w.m.u[0] * total;
     // The first piece whose end lies past the goal; the last with any mass where rounding leaves none.
-    uint32_t pick = ~0u, some = 0;
-    double start = up - mine;
-    if (mine > 0) {
-      double sum = start;
+    const double goal = (double)m.u[0] * total;
+    const uint64_t past = __builtin_amdgcn_ballot_w64(mine > 0 && up > goal), any = __builtin_amdgcn_ballot_w64(mine > 0);
+    const bool inside = past != 0;
+    const uint32_t owner = inside ? __ffsll((unsigned long long)past) - 1 : any ? 63 - __clzll((long long)any) : 0;
+    double sum = up - mine;
+    uint32_t from = first;
+    if (per > 1) {
+      double at = sum;
+      uint32_t pick = ~0u;
       for (uint32_t i = first; i < end; i++) {
         const double x = mass(i);
-        if (x > 0) some = i;
-        if (x > 0 && pick == ~0u && sum + x > goal) pick = i, start = sum;
-        sum += x;
+        if (x > 0 && (pick == ~0u || !inside)) {
+          if (!inside || at + x > goal) pick = i, sum = at;
+        }
+        at += x;
       }
+      from = pick != ~0u ? pick : first;
     }
-    uint32_t lowest = pick, highest = some;
-#pragma unroll
-    for (int i = 1; i < 64; i *= 2) {
-      lowest = min(lowest, (uint32_t)__shfl_xor((int)lowest, i, 64));
-      highest = max(highest, (uint32_t)__shfl_xor((int)highest, i, 64));
-    }
-    if (lane == 0) pick_s[wave] = lowest, some_s[wave] = highest;
-    __syncthreads();
-    for (uint32_t i = 0; i < WAVES; i++) lowest = min(lowest, pick_s[i]), highest = max(highest, some_s[i]);
-    if (lowest != ~0u && pick == lowest) scratch[0] = start;
-    __syncthreads();
-    double sum = lowest == ~0u ? 2 * total : scratch[0];  // (past every goal: the piece's last token with any)
-    __syncthreads();
+    sum = __shfl(sum, owner, 64);
+    from = __builtin_amdgcn_readfirstlane(__shfl((int)from, owner, 64));
     // The token in the piece.  Its own sum may end below the goal by rounding: the last token with any weight
     // then, or where it has none (all of it was fallen children) the pieces behind it, then those before.
-    const auto row = w.row();
-    const uint32_t from = lowest == ~0u ? highest : lowest;
-    uint32_t found = BCH_NO_TOKEN;
-    for (uint32_t k = 0; k < a.n_pieces && found == BCH_NO_TOKEN; k++) {
+#pragma unroll 1
+    for (uint32_t k = 0; k < a.n_pieces; k++) {
       const uint32_t piece = from + k < a.n_pieces ? from + k : a.n_pieces - 1 - k;
-      float x[PER];
+      // Read side by side, and taken PER in a row.  (Eight at a time, for the registers.)
+      {
+        const Piece part = piece_of(piece);
+#pragma unroll 1
+        for (uint32_t i0 = tid; i0 < kPiece; i0 += kWalkThreads * 8) {
+          float x[8];
+          part.load<kWalkThreads>(heat, x, i0);
+#pragma unroll
+          for (uint32_t j = 0; j < 8; j++) {
+            const uint32_t i = i0 + kWalkThreads * j;
+            x_s[i + i / PER] = x[j];
+          }
+        }
+      }
+      __syncthreads();
+      if (without) {
+        for (uint32_t s = m.child[t]; s != kKvNone; s = m.sibling[s]) {
+          const uint32_t i = m.token[s] - piece * kPiece;
+          if (i < kPiece) x_s[i + i / PER] = 0.f;  // (every thread the same)
+        }
+        __syncthreads();
+      }
+      const float *mine_s = x_s + tid * (PER + 1);
       double run = 0;
-#pragma unroll
-      for (uint32_t j = 0; j < PER; j++) {
-        const uint32_t i = piece * kPiece + PER * tid + j;
-        x[j] = row.at(w.heat, i);
-        if (without && x[j] > 0.f && fallen(i)) x[j] = 0.f;
-        run += (double)x[j];
-      }
-      double up = run;
-#pragma unroll
-      for (int i = 1; i < 64; i *= 2) {
-        const double y = __shfl_up(up, i, 64);
-        if (lane >= (uint32_t)i) up += y;
-      }
-      if (lane == 63) before_s[wave] = up;
+#pragma unroll 4
+      for (uint32_t j = 0; j < PER; j++) run += (double)mine_s[j];
+      const double upto = wave_scan_f64(run);
+      if (lane == 63) run_s[wave] = upto;
       __syncthreads();
-      double at = sum + up - run;
-      for (uint32_t i = 0; i < wave; i++) at += before_s[i];
-      uint32_t pick = BCH_NO_TOKEN, last = 0;
-#pragma unroll
+      double at = sum + upto - run;
+      for (uint32_t i = 0; i < wave; i++) at += run_s[i];
+      uint32_t pick = ~0u, last = ~0u;  // (last: counted down, so that the least is the last)
+#pragma unroll 4
       for (uint32_t j = 0; j < PER; j++) {
-        at += (double)x[j];
+        const float x = mine_s[j];
+        at += (double)x;
         const uint32_t i = piece * kPiece + PER * tid + j;
-        if (x[j] > 0.f) last = i + 1;
-        if (x[j] > 0.f && pick == BCH_NO_TOKEN && at > goal && lowest != ~0u) pick = i;
+        if (x > 0.f) last = ~i;
+        if (x > 0.f && pick == ~0u && at > goal && inside) pick = i;
       }
-#pragma unroll
-      for (int i = 1; i < 64; i *= 2) {
-        pick = min(pick, (uint32_t)__shfl_xor((int)pick, i, 64));
-        last = max(last, (uint32_t)__shfl_xor((int)last, i, 64));
-      }
-      if (lane == 0) pick_s[wave] = pick, some_s[wave] = last;
+      pick = wave_min_u32(pick), last = wave_min_u32(last);
+      if (lane == 0) pick_s[wave] = pick, last_s[wave] = last;
       __syncthreads();
-      for (uint32_t i = 0; i < WAVES; i++) pick = min(pick, pick_s[i]), last = max(last, some_s[i]);
-      found = pick != BCH_NO_TOKEN ? pick : last ? last - 1 : BCH_NO_TOKEN;
+      for (uint32_t i = 0; i < WAVES; i++) pick = min(pick, pick_s[i]), last = min(last, last_s[i]);
+      if (pick != ~0u) return pick;
+      if (last != ~0u) return ~last;
       __syncthreads();
     }
-    next = found;
+    return BCH_NO_TOKEN;
   }
+};
+
+// REST: workgroups for every piece of every sequence, of which those of the last launch also end the walk.
+template <bool REST>
+__global__ __launch_bounds__(kWalkThreads, REST ? 6 : 2) void k_verify_walk(VerifyArgs a, uint32_t known, bool last) {
+  extern __shared__ double memory[];
+  __shared__ double sum_s[kWalkThreads / 64];
+  __shared__ uint32_t arrived_s;
+  const uint32_t tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
+  const uint32_t piece = REST ? blockIdx.x % a.n_pieces : 0, which = REST ? blockIdx.x / a.n_pieces : blockIdx.x;
+  Walk w(a, which, memory);
+  if (REST && piece && !w.drawn) return;
+  if (!w.n) {
+    if (tid == 0 && last && !piece) a.kept[which] = 0, a.next[which] = BCH_NO_TOKEN;
+    return;
+  }
+  w.load(a.chances && last && !piece);
+  if (REST) {
+    const bool open = !w.down([&](uint32_t round) { return round < known ? w.total_of_pieces(round) : -1.0; });
+    if (open) {
+      float x[kPiece / kWalkThreads];
+      w.piece_of(piece).load<kWalkThreads>(w.heat, x, tid);
+      float sum = 0.f;
+#pragma unroll
+      for (uint32_t j = 0; j < kPiece / kWalkThreads; j++) sum += x[j];
+      const double by_wave = wave_sum_f64((double)sum);
+      if (lane == 0) sum_s[wave] = by_wave;
+      __syncthreads();
+      if (tid == 0) {
+        coherent_store(w.rest(known) + piece, (sum_s[0] + sum_s[1]) + (sum_s[2] + sum_s[3]));
+        if (last) {
+          // The piece is complete before it is counted.
+          __atomic_signal_fence(__ATOMIC_SEQ_CST);
+          __builtin_amdgcn_s_waitcnt(0);
+          __atomic_signal_fence(__ATOMIC_SEQ_CST);
+          arrived_s = __hip_atomic_fetch_add(a.arrived + which, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+      }
+      if (!last) return;
+      __syncthreads();
+      if (arrived_s != a.n_pieces - 1) return;
+    } else if (!last || piece) {
+      return;
+    }
+  }
+  uint32_t latest = 0;  // the round whose pieces are those of the last c
+  w.down([&](uint32_t round) {
+    latest = min(round, a.rounds);
+    if (round >= a.rounds) {  // further rejections: a wave sums every fourth piece
+      __syncthreads();
+      for (uint32_t i = wave; i < a.n_pieces; i += kWalkThreads / 64) {
+        const double sum = w.piece_by_wave(i);
+        if (lane == 0) coherent_store(w.rest(latest) + i, sum);
+      }
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+    }
+    return w.total_of_pieces(latest);
+  });
+  const uint32_t next = w.next(latest);
   __syncthreads();  // (the path is thread 0's)
   for (uint32_t i = tid; i < w.n; i += kWalkThreads) a.path[w.row0 + i] = w.m.path[i];
   if (tid == 0) {
-    a.kept[blockIdx.x] = w.kept;
-    a.next[blockIdx.x] = next;
+    a.kept[which] = w.kept;
+    a.next[which] = next;
     if (a.chances) a.chances[w.row0] = next == BCH_NO_TOKEN ? 0.f : (float)w.chance(w.t, next);
   }
 }
@@ -519,7 +552,7 @@ extern "C" int bch_verify_drafts(bch_ctx *ctx, const bch_kv_plan *plan, uint32_t
   a.n_vocab = n_vocab;
   a.n_pieces = div_ceil(n_vocab, kPiece);
   a.distinct = drafts->distinct != 0;
-  if ((uint64_t)a.n_rows * a.n_pieces >= 1u << 23) return fail(BCH_ERR_ARGUMENT, "verify_drafts: too many logits");
+  if ((uint64_t)std::max(a.n_rows, n_seqs) * a.n_pieces >= 1u << 23) return fail(BCH_ERR_ARGUMENT, "verify_drafts: too many logits");
   const uint64_t rows = a.n_rows, bytes = rows * n_vocab * 4;
   BCH_TRY(view_ptr(ctx, "verify_drafts", drafts->logits, bytes, &a.logits));
   if (drafts->draft.buffer) BCH_TRY(view_ptr(ctx, "verify_drafts", drafts->draft, bytes, &a.draft));
@@ -555,9 +588,10 @@ extern "C" int bch_verify_drafts(bch_ctx *ctx, const bch_kv_plan *plan, uint32_t
   a.rounds = !a.draft || a.most < 2 ? 0 : plan->d_nodes ? std::min(kRounds, a.most - 1) : 1;
   const uint64_t pieces = rows * a.n_pieces * sizeof(VerifyPiece), rest = (uint64_t)n_seqs * a.n_pieces * 8;
   void *scratch;
-  BCH_TRY(ctx_scratch(ctx, pieces + (a.rounds + 1) * rest + 16, &scratch));
+  BCH_TRY(ctx_scratch(ctx, pieces + (a.rounds + 1) * rest + n_seqs * 4ull + 16, &scratch));
   a.pieces = static_cast<VerifyPiece *>(scratch);
   a.rest = reinterpret_cast<double *>(static_cast<char *>(scratch) + pieces);
+  a.arrived = reinterpret_cast<uint32_t *>(static_cast<char *>(scratch) + pieces + (a.rounds + 1) * rest);
   return launch(ctx, {"verify_drafts", a.n_rows, n_vocab, 0}, [&](hipStream_t st) {
     if (!n_seqs) return;
     kv_plan_use(ctx, plan);
@@ -570,7 +604,9 @@ extern "C" int bch_verify_drafts(bch_ctx *ctx, const bch_kv_plan *plan, uint32_t
       else
         k_verify_rows<false><<<a.n_rows * a.n_pieces, kRowThreads, 0, st>>>(a);
     }
-    for (uint32_t i = 0; i < a.rounds; i++) k_verify_rest<<<n_seqs * a.n_pieces, kRowThreads, memory, st>>>(a, i);
-    k_verify_walk<<<n_seqs, kWalkThreads, memory, st>>>(a);
+    if (!a.rounds)
+      k_verify_walk<false><<<n_seqs, kWalkThreads, memory, st>>>(a, 0, true);
+    for (uint32_t i = 0; i < a.rounds; i++)
+      k_verify_walk<true><<<n_seqs * a.n_pieces, kWalkThreads, memory, st>>>(a, i, i + 1 == a.rounds);
   });
 }
