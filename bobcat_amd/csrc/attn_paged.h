@@ -32,9 +32,9 @@
 // whatever the scales, and p needs no bound of its own (scales lie in 2^-40 ..
 // 2^60).  m moves only when p·b could leave its range, so most steps rescale
 // nothing.
-// A plan with trees has kernels of its own (attn_tree.hip): TREE takes what a
-// token sees from the plan's masks, a word for 32 keys, in the steps with new
-// tokens' keys; the steps of the past are the same.
+// A plan with trees has narrow tiles of its own (attn_tree.hip) and the wide ones
+// with TREE, which takes what a token sees from the plan's masks, a word for 32
+// keys, in the steps with new tokens' keys; the steps of the past are the same.
 #pragma once
 #include <cmath>
 
@@ -158,10 +158,10 @@ constexpr uint32_t chunk_groups(uint32_t format, uint32_t hd) {
 // ROWS 8: the high parts of the queries and probabilities are the operands'
 // columns 0..7, the low parts columns 8..15, so one MFMA does both and the
 // halves of O are added once at the end.  ROWS 16: two MFMAs each.
-template <uint32_t FORMAT, uint32_t HD, uint32_t ROWS, bool TREE>
+template <uint32_t FORMAT, uint32_t HD, uint32_t ROWS>
 __global__ __launch_bounds__(256, token_groups(FORMAT, HD)) void k_attn_tokens(
     KvGeometry g, const KvAttnItem *__restrict__ items, const uint32_t *__restrict__ starts, const float *__restrict__ q,
-    uint32_t q_stride, AttnOut to, uint32_t group, float c2, AttnTrees trees) {
+    uint32_t q_stride, AttnOut to, uint32_t group, float c2) {
   constexpr bool PACK = ROWS == 8, QUANT = FORMAT != BCH_KV_F16;
   constexpr uint32_t SIZE = kv_elem_bytes(FORMAT), BYTES = kv_block_bytes(FORMAT, HD), PART = kKvBlock * HD * SIZE;
   constexpr uint32_t NL = PART / 1024;  // KB of a block's keys, and of its values
@@ -178,15 +178,6 @@ __global__ __launch_bounds__(256, token_groups(FORMAT, HD)) void k_attn_tokens(
     const uint32_t pos0 = it.past + it.first / group;                             // of the tile's first row
     const uint32_t n_keys = it.past + (it.first + it.rows - 1) / group + 1;       // of its last
     const uint32_t last = (n_keys - 1) / kKvBlock;
-    // Keys that every row of the tile sees, and where the row's mask has key 0.
-    int whole = pos0 + 1;
-    bool tree = false;
-    const uint32_t *mask = nullptr;
-    if constexpr (TREE) {
-      tree = trees.nodes[it.row].mask != kKvNone;
-      whole = tree ? it.past : whole;
-      mask = trees.masks + (tree ? (int64_t)trees.nodes[it.row + token].mask - it.past / 32 : 0);
-    }
 
     struct Raw {
       au4_t x[2][NL];
@@ -260,15 +251,6 @@ __global__ __launch_bounds__(256, token_groups(FORMAT, HD)) void k_attn_tokens(
 
     for (; step < it.hi; step += 4) {
       const uint32_t next = min(step + 4, it.hi - 1);
-      const bool masked = (int)(32 * step + 31) >= whole;
-      uint32_t word = 0;  // the step's keys that the row sees
-      if constexpr (TREE) {
-        if (masked) word = tree ? mask[step] : keys_to((int)(pos - 32 * step));
-      }
-      auto sees = [&](uint32_t key) {  // of the step
-        if constexpr (TREE) return (word >> key & 1) != 0;
-        return 32 * step + key <= pos;
-      };
       // Scores of the tile's 2 x 16 keys: this lane's are 16t + 4·quad + i.
       float u[2][4];
 #pragma unroll
@@ -299,12 +281,13 @@ __global__ __launch_bounds__(256, token_groups(FORMAT, HD)) void k_attn_tokens(
 #pragma unroll
         for (int t = 0; t < 2; t++) vs[t][0] = vr.s[t].x, vs[t][1] = vr.s[t].y, vs[t][2] = vr.s[t].z, vs[t][3] = vr.s[t].w;
       }
+      const bool masked = 32 * step + 31 > pos0;
       if (masked) {
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            const bool seen = sees(16 * t + 4 * quad + i);
+            const bool seen = 32 * step + 16 * t + 4 * quad + i <= pos;
             u[t][i] = seen ? u[t][i] : -INFINITY;
             if constexpr (QUANT) vs[t][i] = seen ? vs[t][i] : 0.f;
           }
@@ -400,7 +383,7 @@ __global__ __launch_bounds__(256, token_groups(FORMAT, HD)) void k_attn_tokens(
               ah8_t seen, bad;
 #pragma unroll
               for (int j = 0; j < 8; j++) {
-                seen[j] = (_Float16)(sees(16 * (j / 4) + 4 * quad + j % 4) ? 1.f : 0.f);
+                seen[j] = (_Float16)(32 * step + 16 * (j / 4) + 4 * quad + j % 4 <= pos ? 1.f : 0.f);
                 bad[j] = (_Float16)(not_finite(a[j]) ? 1.f : 0.f);
                 a[j] = not_finite(a[j]) ? (_Float16)0.f : a[j];
               }
@@ -822,7 +805,8 @@ __global__ __launch_bounds__(256, chunk_groups(FORMAT, HD)) void k_attn_chunk(
   }
 }
 
-// The launches of a plan's tiles (not the join).
+// An attention call's operands, and attn_tree.hip's launches for a plan with trees
+// (all but the join): its tiles16 are tiles of up to tree_tile_rows rows.
 struct AttnCall {
   hipStream_t stream;
   const bch_kv_plan *plan;
@@ -832,28 +816,8 @@ struct AttnCall {
   AttnOut to;
   float c2;
 };
-
-template <bool TREE>
-void launch_tiles(const AttnCall &a) {
-  const bch_kv_plan *plan = a.plan;
-  const uint32_t n_kv = plan->shape.n_kv_heads;
-  const AttnTrees trees{plan->d_nodes, plan->d_masks};
-  kv_dispatch(plan->shape.format, plan->shape.head_dim, [&](auto format, auto hd) {
-    constexpr uint32_t F = decltype(format)::value, HD = decltype(hd)::value;
-    const bch_kv_plan::Work &c = plan->chunks, &t16 = plan->tiles16, &t8 = plan->tiles8;
-    if (c.groups)
-      k_attn_chunk<F, HD, TREE><<<c.groups * n_kv, 256, 0, a.stream>>>(a.geo, c.items, c.starts, a.q, a.q_stride, a.to,
-                                                                        a.group, a.c2, trees);
-    if (t16.groups)
-      k_attn_tokens<F, HD, 16, TREE><<<t16.groups * n_kv, 256, 0, a.stream>>>(a.geo, t16.items, t16.starts, a.q, a.q_stride,
-                                                                               a.to, a.group, a.c2, trees);
-    if (t8.groups)
-      k_attn_tokens<F, HD, 8, TREE><<<t8.groups * n_kv, 256, 0, a.stream>>>(a.geo, t8.items, t8.starts, a.q, a.q_stride,
-                                                                             a.to, a.group, a.c2, trees);
-  });
-}
-
-// attn_tree.hip
 void launch_tree_tiles(const AttnCall &a);
+uint32_t tree_tile_rows(uint32_t format, uint32_t hd);
+uint32_t tree_tile_groups(uint32_t hd);
 
 }  // namespace bch

@@ -242,8 +242,41 @@ static void deal(KvSchedule &w, KvWork &work, const std::vector<Tile> &tiles, ui
   if (work.starts.back() != work.items.size()) next();
 }
 
+// Which tiles a batch with trees takes: wide ones, or narrow ones of `blocks` times 16
+// rows.  Narrow tiles cost about the same for every block and step of 32 keys once
+// there is work for all waves; a wide one as much as 6.3 blocks in the 8-bit formats,
+// where a narrow tile widens the keys for itself, and 5 in f16, or 2.5 where the
+// keys are more than the last cache holds and the narrow tiles bring them from memory one after
+// the other.  (32 sequences of up to 6,000 keys, eight KV heads of 128, int8, up to 64, 128
+// and 192 rows: 97, 164, 199 us narrow and 141, 166, 213 wide; f16 183, 346, 476 and 131, 173,
+// 251.)  Below 16 steps of a block for each wave the time is latency, and tiles of one
+// block share it among more waves (one sequence of 600 keys and 32 rows, heads of 64: 8.2
+// us, in tiles of two 11.3, wide 20.6; twelve of up to 2,500 keys and 96 rows 21, 24 and 36);
+// three beat two only where there is much more (12 of 256 rows: 52 us and 45; 32 of 96 rows
+// and 6,000 keys 73 and 75).
+struct TreeTiles {
+  bool wide;
+  uint32_t blocks;
+};
+static TreeTiles tree_tiles(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t n_kv, uint32_t format,
+                            uint32_t head_dim, uint32_t n_cus) {
+  uint64_t block_steps = 0, wide_steps = 0, keys = 0;
+  for (const KvSeq &q : seqs) {
+    const uint64_t rows = (uint64_t)q.n_new * group, steps = (q.past + q.n_new + 31) / 32;
+    block_steps += (rows + 15) / 16 * steps;
+    wide_steps += (rows + kChunkRows - 1) / kChunkRows * steps;
+    keys += q.past + q.n_new;
+  }
+  const uint64_t waves = 4ull * n_cus * tree_tile_groups(head_dim), work = block_steps * n_kv;
+  const uint64_t bytes = keys * n_kv * kv_block_bytes(format, head_dim) / kKvBlock;
+  if (work <= 16 * waves) return {false, 1};
+  const double ratio = format != BCH_KV_F16 ? 6.3 : bytes <= (128ull << 20) ? 5.0 : 2.5;
+  return {ratio * wide_steps < block_steps,
+          std::min(work <= 32 * waves ? 2u : 3u, tree_tile_rows(format, head_dim) / 16)};
+}
+
 KvSchedule kv_schedule(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t n_kv, uint32_t format, uint32_t head_dim,
-                       uint32_t n_cus, uint64_t partial_floats) {
+                       uint32_t n_cus, uint64_t partial_floats, bool trees) {
   KvSchedule w;
   const uint64_t records = std::min<uint64_t>(partial_floats / (head_dim + 4), 0xfffffffeu);
   if (!n_cus) n_cus = 256;
@@ -264,17 +297,23 @@ KvSchedule kv_schedule(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t 
     large |= rows > 96;
     if (rows > 16 && rows <= kChunkRows) narrow_work += (rows + 15) / 16 * ((q.past + q.n_new + 31) / 32) * n_kv * head_dim;
   }
-  const uint32_t few_rows = wide || (large && narrow_work > kSmallBatch) ? 32 : kChunkRows;
+  const TreeTiles tree = trees ? tree_tiles(seqs, group, n_kv, format, head_dim, n_cus) : TreeTiles{};
+  // (Beside trees in wide tiles what one block holds stays narrow, beside others a prompt is wide.)
+  const uint32_t few_rows = trees ? (tree.wide ? 16 : 4 * kChunkRows)
+                                  : wide || (large && narrow_work > kSmallBatch) ? 32 : kChunkRows;
   std::vector<Tile> narrow, tokens, chunks;
   uint32_t longest = 0;
   uint64_t narrow_steps = 0, token_steps = 0;
   for (const KvSeq &q : seqs) {
     const uint32_t rows = q.n_new * group;
     const bool few = rows <= few_rows;
-    for (uint32_t first = 0; first < rows; first += few ? 16 : kChunkRows) {
-      const uint32_t n = std::min(few ? 16 : kChunkRows, rows - first), keys = q.past + (first + n - 1) / group + 1;
+    // (A tree's in equal tiles of whole blocks.)
+    const uint32_t most = trees ? 16 * tree.blocks : 16, tiles = (rows + most - 1) / most;
+    const uint32_t narrow_rows = !trees || !tiles ? 16 : ((rows + 15) / 16 + tiles - 1) / tiles * 16;
+    for (uint32_t first = 0; first < rows; first += few ? narrow_rows : kChunkRows) {
+      const uint32_t n = std::min(few ? narrow_rows : kChunkRows, rows - first), keys = q.past + (first + n - 1) / group + 1;
       const Tile t{{q.table, q.past, q.row, first, n, 0, 0, ~0u}, (keys + 31) / 32};
-      (!few ? chunks : n <= 8 ? narrow : tokens).push_back(t);
+      (!few ? chunks : n <= 8 && !trees ? narrow : tokens).push_back(t);
       if (few) {
         longest = std::max(longest, t.steps);
         (n <= 8 ? narrow_steps : token_steps) += t.steps;
@@ -296,7 +335,8 @@ KvSchedule kv_schedule(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t 
   // sequences of 4,000 int8 keys, two KV heads, 29.8 and 27.9; of eight, eight KV
   // heads, 24.4 and 22.2, in e4m3 16.2 and 17.9; of one with 32,000 keys 29.4 and
   // 30.6.)
-  const uint64_t few_groups = (uint64_t)n_cus * (head_dim == 256 ? 1 : token_groups(format, head_dim)) / n_kv;
+  const uint32_t at_once = trees ? tree_tile_groups(head_dim) : head_dim == 256 ? 1 : token_groups(format, head_dim);
+  const uint64_t few_groups = (uint64_t)n_cus * at_once / n_kv;
   deal(w, w.tiles8, narrow, few_groups, 8, longest <= unsplit, 4, n_kv, 1, records);
   deal(w, w.tiles16, tokens, few_groups, 8, longest <= unsplit, 4, n_kv, 1, records);
   // Where a workgroup has one item, the order is free.  (Heads of 256, 12 sequences
@@ -346,19 +386,27 @@ extern "C" int bch_attention_paged(bch_ctx *ctx, const bch_kv_plan *plan, bch_vi
     const AttnOut to{op, out_stride, ctx->attn_partials};
     const AttnCall call{st, plan, plan->geometry(cp), qp, q_stride, group, to,
                         (float)(1.44269504088896340736 / std::sqrt((double)s.head_dim))};
-    if (plan->d_nodes)
-      launch_tree_tiles(call);
-    else
-      launch_tiles<false>(call);
-    if (plan->n_join)
-      kv_dispatch(s.format, s.head_dim, [&](auto, auto hd) {
-        constexpr uint32_t HD = decltype(hd)::value;
+    if (plan->d_nodes) launch_tree_tiles(call);
+    kv_dispatch(s.format, s.head_dim, [&](auto format, auto hd) {
+      constexpr uint32_t F = decltype(format)::value, HD = decltype(hd)::value;
+      const bch_kv_plan::Work &c = plan->chunks, &t16 = plan->tiles16, &t8 = plan->tiles8;
+      if (!plan->d_nodes) {
+        if (c.groups)
+          k_attn_chunk<F, HD, false><<<c.groups * n_kv, 256, 0, st>>>(call.geo, c.items, c.starts, qp, q_stride, to, group,
+                                                                      call.c2, {});
+        if (t16.groups)
+          k_attn_tokens<F, HD, 16><<<t16.groups * n_kv, 256, 0, st>>>(call.geo, t16.items, t16.starts, qp, q_stride, to, group, call.c2);
+        if (t8.groups)
+          k_attn_tokens<F, HD, 8><<<t8.groups * n_kv, 256, 0, st>>>(call.geo, t8.items, t8.starts, qp, q_stride, to, group, call.c2);
+      }
+      if (plan->n_join) {
         // Up to eight records each in one round of loads.
         constexpr uint32_t kGroups = 1024 / HD;
         uint32_t parts = 1;
         while (parts < kGroups && parts * 8 < plan->join_splits) parts *= 2;
         k_attn_join<HD><<<dim3(plan->n_join, n_kv, div_ceil(plan->join_rows * parts, kGroups)), 256, 0, st>>>(
             plan->d_join, n_kv, group, parts, to);
-      });
+      }
+    });
   });
 }

@@ -112,9 +112,9 @@ struct KvSchedule {
   uint64_t records = 0;
 };
 // attn_paged.hip: the attention's work of a batch, with no more partial
-// results than partial_floats hold.
+// results than partial_floats hold; with `trees` for the kernels of attn_tree.hip.
 KvSchedule kv_schedule(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t n_kv, uint32_t format, uint32_t head_dim,
-                       uint32_t n_cus, uint64_t partial_floats);
+                       uint32_t n_cus, uint64_t partial_floats, bool trees);
 
 struct KvGeometry {
   uint8_t *cache;

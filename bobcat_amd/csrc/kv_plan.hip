@@ -203,8 +203,6 @@ static int plan_set(bch_kv_plan *plan, uint32_t n_seqs, const uint32_t *n_past, 
     row += n_new[i];
     table += (end + plan->shape.page_size - 1) / plan->shape.page_size;
   }
-  const KvSchedule work = kv_schedule(seqs, plan->n_heads / plan->shape.n_kv_heads, plan->shape.n_kv_heads,
-                                      plan->shape.format, plan->shape.head_dim, plan->ctx->n_cus, plan->ctx->attn_partials ? kAttnPartialFloats : 0);
   // (Parents that make chains of all sequences are no trees.)
   std::vector<KvNode> nodes;
   std::vector<uint32_t> masks;
@@ -215,6 +213,8 @@ static int plan_set(bch_kv_plan *plan, uint32_t n_seqs, const uint32_t *n_past, 
     nodes.resize(row);
     lay_trees(seqs, parents, nodes, masks, rooted);
   }
+  const KvSchedule work = kv_schedule(seqs, plan->n_heads / plan->shape.n_kv_heads, plan->shape.n_kv_heads,
+                                      plan->shape.format, plan->shape.head_dim, plan->ctx->n_cus, plan->ctx->attn_partials ? kAttnPartialFloats : 0, trees);
   Layout all;
   const uint64_t at_seqs = all.add(seqs.data(), seqs.size());
   const uint64_t at_nodes = all.add(nodes.data(), nodes.size());
