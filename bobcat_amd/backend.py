@@ -256,10 +256,16 @@ class RopeRows:
     norm: NormSpec | None = None
 
     def c(self, head_dim: int) -> RopeRowsC:
-        norm = _View() if self.norm is None else _view(self.norm.weight)
-        return RopeRowsC(_view(self.src), _view(self.dst), norm, self.n_heads,
-                         head_dim if self.head_stride is None else self.head_stride, self.src_stride, self.dst_stride,
-                         0.0 if self.norm is None else self.norm.eps)
+        """What the library takes, made once (for as long as the buffers live)."""
+        norm = self.norm
+        of = (self.src.buffer.handle, self.dst.buffer.handle, norm and norm.weight.buffer.handle, head_dim)
+        made = self.__dict__.get("_made")
+        if made is None or made[0] != of:
+            rows = RopeRowsC(_view(self.src), _view(self.dst), _View() if norm is None else _view(norm.weight), self.n_heads,
+                             head_dim if self.head_stride is None else self.head_stride, self.src_stride, self.dst_stride,
+                             0.0 if norm is None else norm.eps)
+            made = self.__dict__["_made"] = (of, rows)
+        return made[1]
 
 
 class Hip:

@@ -29,12 +29,17 @@ struct bch_ctx {
   // the host knows that all work up to it has run.
   uint64_t begun = 0;
   uint64_t finished = 0;
-  hipEvent_t begin_event = nullptr;  // recorded at bch_begin
+  hipEvent_t begin_event = nullptr;  // marks the open recording's start
+  // Where that is the last pending one's end, which the stream had not reached at
+  // bch_begin, the event is that one's (each takes the stream 4 us or so).
+  bool begin_shared = false;
+  bool discarded = false;  // a recording was, since the last commit: its work lies between
   struct Pending {
     uint64_t ticket;
     uint64_t recording;
     hipEvent_t begin;
     hipEvent_t end;
+    bool begin_shared;  // the one's before it, as long as that is pending
   };
   std::vector<Pending> pending;
   bool profiling = false;

@@ -125,10 +125,10 @@ void bch_close(bch_ctx *ctx) {
   if (!ctx) return;
   hipStreamSynchronize(ctx->stream);
   for (auto &p : ctx->pending) {
-    hipEventDestroy(p.begin);
+    if (!p.begin_shared) hipEventDestroy(p.begin);
     hipEventDestroy(p.end);
   }
-  if (ctx->begin_event) hipEventDestroy(ctx->begin_event);
+  if (ctx->begin_event && !ctx->begin_shared) hipEventDestroy(ctx->begin_event);
   if (ctx->counters) hipFree(ctx->counters);
   if (ctx->scratch) hipFree(ctx->scratch);
   if (ctx->attn_partials) hipFree(ctx->attn_partials);
@@ -217,8 +217,20 @@ int bch_read(bch_ctx *ctx, bch_view view, void *out, uint64_t bytes) {
 
 int bch_begin(bch_ctx *ctx) {
   if (ctx->recording) return fail(BCH_ERR_ALREADY_RECORDING, "a recording is already open");
-  if (!ctx->begin_event) hipEventCreate(&ctx->begin_event);
-  hipEventRecord(ctx->begin_event, ctx->stream);
+  // Behind a recording that is still running this one starts where that one ends.
+  bool behind = false;
+  if (!ctx->pending.empty() && !ctx->discarded) {
+    behind = hipEventQuery(ctx->pending.back().end) == hipErrorNotReady;
+    if (behind) (void)hipGetLastError();
+  }
+  if (behind) {
+    if (ctx->begin_event && !ctx->begin_shared) hipEventDestroy(ctx->begin_event);
+    ctx->begin_event = ctx->pending.back().end;
+  } else {
+    if (!ctx->begin_event || ctx->begin_shared) hipEventCreate(&ctx->begin_event);
+    hipEventRecord(ctx->begin_event, ctx->stream);
+  }
+  ctx->begin_shared = behind;
   ctx->recording = true;
   ctx->begun++;
   return BCH_OK;
@@ -226,7 +238,10 @@ int bch_begin(bch_ctx *ctx) {
 
 // Metal::discard (backend.rs:1249): work already handed to the stream still
 // runs; the recording closes without a ticket.
-void bch_discard(bch_ctx *ctx) { ctx->recording = false; }
+void bch_discard(bch_ctx *ctx) {
+  ctx->discarded |= ctx->recording;
+  ctx->recording = false;
+}
 
 void bch_barrier(bch_ctx *) {}
 
@@ -235,11 +250,11 @@ int bch_commit(bch_ctx *ctx, uint64_t *ticket) {
   bch_ctx::Pending p;
   p.ticket = ++ctx->committed;
   p.recording = ctx->begun;
-  hipEventCreate(&p.begin);
   hipEventCreate(&p.end);
-  // The event recorded at bch_begin marks this ticket's start; the fresh
-  // event takes its place for the next recording.
-  std::swap(p.begin, ctx->begin_event);
+  // The event of bch_begin marks this ticket's start.
+  p.begin = std::exchange(ctx->begin_event, nullptr);
+  p.begin_shared = std::exchange(ctx->begin_shared, false);
+  ctx->discarded = false;
   hipEventRecord(p.end, ctx->stream);
   ctx->pending.push_back(p);
   ctx->recording = false;
@@ -258,8 +273,14 @@ int bch_wait(bch_ctx *ctx, uint64_t ticket, double *gpu_seconds) {
       rc = fail(BCH_ERR_EXECUTION, "the GPU failed to run the work: %s", hipGetErrorString(e));
     float ms = 0.f;
     if (e == hipSuccess && hipEventElapsedTime(&ms, p.begin, p.end) == hipSuccess) total += ms * 1e-3;
-    hipEventDestroy(p.begin);
-    hipEventDestroy(p.end);
+    if (!p.begin_shared) hipEventDestroy(p.begin);
+    // The recording behind it may have its end for a start.
+    if (!ctx->pending.empty() && ctx->pending.front().begin == p.end)
+      ctx->pending.front().begin_shared = false;
+    else if (ctx->begin_shared && ctx->begin_event == p.end)
+      ctx->begin_shared = false;
+    else
+      hipEventDestroy(p.end);
     if (p.ticket > ctx->waited) ctx->waited = p.ticket;
     if (p.recording > ctx->finished) ctx->finished = p.recording;
   }
