@@ -129,6 +129,7 @@ def test_refusals(hip):
     refused("Argument", layers=2, apart=size - 16)
     refused("Argument", layers=2, apart=size + 8)
     refused("Argument", layers=2, apart=(1 << 64) - 16)
+    refused("Argument", layers=129)
     refused("Argument", at=8)
     refused("OutOfBounds", kept=kb.at(4))
     refused("OutOfBounds", path=pb.at(4))
