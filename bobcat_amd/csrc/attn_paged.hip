@@ -267,7 +267,7 @@ static TreeTiles tree_tiles(const std::vector<KvSeq> &seqs, uint32_t group, uint
     wide_steps += (rows + kChunkRows - 1) / kChunkRows * steps;
     keys += q.past + q.n_new;
   }
-  const uint64_t waves = 4ull * n_cus * tree_tile_groups(head_dim), work = block_steps * n_kv;
+  const uint64_t waves = 4ull * n_cus * tree_tile_groups(format, head_dim), work = block_steps * n_kv;
   const uint64_t bytes = keys * n_kv * kv_block_bytes(format, head_dim) / kKvBlock;
   if (work <= 16 * waves) return {false, 1};
   const double ratio = format != BCH_KV_F16 ? 6.3 : bytes <= (128ull << 20) ? 5.0 : 2.5;
@@ -335,7 +335,7 @@ KvSchedule kv_schedule(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t 
   // sequences of 4,000 int8 keys, two KV heads, 29.8 and 27.9; of eight, eight KV
   // heads, 24.4 and 22.2, in e4m3 16.2 and 17.9; of one with 32,000 keys 29.4 and
   // 30.6.)
-  const uint32_t at_once = trees ? tree_tile_groups(head_dim) : head_dim == 256 ? 1 : token_groups(format, head_dim);
+  const uint32_t at_once = trees ? tree_tile_groups(format, head_dim) : head_dim == 256 ? 1 : token_groups(format, head_dim);
   const uint64_t few_groups = (uint64_t)n_cus * at_once / n_kv;
   deal(w, w.tiles8, narrow, few_groups, 8, longest <= unsplit, 4, n_kv, 1, records);
   deal(w, w.tiles16, tokens, few_groups, 8, longest <= unsplit, 4, n_kv, 1, records);

@@ -22,13 +22,13 @@ namespace bch {
 constexpr uint32_t tree_blocks(uint32_t format, uint32_t hd) {
   return (hd == 64 ? 3 : hd == 128 ? 2 : 1) - (hd < 256 && format == BCH_KV_F16);
 }
-constexpr uint32_t tree_groups(uint32_t hd) { return hd == 256 ? 1 : 2; }
+constexpr uint32_t tree_groups(uint32_t format, uint32_t hd) { return hd == 256 && format == BCH_KV_F16 ? 1 : 2; }
 
 uint32_t tree_tile_rows(uint32_t format, uint32_t hd) { return 16 * tree_blocks(format, hd); }
-uint32_t tree_tile_groups(uint32_t hd) { return tree_groups(hd); }
+uint32_t tree_tile_groups(uint32_t format, uint32_t hd) { return tree_groups(format, hd); }
 
 template <uint32_t FORMAT, uint32_t HD>
-__global__ __launch_bounds__(256, tree_groups(HD)) void k_attn_tree(
+__global__ __launch_bounds__(256, tree_groups(FORMAT, HD)) void k_attn_tree(
     KvGeometry g, const KvAttnItem *__restrict__ items, const uint32_t *__restrict__ starts, const float *__restrict__ q,
     uint32_t q_stride, AttnOut to, uint32_t group, float c2, AttnTrees trees) {
   constexpr bool QUANT = FORMAT != BCH_KV_F16;

@@ -42,6 +42,17 @@ __device__ __forceinline__ float2 cos_sin(uint64_t t) {
   return {(quarter + 1) & 2 ? -a : a, quarter & 2 ? -b : b};
 }
 
+// Four floats, with STREAM past the caches.
+template <bool STREAM>
+__device__ __forceinline__ void put4(float *p, const float *z) {
+  typedef float f4 __attribute__((ext_vector_type(4)));
+  const f4 v = {z[0], z[1], z[2], z[3]};
+  if constexpr (STREAM)
+    __builtin_nontemporal_store(v, reinterpret_cast<f4 *>(p));
+  else
+    *reinterpret_cast<f4 *>(p) = v;
+}
+
 struct RopeSide {
   const float *from;
   float *to;
@@ -63,7 +74,7 @@ struct RopeArgs {
 // round's row of a lane has the same token, whose angles the lane keeps.  QUADS: a
 // lane has two pieces of four elements, and pairs 4·lane .. + 3 where those turn;
 // else up to 8 pairs and single elements, one by one, for any n_rot.
-template <uint32_t HD, uint32_t LAYOUT, bool QUADS>
+template <uint32_t HD, uint32_t LAYOUT, bool QUADS, bool STREAM>
 __global__ __launch_bounds__(kRopeThreads) void k_rope(RopeArgs a) {
   constexpr uint32_t LANES = HD / 8, ROWS = kRopeThreads / LANES;
   const KvStoreItem it = a.items[blockIdx.x];
@@ -148,8 +159,8 @@ __global__ __launch_bounds__(kRopeThreads) void k_rope(RopeArgs a) {
         z[p] = turns ? fmaf(x[p], co[i], -x[q] * si[i]) : x[p];
         z[q] = turns ? fmaf(x[p], si[i], x[q] * co[i]) : x[q];
       }
-      *reinterpret_cast<float4 *>(to + q0) = float4{z[0], z[1], z[2], z[3]};
-      *reinterpret_cast<float4 *>(to + q1) = float4{z[4], z[5], z[6], z[7]};
+      put4<STREAM>(to + q0, z);
+      put4<STREAM>(to + q1, z + 4);
     } else {
 #pragma unroll
       for (uint32_t i = 0; i < 8; i++) {
@@ -317,19 +328,24 @@ extern "C" int bch_rope_paged(bch_ctx *ctx, const bch_rope *rope, const bch_kv_p
     a.turns = rope->turns;
     a.half = rope->n_rot / 2;
     a.magnitude = rope->magnitude;
+    // Rows that no L2 holds until they are read go past the caches (151 MB of them: 62 us instead of
+    // 71; 4.5 MB are read back from the L2 and take 5 us either way).
+    const bool stream = (uint64_t)plan->n_tokens * heads * hd * 4 > 32u << 20;
     const bool quads = rope->n_rot % (rope->layout == BCH_ROPE_PAIRS ? 4 : 8) == 0;
-    auto go = [&](auto width, auto layout, auto by_quads) {
+    auto go = [&](auto width, auto layout, auto by_quads, auto streams) {
       constexpr uint32_t HD = decltype(width)::value, ROWS = kRopeThreads / (HD / 8);
       const uint32_t most = div_ceil(heads * std::min(kKvBlock, plan->n_tokens), ROWS);
-      const dim3 grid(plan->n_store, std::max(1u, std::min(most, div_ceil(4 * 256, plan->n_store))));
-      k_rope<HD, decltype(layout)::value, decltype(by_quads)::value><<<grid, kRopeThreads, 0, st>>>(a);
+      const dim3 grid(plan->n_store, std::max(1u, std::min(most, div_ceil(8 * 256, plan->n_store))));
+      k_rope<HD, decltype(layout)::value, decltype(by_quads)::value, decltype(streams)::value><<<grid, kRopeThreads, 0, st>>>(a);
     };
     auto with_layout = [&](auto width) {
       auto with_quads = [&](auto layout) {
-        if (quads)
-          go(width, layout, std::true_type{});
+        if (quads && stream)
+          go(width, layout, std::true_type{}, std::true_type{});
+        else if (quads)
+          go(width, layout, std::true_type{}, std::false_type{});
         else
-          go(width, layout, std::false_type{});
+          go(width, layout, std::false_type{}, std::false_type{});
       };
       if (rope->layout == BCH_ROPE_PAIRS)
         with_quads(std::integral_constant<uint32_t, BCH_ROPE_PAIRS>{});

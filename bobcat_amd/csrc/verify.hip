@@ -270,26 +270,36 @@ struct Walk {
     __syncthreads();
   }
 
-  // Down the tree from its first token; total_of(round) is the sum of (p - c·q)+, or below 0 where it is not
-  // known yet: false then.
+  // Down the tree, from its first token or from where it stopped; total_of(round) is the sum of
+  // (p - c·q)+, or below 0 where it is not known yet: false then.
+  uint32_t looked = kKvNone;  // the child whose rejection waits for its sum
+  double left = 1, total = 1;
   template <class Total>
   __device__ bool down(Total &&total_of) {
-    t = 0, kept = 1, round = 0;
     for (;;) {
-      double left = 1, total = 1;
-      c = 0;
-      uint32_t s = m.child[t];
+      uint32_t s = looked;
+      if (s == kKvNone) {
+        c = 0, left = total = 1;
+        s = m.child[t];
+      }
       for (; s != kKvNone; s = m.sibling[s]) {
         const double u = (double)m.u[s], p = m.p[s], q = m.q[s];
-        if (p > 0 && (greedy ? true : drawn ? u * q * total < (p - c * q) * left : u * total < p)) break;
+        if (looked == kKvNone) {
+          if (p > 0 && (greedy ? true : drawn ? u * q * total < (p - c * q) * left : u * total < p)) break;
+          if (drawn) {
+            if (left > 0) c += total / left;
+            if (a.distinct) left -= q;
+          } else if (!greedy) {
+            total -= p;
+          }
+        }
         if (drawn) {
-          if (left > 0) c += total / left;
-          if (a.distinct) left -= q;
-          total = total_of(round);
-          if (total < 0) return false;
+          looked = s;
+          const double sum = total_of(round);
+          if (sum < 0) return false;
+          total = sum;
+          looked = kKvNone;
           round++;
-        } else if (!greedy) {
-          total -= p;
         }
       }
       if (s == kKvNone) return true;
@@ -478,8 +488,13 @@ __global__ __launch_bounds__(kWalkThreads, REST ? 6 : 2) void k_verify_walk(Veri
     return;
   }
   w.load(a.chances && last && !piece);
+  uint32_t latest = 0;  // the round whose pieces are those of the last c
+  bool open = true;
   if (REST) {
-    const bool open = !w.down([&](uint32_t round) { return round < known ? w.total_of_pieces(round) : -1.0; });
+    open = !w.down([&](uint32_t round) {
+      latest = round;
+      return round < known ? w.total_of_pieces(round) : -1.0;
+    });
     if (open) {
       float x[kPiece / kWalkThreads];
       w.piece_of(piece).load<kWalkThreads>(w.heat, x, tid);
@@ -506,8 +521,7 @@ __global__ __launch_bounds__(kWalkThreads, REST ? 6 : 2) void k_verify_walk(Veri
       return;
     }
   }
-  uint32_t latest = 0;  // the round whose pieces are those of the last c
-  w.down([&](uint32_t round) {
+  if (open) w.down([&](uint32_t round) {
     latest = min(round, a.rounds);
     if (round >= a.rounds) {  // further rejections: a wave sums every fourth piece
       __syncthreads();

@@ -193,3 +193,17 @@ def test_refusals(hip):
         hip.rope(4, 1e4, frequencies=[1.0])
     empty = hip.kv_plan("i8", 1, 64, 16, 1, 2)
     refused("Argument", plan_=empty)
+
+
+def test_a_batch_that_no_l2_holds(hip):
+    """More than 32 MiB of rows: they are written past the caches."""
+    rng, hd, heads, kv = np.random.default_rng(8), 256, 30, 2
+    past, new = [1000, 0], [600, 530]
+    q, k = (rng.standard_normal((1130, h, hd)).astype(np.float32) for h in (heads, kv))
+    c = rope_spec(128, 1e6)
+    got = turned(hip, plan_of(hip, past, new, hd, heads, kv), c, (q, k))
+    at = [p + i for p, n in zip(past, new) for i in range(n)]
+    for y, x in zip(got, (q, k)):
+        want, size = rope(x, at, rope_frequencies(c), "halves")
+        assert (np.abs(y - want) / (size * STEP)).max() <= 9
+        assert np.array_equal(y[..., 128:], x[..., 128:])
