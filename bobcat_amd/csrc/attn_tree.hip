@@ -183,36 +183,47 @@ __global__ __launch_bounds__(256, tree_groups(FORMAT, HD)) void k_attn_tree(
         }
         cap = scale_log(cap) - 127.f;
       }
+      // A row's bound on u + log2 b: the largest u with the largest log2 b of the keys, which all rows see;
+      // where they may not, of each key that the row sees.
       bool look = false;
+      float bound[NB];
 #pragma unroll
       for (uint32_t n = 0; n < NB; n++) {
-        if constexpr (masked) {
+        bound[n] = -INFINITY;
 #pragma unroll
-          for (int t = 0; t < 2; t++)
+        for (int t = 0; t < 2; t++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) u[n][t][i] = word[n] >> (16 * t + 4 * quad + i) & 1 ? u[n][t][i] : -INFINITY;
-        }
-        const float top = fmaxf(fmaxf(fmaxf(u[n][0][0], u[n][0][1]), fmaxf(u[n][0][2], u[n][0][3])),
-                                fmaxf(fmaxf(u[n][1][0], u[n][1][1]), fmaxf(u[n][1][2], u[n][1][3])));
-        look |= top + cap > lazy[n];
+          for (int i = 0; i < 4; i++) {
+            if constexpr (masked) {
+              u[n][t][i] = word[n] >> (16 * t + 4 * quad + i) & 1 ? u[n][t][i] : -INFINITY;
+              bound[n] = fmaxf(bound[n], QUANT ? u[n][t][i] + (scale_log(vs[t][i]) - 127.f) : u[n][t][i]);
+            } else {
+              bound[n] = fmaxf(bound[n], u[n][t][i]);
+            }
+          }
+        if constexpr (!masked) bound[n] += cap;
+        look |= bound[n] > lazy[n];
       }
-      // The largest u and the largest log2 b bound their sum; where that is past a
-      // row's limit, key by key.  Rows past kPeak then move, so that the next steps look less often.
+      // Where it is past a row's limit, key by key.  That row then moves from kPeak on, so that the next
+      // steps look less often.  (Other rows stay: what a row does goes by its own keys alone.)
       if (__builtin_amdgcn_ballot_w64(look)) {
 #pragma unroll
         for (uint32_t n = 0; n < NB; n++) {
+          auto of_row = [](float x) {
+            x = fmaxf(x, __shfl_xor(x, 16, 64));
+            return fmaxf(x, __shfl_xor(x, 32, 64));
+          };
           auto highest = [&]() __attribute__((always_inline)) {
             float top = -INFINITY;
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
               for (int i = 0; i < 4; i++) top = fmaxf(top, QUANT ? u[n][t][i] + scale_log(vs[t][i]) : u[n][t][i]);
-            top = QUANT ? top - 127.f : top;
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            return fmaxf(top, __shfl_xor(top, 32, 64));
+            return of_row(QUANT ? top - 127.f : top);
           };
           float top = highest();
-          const bool move = top > fminf(lazy[n], kPeak);  // the same in the four lanes of a row
+          // (The same in the four lanes of a row.)
+          const bool move = of_row(bound[n]) > lazy[n] && top > fminf(lazy[n], kPeak);
           const float d = move ? top - kPeak : 0.f, corr = !move || lazy[n] == kUnset ? 1.f : __builtin_amdgcn_exp2f(-d);
           m[n] += d;
           l[n] *= corr;

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from _drafts import ancestors, as_given, chain, random_tree, tree_attention
-from _paged import Batch, Pool, attention_bound, random_rows
+from _paged import Batch, Pool, attention_bound, dequantise, random_rows
 from bobcat_amd.backend import Hip
 from test_gpu_paged import attend
 
@@ -134,3 +134,96 @@ def test_a_plan_with_trees_becomes_one_without(hip):
     check(hip, pool, batch, 8, q, [chain(9), chain(14)], plan=plan)
     plan.set(batch.past, batch.new, batch.pages, parents=as_given(trees))
     check(hip, pool, batch, 8, q, trees, plan=plan)
+
+
+# --- batches with work for tiles of more blocks, and for wide ones -----------------------
+
+def decoded(pool, page_list, n):
+    """A sequence's first n positions' (k, v) [n, kv, hd] in float64, all at once."""
+    size = 2 if pool.fmt == "f16" else 1
+    raw, part = pool.bytes[page_list], 16 * pool.hd * size  # [page, kv, block, bytes]
+    out = []
+    for i, where in enumerate((pool.key_at, pool.value_at)):
+        bits = np.ascontiguousarray(raw[..., i * part:(i + 1) * part]).view(np.uint16 if size == 2 else np.uint8)[..., where]
+        scale = None if size == 2 else np.ascontiguousarray(raw[..., 2 * part:]).view(np.float32)[..., 16 * i:16 * i + 16]
+        x = dequantise(bits, scale, pool.fmt)  # [page, kv, block, 16, hd]
+        out.append(x.transpose(0, 2, 3, 1, 4).reshape(-1, pool.kv, pool.hd)[:n])
+    return out
+
+
+def large(rng, fmt, hd, kv, heads, seqs, new, past):
+    """A batch of trees (and a chain) with random caches: (batch, pool, queries, trees, past positions)."""
+    trees = [random_tree(rng, int(n), width=4) for n in rng.integers(new // 2, new + 1, seqs - 1)] + [chain(new)]
+    pasts = [past] + [int(n) for n in rng.integers(past // 2, past, seqs - 1)]
+    batch = Batch(rng, [(p, len(t)) for p, t in zip(pasts, trees)], 64)
+    pool = Pool(fmt, kv, hd, 64, batch.n_pages)
+    part = 16 * hd * (2 if fmt == "f16" else 1)
+    if fmt == "f16":
+        values = rng.standard_normal(pool.bytes.size // 2, np.float32).astype(np.float16)
+        pool.bytes[:] = values.view(np.uint8).reshape(pool.bytes.shape)
+    else:
+        pool.bytes[..., :2 * part] = rng.integers(0, 256, pool.bytes[..., :2 * part].shape, np.uint8)
+        if fmt == "f8":
+            pool.bytes[..., :2 * part] &= 0xBF  # (below 2, and no NaN)
+        scales = np.exp(0.4 * rng.standard_normal(pool.bytes[..., 2 * part:].shape[:-1] + (32,))) / (64 if fmt == "i8" else 1)
+        pool.bytes[..., 2 * part:] = np.ascontiguousarray(scales.astype(np.float32)).view(np.uint8)
+    return batch, pool, rng.standard_normal((batch.tokens, heads, hd)).astype(np.float32), trees, pasts
+
+
+@pytest.mark.parametrize("fmt,hd,kv,heads,seqs,new,past", [
+    ("i8", 64, 8, 32, 40, 24, 3000),    # 64 steps for each wave and more: three blocks
+    ("i8", 64, 8, 32, 16, 18, 2500),    # two
+    ("f8", 64, 8, 24, 40, 30, 3000), ("i8", 128, 8, 32, 24, 20, 2500), ("f8", 128, 4, 32, 24, 12, 3500),
+    ("f16", 64, 8, 16, 40, 16, 3500),   # two blocks of an unquantised cache
+    ("f16", 128, 8, 32, 16, 40, 2500),  # wide ones
+    ("i8", 64, 8, 32, 12, 96, 2000), ("f8", 256, 2, 16, 24, 40, 3000), ("f16", 256, 2, 8, 40, 40, 2500)])
+def test_tiles_by_the_batchs_work(hip, fmt, hd, kv, heads, seqs, new, past):
+    print("work", fmt, hd, kv, heads, seqs, new, past, flush=True)
+    rng = np.random.default_rng(hd + new)
+    batch, pool, q, trees, pasts = large(rng, fmt, hd, kv, heads, seqs, new, past)
+    if new % 8:
+        q[::3] *= np.float32(2.0 ** -9)  # queries that get a factor, beside others that do not
+    got, row = attend(hip, pool, batch, heads, q, plan=plan_of(hip, pool, batch, heads, trees)), 0
+    group = heads // kv
+    for s, t in enumerate(trees):
+        n = len(t)
+        if s % 5 == 0 or s == seqs - 1:
+            k, v = decoded(pool, batch.pages[s], pasts[s] + n)
+            seen = np.concatenate([np.ones((n, pasts[s]), bool), ancestors(t)], 1)
+            qs = q[row:row + n].astype(np.float64).reshape(n, kv, group, hd)
+            for h in range(kv):
+                a = qs[:, h].reshape(n * group, hd) @ k[:, h].T / np.sqrt(hd)
+                a = np.where(np.repeat(seen, group, 0), a, -np.inf)
+                p = np.exp(a - a.max(1, keepdims=True))
+                want = ((p / p.sum(1, keepdims=True)) @ v[:, h]).reshape(n, group, hd)
+                mine = got[row:row + n, h * group:(h + 1) * group]
+                bound = attention_bound(q[row:row + n, h * group:(h + 1) * group], k[:, h:h + 1], v[:, h:h + 1])
+                assert np.abs(mine - want).max() <= bound, (s, h)
+        row += n
+
+
+@pytest.mark.parametrize("fmt,hd,kv,heads,seqs,new,past", [
+    ("i8", 64, 8, 32, 40, 24, 3000), ("i8", 128, 8, 32, 24, 20, 2500), ("f16", 64, 8, 16, 40, 16, 3500),
+    ("f16", 128, 8, 32, 16, 40, 2500), ("i8", 64, 8, 32, 12, 96, 2000)])
+def test_rows_that_are_not_finite_in_larger_tiles(hip, fmt, hd, kv, heads, seqs, new, past):
+    rng = np.random.default_rng(new)
+    batch, pool, q, trees, pasts = large(rng, fmt, hd, kv, heads, seqs, new, past)
+    clean = attend(hip, pool, batch, heads, q, plan=plan_of(hip, pool, batch, heads, trees))
+    hit, row = [], 0
+    for s, t in enumerate(trees):
+        n, at = len(t), int(rng.integers(len(t)))
+        k, v = random_rows(rng, kv, hd)
+        (v if s % 2 else k)[:, 5] = np.inf if s % 2 else np.nan
+        pos = pasts[s] + at
+        pool.put(batch.pages[s][pos // 64], pos % 64, k, v)
+        sees = ancestors(t)[:, at]
+        hit += [(row + i, bool(sees[i]), s % 2) for i in range(n)]
+        row += n
+    got = attend(hip, pool, batch, heads, q, plan=plan_of(hip, pool, batch, heads, trees))
+    for i, sees, value in hit:
+        if not sees:
+            assert np.array_equal(got[i], clean[i]), i
+        elif value and fmt == "f16":
+            assert np.isnan(got[i][:, 5]).all() and np.isfinite(np.delete(got[i], 5, 1)).all(), i
+        else:
+            assert np.isnan(got[i]).all(), i
