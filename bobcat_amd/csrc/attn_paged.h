@@ -818,6 +818,6 @@ struct AttnCall {
 };
 void launch_tree_tiles(const AttnCall &a);
 uint32_t tree_tile_rows(uint32_t format, uint32_t hd);
-uint32_t tree_tile_groups(uint32_t format, uint32_t hd);
+uint32_t tree_tile_groups(uint32_t format, uint32_t hd, uint32_t blocks);  // workgroups of a CU
 
 }  // namespace bch

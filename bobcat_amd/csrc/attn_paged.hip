@@ -242,15 +242,15 @@ static void deal(KvSchedule &w, KvWork &work, const std::vector<Tile> &tiles, ui
   if (work.starts.back() != work.items.size()) next();
 }
 
-// Which tiles a batch with trees takes: wide ones, or narrow ones of `blocks` times 16
+// Which tiles a batch with trees takes: wide ones, or narrow ones of up to `blocks` times 16
 // rows.  Narrow tiles cost about the same for every block and step of 32 keys once
 // there is work for all waves; a wide one as much as 6.3 blocks in the 8-bit formats,
-// where a narrow tile widens the keys for itself, and 5 in f16, or 2.5 where the
+// where a narrow tile widens the keys for itself, and 5 in f16, or 3 where the
 // keys are more than the last cache holds and the narrow tiles bring them from memory one after
-// the other.  (32 sequences of up to 6,000 keys, eight KV heads of 128, int8, up to 64, 128
-// and 192 rows: 97, 164, 199 us narrow and 141, 166, 213 wide; f16 183, 346, 476 and 131, 173,
-// 251.)  Below 16 steps of a block for each wave the time is latency, and tiles of one
-// block share it among more waves (one sequence of 600 keys and 32 rows, heads of 64: 8.2
+// the other.  (32 sequences of up to 6,000 keys, eight KV heads of 128, up to 48, 64, 128
+// and 192 rows: int8 82, 106, 177, 213 us narrow and 132, 142, 174, 216 wide; f16 109, 147, 256,
+// 359 and 151, 136, 184, 272.)  Below 16 steps of a block for each wave the time is latency, and tiles of
+// one block share it among more waves (one sequence of 600 keys and 32 rows, heads of 64: 8.2
 // us, in tiles of two 11.3, wide 20.6; twelve of up to 2,500 keys and 96 rows 21, 24 and 36);
 // three beat two only where there is much more (12 of 256 rows: 52 us and 45; 32 of 96 rows
 // and 6,000 keys 73 and 75).
@@ -267,12 +267,12 @@ static TreeTiles tree_tiles(const std::vector<KvSeq> &seqs, uint32_t group, uint
     wide_steps += (rows + kChunkRows - 1) / kChunkRows * steps;
     keys += q.past + q.n_new;
   }
-  const uint64_t waves = 4ull * n_cus * tree_tile_groups(format, head_dim), work = block_steps * n_kv;
+  const uint64_t waves = 4ull * n_cus * tree_tile_groups(format, head_dim, 1), work = block_steps * n_kv;
   const uint64_t bytes = keys * n_kv * kv_block_bytes(format, head_dim) / kKvBlock;
   if (work <= 16 * waves) return {false, 1};
-  const double ratio = format != BCH_KV_F16 ? 6.3 : bytes <= (128ull << 20) ? 5.0 : 2.5;
-  return {ratio * wide_steps < block_steps,
-          std::min(work <= 32 * waves ? 2u : 3u, tree_tile_rows(format, head_dim) / 16)};
+  const double ratio = format != BCH_KV_F16 ? 6.3 : bytes <= (128ull << 20) ? 5.0 : 3.0;
+  if (ratio * wide_steps < block_steps) return {true, 1};
+  return {false, std::min(work <= 32 * waves ? 2u : 3u, tree_tile_rows(format, head_dim) / 16)};
 }
 
 KvSchedule kv_schedule(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t n_kv, uint32_t format, uint32_t head_dim,
@@ -298,6 +298,7 @@ KvSchedule kv_schedule(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t 
     if (rows > 16 && rows <= kChunkRows) narrow_work += (rows + 15) / 16 * ((q.past + q.n_new + 31) / 32) * n_kv * head_dim;
   }
   const TreeTiles tree = trees ? tree_tiles(seqs, group, n_kv, format, head_dim, n_cus) : TreeTiles{};
+  w.tree_blocks = tree.blocks;
   // (Beside trees in wide tiles what one block holds stays narrow, beside others a prompt is wide.)
   const uint32_t few_rows = trees ? (tree.wide ? 16 : 4 * kChunkRows)
                                   : wide || (large && narrow_work > kSmallBatch) ? 32 : kChunkRows;
@@ -335,7 +336,7 @@ KvSchedule kv_schedule(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t 
   // sequences of 4,000 int8 keys, two KV heads, 29.8 and 27.9; of eight, eight KV
   // heads, 24.4 and 22.2, in e4m3 16.2 and 17.9; of one with 32,000 keys 29.4 and
   // 30.6.)
-  const uint32_t at_once = trees ? tree_tile_groups(format, head_dim) : head_dim == 256 ? 1 : token_groups(format, head_dim);
+  const uint32_t at_once = trees ? tree_tile_groups(format, head_dim, tree.blocks) : head_dim == 256 ? 1 : token_groups(format, head_dim);
   const uint64_t few_groups = (uint64_t)n_cus * at_once / n_kv;
   deal(w, w.tiles8, narrow, few_groups, 8, longest <= unsplit, 4, n_kv, 1, records);
   deal(w, w.tiles16, tokens, few_groups, 8, longest <= unsplit, 4, n_kv, 1, records);

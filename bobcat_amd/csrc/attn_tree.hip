@@ -17,18 +17,33 @@
 
 namespace bch {
 
-// Blocks of 16 rows of a tile, and workgroups of a CU: what the registers hold
-// of queries and outputs (2·hd / 4 a block) beside the keys on their way.
+// Blocks of 16 rows of a tile at most, and workgroups of a CU of a kernel for up to `most`: what
+// the registers hold of queries and outputs (2·hd / 4 a block) beside the keys on their way.  16
+// sequences of up to 8,192 positions (the GPU's time, the join's with it), int8, heads of 64 with
+// 96 rows: 62 us, one workgroup a CU 75, four blocks 63; of 128: 90, three blocks 239 (it spills),
+// one block 104; of 256, two KV heads: 70, two blocks 76.  f16, heads of 128, 32 rows of 32
+// sequences of up to 6,000: two blocks with one workgroup a CU 99, one block with two 120;
+// but 12 of up to 2,500, 48 rows, 39 and 30: so there is a kernel for each.  f16, heads of 256, 64 rows,
+// one workgroup a CU 76, two 108 (it spills).
 constexpr uint32_t tree_blocks(uint32_t format, uint32_t hd) {
-  return (hd == 64 ? 3 : hd == 128 ? 2 : 1) - (hd < 256 && format == BCH_KV_F16);
+  return hd == 64 ? (format == BCH_KV_F16 ? 2 : 3) : hd == 128 ? 2 : 1;
 }
-constexpr uint32_t tree_groups(uint32_t format, uint32_t hd) { return hd == 256 && format == BCH_KV_F16 ? 1 : 2; }
+constexpr uint32_t tree_groups(uint32_t format, uint32_t hd, uint32_t most) {
+  return format == BCH_KV_F16 && (hd == 256 || (hd == 128 && most > 1)) ? 1 : 2;
+}
+// The kernel of a batch whose tiles have up to `blocks`.
+constexpr uint32_t tree_most(uint32_t format, uint32_t hd, uint32_t blocks) {
+  const uint32_t most = tree_blocks(format, hd);
+  return blocks > 1 || tree_groups(format, hd, 1) == tree_groups(format, hd, most) ? most : 1;
+}
 
 uint32_t tree_tile_rows(uint32_t format, uint32_t hd) { return 16 * tree_blocks(format, hd); }
-uint32_t tree_tile_groups(uint32_t format, uint32_t hd) { return tree_groups(format, hd); }
+uint32_t tree_tile_groups(uint32_t format, uint32_t hd, uint32_t blocks) {
+  return tree_groups(format, hd, tree_most(format, hd, blocks));
+}
 
-template <uint32_t FORMAT, uint32_t HD>
-__global__ __launch_bounds__(256, tree_groups(FORMAT, HD)) void k_attn_tree(
+template <uint32_t FORMAT, uint32_t HD, uint32_t MOST>
+__global__ __launch_bounds__(256, tree_groups(FORMAT, HD, MOST)) void k_attn_tree(
     KvGeometry g, const KvAttnItem *__restrict__ items, const uint32_t *__restrict__ starts, const float *__restrict__ q,
     uint32_t q_stride, AttnOut to, uint32_t group, float c2, AttnTrees trees) {
   constexpr bool QUANT = FORMAT != BCH_KV_F16;
@@ -367,11 +382,8 @@ __global__ __launch_bounds__(256, tree_groups(FORMAT, HD)) void k_attn_tree(
   };
   for (uint32_t item = starts ? starts[share] : share; item < end; item++) {
     const KvAttnItem it = items[item];
-    constexpr uint32_t MOST = tree_blocks(FORMAT, HD);
     const uint32_t blocks = (it.rows + 15) / 16;
-    if (MOST >= 4 && blocks == 4)
-      tile(it, std::integral_constant<uint32_t, std::min(4u, MOST)>{});
-    else if (MOST >= 3 && blocks == 3)
+    if (MOST >= 3 && blocks == 3)
       tile(it, std::integral_constant<uint32_t, std::min(3u, MOST)>{});
     else if (MOST >= 2 && blocks == 2)
       tile(it, std::integral_constant<uint32_t, std::min(2u, MOST)>{});
@@ -390,9 +402,14 @@ void launch_tree_tiles(const AttnCall &a) {
     if (c.groups)
       k_attn_chunk<F, HD, true><<<c.groups * n_kv, 256, 0, a.stream>>>(a.geo, c.items, c.starts, a.q, a.q_stride, a.to,
                                                                        a.group, a.c2, trees);
-    if (t.groups)
-      k_attn_tree<F, HD><<<t.groups * n_kv, 256, 0, a.stream>>>(a.geo, t.items, t.starts, a.q, a.q_stride, a.to, a.group,
-                                                               a.c2, trees);
+    auto narrow = [&](auto most) {
+      k_attn_tree<F, HD, decltype(most)::value><<<t.groups * n_kv, 256, 0, a.stream>>>(
+          a.geo, t.items, t.starts, a.q, a.q_stride, a.to, a.group, a.c2, trees);
+    };
+    if (t.groups && plan->tree_blocks > 1)
+      narrow(std::integral_constant<uint32_t, tree_most(F, HD, 2)>{});
+    else if (t.groups)
+      narrow(std::integral_constant<uint32_t, tree_most(F, HD, 1)>{});
   });
 }
 

@@ -110,6 +110,7 @@ struct KvSchedule {
   KvWork tiles8, tiles16, chunks;  // tiles of at most 8, at most 16, and up to 128 rows
   std::vector<KvJoinItem> join;
   uint64_t records = 0;
+  uint32_t tree_blocks = 0;  // of 16 rows, of tiles16 at most where there are trees
 };
 // attn_paged.hip: the attention's work of a batch, with no more partial
 // results than partial_floats hold; with `trees` for the kernels of attn_tree.hip.
@@ -160,6 +161,7 @@ struct bch_kv_plan {
   // A batch with trees (else null): a node for each new token, and the masks.
   const bch::KvNode *d_nodes = nullptr;
   const uint32_t *d_masks = nullptr;
+  uint32_t tree_blocks = 0;  // (KvSchedule)
   struct Work {
     const bch::KvAttnItem *items = nullptr;
     const uint32_t *starts = nullptr;

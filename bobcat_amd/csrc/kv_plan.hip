@@ -272,6 +272,7 @@ static int plan_set(bch_kv_plan *plan, uint32_t n_seqs, const uint32_t *n_past, 
                     : reinterpret_cast<const uint32_t *>(plan->memory + at_starts[i]),
                 (uint32_t)works[i]->starts.size() - 1};
   plan->d_join = reinterpret_cast<const KvJoinItem *>(plan->memory + at_join);
+  plan->tree_blocks = work.tree_blocks;
   plan->n_join = (uint32_t)work.join.size();
   plan->join_rows = plan->join_splits = 0;
   for (const KvJoinItem &j : work.join) {

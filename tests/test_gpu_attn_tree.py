@@ -175,6 +175,7 @@ def large(rng, fmt, hd, kv, heads, seqs, new, past):
     ("i8", 64, 8, 32, 16, 18, 2500),    # two
     ("f8", 64, 8, 24, 40, 30, 3000), ("i8", 128, 8, 32, 24, 20, 2500), ("f8", 128, 4, 32, 24, 12, 3500),
     ("f16", 64, 8, 16, 40, 16, 3500),   # two blocks of an unquantised cache
+    ("f16", 128, 8, 32, 24, 12, 4000),  # two, of a workgroup that has its CU to itself
     ("f16", 128, 8, 32, 16, 40, 2500),  # wide ones
     ("i8", 64, 8, 32, 12, 96, 2000), ("f8", 256, 2, 16, 24, 40, 3000), ("f16", 256, 2, 8, 40, 40, 2500)])
 def test_tiles_by_the_batchs_work(hip, fmt, hd, kv, heads, seqs, new, past):
@@ -204,7 +205,7 @@ def test_tiles_by_the_batchs_work(hip, fmt, hd, kv, heads, seqs, new, past):
 
 @pytest.mark.parametrize("fmt,hd,kv,heads,seqs,new,past", [
     ("i8", 64, 8, 32, 40, 24, 3000), ("i8", 128, 8, 32, 24, 20, 2500), ("f16", 64, 8, 16, 40, 16, 3500),
-    ("f16", 128, 8, 32, 16, 40, 2500), ("i8", 64, 8, 32, 12, 96, 2000)])
+    ("f16", 128, 8, 32, 16, 40, 2500), ("f16", 128, 8, 32, 24, 12, 4000), ("i8", 64, 8, 32, 12, 96, 2000)])
 def test_rows_that_are_not_finite_in_larger_tiles(hip, fmt, hd, kv, heads, seqs, new, past):
     rng = np.random.default_rng(new)
     batch, pool, q, trees, pasts = large(rng, fmt, hd, kv, heads, seqs, new, past)
