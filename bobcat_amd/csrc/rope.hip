@@ -8,6 +8,9 @@
 // rest (an eighth of a turn either way) is exact to 2^-32 of a turn as an
 // integer and to 2^-24 of itself as a float, and its sine and cosine are their series to
 // x^9 and x^10, whose next terms are below 2^-28.
+//
+// Bound by the bytes: 7,362 tokens, 40 heads of 128, 301 MB, 61.5 us (4.9 TB/s, a copy's
+// rate); few tokens by latency, one of 40 heads of 64 2.9 us, 437 of 10 heads of 256 5.0.
 #include <algorithm>
 #include <cmath>
 #include <memory>
