@@ -83,21 +83,34 @@ struct Heat {
   }
 };
 
-__device__ __forceinline__ double wave_sum_f64(double x) {
-#pragma unroll
-  for (int i = 1; i < 64; i *= 2) x += __shfl_xor(x, i, 64);
-  return x;
+// What DPP control CTRL names, for the rows of 16 lanes of ROWS; 0 where there is none.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ uint32_t dpp_u32(uint32_t x) {
+  return __builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
 }
-
-// The sum of the lanes up to and with this one.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ double dpp_f64(double x) {
+  const uint64_t v = __builtin_bit_cast(uint64_t, x);
+  return __builtin_bit_cast(double, (uint64_t)dpp_u32<CTRL, ROWS>(v >> 32) << 32 | dpp_u32<CTRL, ROWS>((uint32_t)v));
+}
+// The sum of the lanes up to and with this one: within rows of 16 (from 1, 2, 4 and 8 lanes before), then the first and third
+// rows' into the second and fourth, then the first half's into the second.
 __device__ __forceinline__ double wave_scan_f64(double x) {
-#pragma unroll
-  for (int i = 1; i < 64; i *= 2) {
-    const double y = __shfl_up(x, i, 64);
-    if (threadIdx.x % 64 >= (uint32_t)i) x += y;
-  }
+  x += dpp_f64<0x111>(x);
+  x += dpp_f64<0x112>(x);
+  x += dpp_f64<0x114>(x);
+  x += dpp_f64<0x118>(x);
+  x += dpp_f64<0x142, 0xa>(x);
+  x += dpp_f64<0x143, 0xc>(x);
   return x;
 }
+// Lane `from`'s, the same for the wave.
+__device__ __forceinline__ double lane_f64(double x, uint32_t from) {
+  const uint64_t v = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, from), hi = __builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), from);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum_f64(double x) { return lane_f64(wave_scan_f64(x), 63); }
 __device__ __forceinline__ uint32_t wave_min_u32(uint32_t x) {
 #pragma unroll
   for (int i = 1; i < 64; i *= 2) x = min(x, (uint32_t)__shfl_xor((int)x, i, 64));
@@ -243,16 +256,20 @@ struct Walk {
         for (uint32_t k = 0; k < 4; k++)
           if (x[k].top > -INFINITY) sum += (double)x[k].sum * heat.weight(x[k].top, top);
       }
-      float all = top;
-#pragma unroll
-      for (int k = 1; k < 16; k *= 2) all = fmaxf(all, __shfl_xor(all, k, 64));
+      float all = fmaxf(top, dpp<kDppXor1>(top));
+      all = fmaxf(all, dpp<kDppXor2>(all));
+      all = fmaxf(all, dpp<kDppHalfMirror>(all));
+      all = fmaxf(all, dpp<kDppMirror>(all));
       if (top > -INFINITY) sum *= heat.weight(top, all);
       if (top != all) best = ~0u;
-#pragma unroll
-      for (int k = 1; k < 16; k *= 2) {
-        sum += __shfl_xor(sum, k, 64);
-        best = min(best, (uint32_t)__shfl_xor((int)best, k, 64));
-      }
+      sum += dpp_f64<kDppXor1>(sum);
+      sum += dpp_f64<kDppXor2>(sum);
+      sum += dpp_f64<kDppHalfMirror>(sum);
+      sum += dpp_f64<kDppMirror>(sum);
+      best = min(best, dpp_u32<kDppXor1>(best));
+      best = min(best, dpp_u32<kDppXor2>(best));
+      best = min(best, dpp_u32<kDppHalfMirror>(best));
+      best = min(best, dpp_u32<kDppMirror>(best));
       if (lane == 0) m.top[i] = all, m.sum[i] = sum, m.best[i] = all > -INFINITY ? best : BCH_NO_TOKEN;
     }
     __syncthreads();
@@ -323,7 +340,7 @@ struct Walk {
     // piece by themselves: clamped places would take a register each.)
     template <uint32_t STRIDE, uint32_t N>
     __device__ __forceinline__ void load(const Heat &heat, float (&x)[N], uint32_t first) const {
-      float d[N];
+      float d[N] = {};
       auto bring = [&](float (&to)[N], const float *from) __attribute__((always_inline)) {
         const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(from), 0, len * 4, 0x00020000);
 #pragma unroll
@@ -334,9 +351,9 @@ struct Walk {
       if (draft) bring(d, draft);
 #pragma unroll
       for (uint32_t j = 0; j < N; j++) {
-        const float p = first + STRIDE * j < len ? heat.weight(logit(x[j]), top) * inv : 0.f;
-        // (What the target does not have stays at 0, whatever the draft says.)
-        x[j] = draft && p > 0.f ? fmaxf(fmaf(-c, d[j], p), 0.f) : p;
+        const float p = heat.weight(first + STRIDE * j < len ? logit(x[j]) : -INFINITY, top) * inv;
+        // (What the target does not have stays at 0, whatever the draft says.  Without a draft c is 0.)
+        x[j] = p > 0.f ? fmaxf(fmaf(-c, d[j], p), 0.f) : 0.f;
       }
     }
   };
@@ -344,7 +361,7 @@ struct Walk {
     const uint32_t at_t = __builtin_amdgcn_readfirstlane(t), from = __builtin_amdgcn_readfirstlane(piece) * kPiece;
     const uint64_t at = (uint64_t)(row0 + at_t) * a.n_vocab + from;
     return {a.logits + at, c > 0 ? a.draft + at : nullptr, fmaxf(m.top[t], -kLargest), c > 0 ? (float)(1.0 / m.sum[t]) : 1.f,
-            (float)c, min(kPiece, a.n_vocab - from)};
+            c > 0 ? (float)c : 0.f, min(kPiece, a.n_vocab - from)};
   }
   __device__ double *rest(uint32_t which) const { return a.rest + ((uint64_t)which * a.n_seqs + seq_at) * a.n_pieces; }
   // The sum of a round's pieces (never below 0), by each wave for itself.
@@ -396,7 +413,7 @@ struct Walk {
       mine = 0;
       for (uint32_t i = first; i < end; i++) mine += mass(i);
       up = wave_scan_f64(mine);
-      total = __shfl(up, 63, 64);
+      total = lane_f64(up, 63);
       if (total > 0 || (c == 0 && !without)) break;
       c = 0, without = false;  // nothing is left: p itself
     }
@@ -419,8 +436,8 @@ struct Walk {
       }
       from = pick != ~0u ? pick : first;
     }
-    sum = __shfl(sum, owner, 64);
-    from = __builtin_amdgcn_readfirstlane(__shfl((int)from, owner, 64));
+    sum = lane_f64(sum, __builtin_amdgcn_readfirstlane(owner));
+    from = __builtin_amdgcn_readlane((int)from, __builtin_amdgcn_readfirstlane(owner));
     // The token in the piece.  Its own sum may end below the goal by rounding: the last token with any weight
     // then, or where it has none (all of it was fallen children) the pieces behind it, then those before.
 #pragma unroll 1
@@ -457,21 +474,25 @@ struct Walk {
       __syncthreads();
       double at = sum + upto - run;
       for (uint32_t i = 0; i < wave; i++) at += run_s[i];
-      uint32_t pick = ~0u, last = ~0u;  // (last: counted down, so that the least is the last)
+      uint32_t pick = ~0u, last = ~0u;  // (places go up with the lanes)
 #pragma unroll 4
       for (uint32_t j = 0; j < PER; j++) {
         const float x = mine_s[j];
         at += (double)x;
         const uint32_t i = piece * kPiece + PER * tid + j;
-        if (x > 0.f) last = ~i;
+        if (x > 0.f) last = i;
         if (x > 0.f && pick == ~0u && at > goal && inside) pick = i;
       }
-      pick = wave_min_u32(pick), last = wave_min_u32(last);
-      if (lane == 0) pick_s[wave] = pick, last_s[wave] = last;
+      const uint64_t picks = __builtin_amdgcn_ballot_w64(pick != ~0u), lasts = __builtin_amdgcn_ballot_w64(last != ~0u);
+      if (picks ? lane == __ffsll((unsigned long long)picks) - 1 : lane == 0) pick_s[wave] = pick;
+      if (lasts ? lane == 63 - __clzll((long long)lasts) : lane == 0) last_s[wave] = last;
       __syncthreads();
-      for (uint32_t i = 0; i < WAVES; i++) pick = min(pick, pick_s[i]), last = min(last, last_s[i]);
-      if (pick != ~0u) return pick;
-      if (last != ~0u) return ~last;
+      for (uint32_t i = 0; i < WAVES; i++) {
+        if (pick_s[i] != ~0u) return pick_s[i];
+      }
+      for (uint32_t i = WAVES; i-- > 0;) {
+        if (last_s[i] != ~0u) return last_s[i];
+      }
       __syncthreads();
     }
     return BCH_NO_TOKEN;
