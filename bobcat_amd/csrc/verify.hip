@@ -20,9 +20,10 @@
 //     its goal, then the token in it.  Without a draft a workgroup does a sequence.  With one
 //     (REST) a workgroup for each piece walks by itself to where the sum for a rejection is missing,
 //     adds its own piece to it, and the last one to do so goes on.  (One workgroup's sum
-//     over the whole vocabulary takes about 70 us.)  For trees there are launches before it that only add pieces,
+//     over 151,936 logits takes about 50 us.)  For trees there are launches before it that only add pieces,
 //     for the first rejections; what those do not cover the last workgroup sums alone.  Bound by latency, some
-//     fifteen loads that wait for each other: one sequence of 5 tokens 15 us, 48 of up to 6 19 us.
+//     fifteen loads that wait for each other, and code that runs once: one sequence of 5 tokens 12 us, 48 of up to 6
+//     16 us.  (So lanes are summed by row moves, not through LDS, and a piece's elements have no branches: 14.5 and 19.2.)
 #include <algorithm>
 #include <cmath>
 
@@ -36,8 +37,9 @@ namespace bch {
 constexpr uint32_t kRowThreads = 256, kRowPer = 16, kPiece = kRowThreads * kRowPer;
 constexpr uint32_t kWalkThreads = 256;
 // Rejections of trees that all workgroups sum, a launch each (of chains there is one at most).  Passes with
-// 0, 1, 2, 3, 4 and 6 of them: 16 trees of 16 to 32 drawn drafts, 65,536 logits, 171, 100, 89, 77, 71 and 83 us;
-// 8 of 8 to 16, without replacement, 151,936 logits, 279, 126, 94, 70, 54 and 67; one of 16 90, 51, 40, 37, 39 and 52.
+// 0, 1, 2, 3, 4, 5 and 6 of them: 16 trees of 16 to 32 drawn drafts, 65,536 logits, 101, 82, 74, 66, 62, 65 and
+// 71 us; 8 of 8 to 16, without replacement, 151,936 logits, 153, 100, 77, 59, 47, 53 and 58; one of 16 drawn ones
+// 51, 42, 33, 32, 34, 39 and 45.
 constexpr uint32_t kRounds = 4;
 constexpr float kLargest = 3.402823466e38f;
 
