@@ -251,25 +251,30 @@ static void deal(KvSchedule &w, KvWork &work, const std::vector<Tile> &tiles, ui
 // and 192 rows: int8 82, 106, 177, 213 us narrow and 132, 142, 174, 216 wide; f16 109, 147, 256,
 // 359 and 151, 136, 184, 272.)  Below 16 steps of a block for each wave the time is latency, and tiles of
 // one block share it among more waves (one sequence of 600 keys and 32 rows, heads of 64: 8.2
-// us, in tiles of two 11.3, wide 20.6; twelve of up to 2,500 keys and 96 rows 21, 24 and 36);
-// three beat two only where there is much more (12 of 256 rows: 52 us and 45; 32 of 96 rows
-// and 6,000 keys 73 and 75).
+// us, in tiles of two 11.3, wide 20.6; twelve of up to 2,500 keys and 96 rows 21, 24 and 36).  Not so in f16 where
+// each tile brings more keys than the caches hold, from 96 MB of them on: five sequences of up to 12,868 keys and 48
+// rows, heads of 128, 70 us in tiles of one block and 54 by the rule for large batches; eight of up to 6,000 and 64
+// rows 55 and 48; but three of up to 16,000, 90 MB, 32 and 46, and in int8 20 of up to 6,000 43 and 50.  Three
+// blocks beat two only where there is much more (12 of 256 rows: 52 us and 45; 32 of 96 rows and 6,000 keys 73
+// and 75).
 struct TreeTiles {
   bool wide;
   uint32_t blocks;
 };
 static TreeTiles tree_tiles(const std::vector<KvSeq> &seqs, uint32_t group, uint32_t n_kv, uint32_t format,
                             uint32_t head_dim, uint32_t n_cus) {
-  uint64_t block_steps = 0, wide_steps = 0, keys = 0;
+  uint64_t block_steps = 0, wide_steps = 0, keys = 0, most = 1;
   for (const KvSeq &q : seqs) {
     const uint64_t rows = (uint64_t)q.n_new * group, steps = (q.past + q.n_new + 31) / 32;
+    most = std::max(most, (rows + 15) / 16);
     block_steps += (rows + 15) / 16 * steps;
     wide_steps += (rows + kChunkRows - 1) / kChunkRows * steps;
     keys += q.past + q.n_new;
   }
   const uint64_t waves = 4ull * n_cus * tree_tile_groups(format, head_dim, 1), work = block_steps * n_kv;
   const uint64_t bytes = keys * n_kv * kv_block_bytes(format, head_dim) / kKvBlock;
-  if (work <= 16 * waves) return {false, 1};
+  const bool cached = format != BCH_KV_F16 || bytes <= (96ull << 20);
+  if (most == 1 || (work <= 16 * waves && cached)) return {false, 1};
   const double ratio = format != BCH_KV_F16 ? 6.3 : bytes <= (128ull << 20) ? 5.0 : 3.0;
   if (ratio * wide_steps < block_steps) return {true, 1};
   return {false, std::min(work <= 32 * waves ? 2u : 3u, tree_tile_rows(format, head_dim) / 16)};
