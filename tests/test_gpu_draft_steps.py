@@ -161,7 +161,7 @@ def test_plans_are_held_by_work_that_reads_them(hip):
     b, r = hip.new_buffer(1 << 16), hip.rope(64, 1e4)
     calls = [lambda p: hip.rope_paged(r, p, RopeRows(b.at(0), 64, b.at(1 << 15), 64, 1), None),
              lambda p: hip.kv_keep(p, 0, 1, b.at(0), 1, 0, b.at(1 << 15), b.at(1 << 14)),
-             lambda p: hip.verify_drafts(p, 0, 1, 8, b.at(0), b.at(1024), b.at(2048), b.at(3072), b.at(4096), b.at(5120), b.at(6144))]
+             lambda p: hip.verify_drafts(p, 0, 1, 8, b.at(0), *(b.at(256 * i) for i in range(1, 7)))]
     for call in calls:
         plan = hip.kv_plan("i8", 1, 64, 16, 1, 1)
         give = lambda: plan.set([0], [5], [[0]], parents=as_given(tree))  # noqa: E731
