@@ -410,94 +410,94 @@ struct Walk {
     };
     // Every wave finds the piece for itself, a lane has `per` consecutive ones.
     const uint32_t per = (a.n_pieces + 63) / 64, first = min(lane * per, a.n_pieces), end = min(first + per, a.n_pieces);
-    double mine, up, total;
-    for (;;) {
-      mine = 0;
+    for (;; c = 0, without = false) {  // (where nothing is left: p itself)
+      double mine = 0;
       for (uint32_t i = first; i < end; i++) mine += mass(i);
-      up = wave_scan_f64(mine);
-      total = lane_f64(up, 63);
-      if (total > 0 || (c == 0 && !without)) break;
-      c = 0, without = false;  // nothing is left: p itself
-    }
-    // The first piece whose end lies past the goal; the last with any mass where rounding leaves none.
-    const double goal = (double)m.u[0] * total;
-    const uint64_t past = __builtin_amdgcn_ballot_w64(mine > 0 && up > goal), any = __builtin_amdgcn_ballot_w64(mine > 0);
-    const bool inside = past != 0;
-    const uint32_t owner = inside ? __ffsll((unsigned long long)past) - 1 : any ? 63 - __clzll((long long)any) : 0;
-    double sum = up - mine;
-    uint32_t from = first;
-    if (per > 1) {
-      double at = sum;
-      uint32_t pick = ~0u;
-      for (uint32_t i = first; i < end; i++) {
-        const double x = mass(i);
-        if (x > 0 && (pick == ~0u || !inside)) {
-          if (!inside || at + x > goal) pick = i, sum = at;
+      const double up = wave_scan_f64(mine), total = lane_f64(up, 63);
+      const bool itself = c == 0 && !without;
+      if (!(total > 0) && !itself) continue;
+      // The first piece whose end lies past the goal; the last with any mass where rounding leaves none.
+      const double goal = (double)m.u[0] * total;
+      const uint64_t past = __builtin_amdgcn_ballot_w64(mine > 0 && up > goal), any = __builtin_amdgcn_ballot_w64(mine > 0);
+      const bool inside = past != 0;
+      const uint32_t owner = inside ? __ffsll((unsigned long long)past) - 1 : any ? 63 - __clzll((long long)any) : 0;
+      double sum = up - mine;
+      uint32_t from = first;
+      if (per > 1) {
+        double at = sum;
+        uint32_t pick = ~0u;
+        for (uint32_t i = first; i < end; i++) {
+          const double x = mass(i);
+          if (x > 0 && (pick == ~0u || !inside)) {
+            if (!inside || at + x > goal) pick = i, sum = at;
+          }
+          at += x;
         }
-        at += x;
+        from = pick != ~0u ? pick : first;
       }
-      from = pick != ~0u ? pick : first;
-    }
-    sum = lane_f64(sum, __builtin_amdgcn_readfirstlane(owner));
-    from = __builtin_amdgcn_readlane((int)from, __builtin_amdgcn_readfirstlane(owner));
-    // The token in the piece.  Its own sum may end below the goal by rounding: the last token with any weight
-    // then, or where it has none (all of it was fallen children) the pieces behind it, then those before.
+      sum = lane_f64(sum, __builtin_amdgcn_readfirstlane(owner));
+      from = __builtin_amdgcn_readlane((int)from, __builtin_amdgcn_readfirstlane(owner));
+      // The token in the piece.  Its own sum may end below the goal by rounding: the last token with any weight
+      // then, or where it has none (all of it was fallen children) the pieces behind it, then those before.
 #pragma unroll 1
-    for (uint32_t k = 0; k < a.n_pieces; k++) {
-      const uint32_t piece = from + k < a.n_pieces ? from + k : a.n_pieces - 1 - k;
-      // Read side by side, and taken PER in a row.  (Eight at a time, for the registers.)
-      {
-        const Piece part = piece_of(piece);
+      for (uint32_t k = 0; k < a.n_pieces; k++) {
+        const uint32_t piece = from + k < a.n_pieces ? from + k : a.n_pieces - 1 - k;
+        // Read side by side, and taken PER in a row.  (Eight at a time, for the registers.)
+        {
+          const Piece part = piece_of(piece);
 #pragma unroll 1
-        for (uint32_t i0 = tid; i0 < kPiece; i0 += kWalkThreads * 8) {
-          float x[8];
-          part.load<kWalkThreads>(heat, x, i0);
+          for (uint32_t i0 = tid; i0 < kPiece; i0 += kWalkThreads * 8) {
+            float x[8];
+            part.load<kWalkThreads>(heat, x, i0);
 #pragma unroll
-          for (uint32_t j = 0; j < 8; j++) {
-            const uint32_t i = i0 + kWalkThreads * j;
-            x_s[i + i / PER] = x[j];
+            for (uint32_t j = 0; j < 8; j++) {
+              const uint32_t i = i0 + kWalkThreads * j;
+              x_s[i + i / PER] = x[j];
+            }
           }
         }
-      }
-      __syncthreads();
-      if (without) {
-        for (uint32_t s = m.child[t]; s != kKvNone; s = m.sibling[s]) {
-          const uint32_t i = m.token[s] - piece * kPiece;
-          if (i < kPiece) x_s[i + i / PER] = 0.f;  // (every thread the same)
+        __syncthreads();
+        if (without) {
+          for (uint32_t s = m.child[t]; s != kKvNone; s = m.sibling[s]) {
+            const uint32_t i = m.token[s] - piece * kPiece;
+            if (i < kPiece) x_s[i + i / PER] = 0.f;  // (every thread the same)
+          }
+          __syncthreads();
+        }
+        const float *mine_s = x_s + tid * (PER + 1);
+        double run = 0;
+#pragma unroll 4
+        for (uint32_t j = 0; j < PER; j++) run += (double)mine_s[j];
+        const double upto = wave_scan_f64(run);
+        if (lane == 63) run_s[wave] = upto;
+        __syncthreads();
+        double at = sum + upto - run;
+        for (uint32_t i = 0; i < wave; i++) at += run_s[i];
+        uint32_t pick = ~0u, last = ~0u;  // (places go up with the lanes)
+#pragma unroll 4
+        for (uint32_t j = 0; j < PER; j++) {
+          const float x = mine_s[j];
+          at += (double)x;
+          const uint32_t i = piece * kPiece + PER * tid + j;
+          if (x > 0.f) last = i;
+          if (x > 0.f && pick == ~0u && at > goal && inside) pick = i;
+        }
+        const uint64_t picks = __builtin_amdgcn_ballot_w64(pick != ~0u), lasts = __builtin_amdgcn_ballot_w64(last != ~0u);
+        if (picks ? lane == __ffsll((unsigned long long)picks) - 1 : lane == 0) pick_s[wave] = pick;
+        if (lasts ? lane == 63 - __clzll((long long)lasts) : lane == 0) last_s[wave] = last;
+        __syncthreads();
+        for (uint32_t i = 0; i < WAVES; i++) {
+          if (pick_s[i] != ~0u) return pick_s[i];
+        }
+        for (uint32_t i = WAVES; i-- > 0;) {
+          if (last_s[i] != ~0u) return last_s[i];
         }
         __syncthreads();
       }
-      const float *mine_s = x_s + tid * (PER + 1);
-      double run = 0;
-#pragma unroll 4
-      for (uint32_t j = 0; j < PER; j++) run += (double)mine_s[j];
-      const double upto = wave_scan_f64(run);
-      if (lane == 63) run_s[wave] = upto;
-      __syncthreads();
-      double at = sum + upto - run;
-      for (uint32_t i = 0; i < wave; i++) at += run_s[i];
-      uint32_t pick = ~0u, last = ~0u;  // (places go up with the lanes)
-#pragma unroll 4
-      for (uint32_t j = 0; j < PER; j++) {
-        const float x = mine_s[j];
-        at += (double)x;
-        const uint32_t i = piece * kPiece + PER * tid + j;
-        if (x > 0.f) last = i;
-        if (x > 0.f && pick == ~0u && at > goal && inside) pick = i;
-      }
-      const uint64_t picks = __builtin_amdgcn_ballot_w64(pick != ~0u), lasts = __builtin_amdgcn_ballot_w64(last != ~0u);
-      if (picks ? lane == __ffsll((unsigned long long)picks) - 1 : lane == 0) pick_s[wave] = pick;
-      if (lasts ? lane == 63 - __clzll((long long)lasts) : lane == 0) last_s[wave] = last;
-      __syncthreads();
-      for (uint32_t i = 0; i < WAVES; i++) {
-        if (pick_s[i] != ~0u) return pick_s[i];
-      }
-      for (uint32_t i = WAVES; i-- > 0;) {
-        if (last_s[i] != ~0u) return last_s[i];
-      }
-      __syncthreads();
+      // No token has any weight: what was left was roundings (a chosen child's p is f64, its term in a piece's sum
+      // f32).  Of p itself the largest logit has the weight 1.
+      if (itself) return BCH_NO_TOKEN;
     }
-    return BCH_NO_TOKEN;
   }
 };
 
