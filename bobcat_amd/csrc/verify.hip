@@ -309,7 +309,9 @@ struct Walk {
       for (; s != kKvNone; s = m.sibling[s]) {
         const double u = (double)m.u[s], p = m.p[s], q = m.q[s];
         if (looked == kKvNone) {
-          if (p > 0 && (greedy ? true : drawn ? u * q * total < (p - c * q) * left : u * total < p)) break;
+          // (A child's q is part of the draft's mass that is left, but for roundings of the f32 probabilities.)
+          if (a.distinct) left = fmax(left, q);
+          if (p > 0 && (greedy ? true : drawn ? p > c * q && u * q * total < (p - c * q) * left : u * total < p)) break;
           if (drawn) {
             if (left > 0) c += total / left;
             if (a.distinct) left -= q;

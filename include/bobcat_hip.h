@@ -587,7 +587,8 @@ typedef struct bch_verdict {
  * with u·q(x) < p(x) stays and becomes the current token; for each child that does not,
  *   p <- max(p - q, 0), normalised,
  * before the next is looked at, and with `distinct` q <- q without x, divided by 1 - Σ q
- * of those looked at.  Children chosen without chance have q = 1 each for themselves.
+ * of those looked at (or by the next child's own q where rounded probabilities leave less than
+ * that).  Children chosen without chance have q = 1 each for themselves.
  * Where no child stays, the next token is the first in token order up to which p sums to
  * more than the first token's uniform times the whole.  At a temperature not above 0
  * (or NaN) p is 1 for the first of the largest logits and `draft` is not looked at.

@@ -4,6 +4,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
+from _drafts import verify
 from bobcat_amd.backend import NO_TOKEN
 from test_gpu_verify import plan_of, verdict
 
@@ -41,3 +42,40 @@ def test_children_that_are_all_the_target_has(hip, vocab, places):
     assert sure.sum() > none.sum() // 2 and (got[2][sure] == want[sure]).all()
     chances = got[3].reshape(n, kids + 1)[none, 0]
     assert (chances > 0).all()
+
+
+@pytest.mark.parametrize("masses", [(0.5, 0.5), (0.75, 0.25), (0.25, 0.25, 0.125, 0.25, 0.0625, 0.0625)])
+@pytest.mark.parametrize("vocab", [40, 5000])
+def test_a_draft_whose_tokens_are_all_drawn(hip, masses, vocab):
+    """A draft of a few tokens, drawn without replacement to the last, whose f32 probabilities sum to just over 1: the last
+    one has all of the draft that is left, whatever the rounded sums of the others say.  Its row normalised in f64 is the
+    definition's.  (Tests lie 0.1 and more from their borders, draws by chance: 2^-20 each, with fixed seeds.)"""
+    rng = np.random.default_rng(vocab + len(masses))
+    few = len(masses) + 1
+    tree, n = [-1] + [0] * few, 64
+    q = np.zeros((n, few + 1, vocab), np.float32)
+    x = np.stack([rng.permutation(vocab)[:few] for _ in range(n)])
+    logits = rng.standard_normal((n, few + 1, vocab)).astype(np.float32)
+    u = np.full((n, few + 1), 0.9, np.float32)
+    for i in range(n):
+        q[i, 0, x[i, :-1]] = masses
+        q[i, 0, x[i, -2]] = np.nextafter(np.float32(masses[-1]), np.float32(1))
+        q[i, 0, x[i, -1]] = 2.0 ** -30
+        q[i, 1:] = 1 / vocab
+        # The target: next to nothing of the first; of the last less than c·q leaves, or half of all.
+        logits[i, 0, x[i, :-1]] = -9
+        others = np.delete(logits[i, 0].astype(np.float64), x[i, -1])
+        logits[i, 0, x[i, -1]] = -40 if i % 2 else np.log(np.exp(others).sum())
+    u[1::2, -1], u[::2, -1] = 0.0, 0.3  # the last: rejected with any uniform; kept with half of what is left
+    u[:, 0] = rng.random(n, np.float32)
+    tokens = np.concatenate([np.zeros((n, 1)), x], 1).astype(np.uint32).reshape(-1)
+    heat = np.ones(n, np.float32)
+    got = verdict(hip, plan_of(hip, [tree] * n), [tree] * n, logits.reshape(-1, vocab), q.reshape(-1, vocab), tokens, u.reshape(-1),
+                  heat, True)
+    for i in range(n):
+        row = q[i].astype(np.float64)
+        assert row[0].sum() > 1
+        kept, path, token, _ = verify(tree, logits[i], row / row.sum(1, keepdims=True), tokens[i * (few + 1):][:few + 1], u[i], 1.0,
+                                      True)
+        assert kept == (1 if i % 2 else 2)
+        assert got[0][i] == kept and got[1][i * (few + 1):][:few + 1].tolist() == path and got[2][i] == token, i
