@@ -15,7 +15,8 @@
 //
 //   k_verify_rows reads every token's logits once, in pieces of the vocabulary: the
 //     largest, the first place of it, and the sum of the exponentials.  Bound by
-//     those bytes: 231 rows of 151,936 logits 24 us (5.7 TB/s, some of it out of the caches).
+//     those bytes: 231 rows of 151,936 logits 26 us (5.4 TB/s, some of it out of the caches); with
+//     f32 sums, which lose what is below 2^-24 of a thread's or a wave's, 24.6.
 //   k_verify_walk walks down each tree, out of LDS, and draws: the piece in which the sum passes
 //     its goal, then the token in it.  Without a draft a workgroup does a sequence.  With one
 //     (REST) a workgroup for each piece walks by itself to where the sum for a rejection is missing,
@@ -46,8 +47,9 @@ constexpr float kLargest = 3.402823466e38f;
 // One piece of a row: its largest logit, where it is first, and the sum of
 // exp((x - largest) / temperature).
 struct VerifyPiece {
-  float top, sum;
-  uint32_t at, pad;
+  double sum;
+  float top;
+  uint32_t at;
 };
 
 struct VerifyArgs {
@@ -136,7 +138,8 @@ __device__ __forceinline__ uint32_t seq_of_row(const VerifyArgs &a, uint32_t row
 // VEC: rows are 16-byte aligned.
 template <bool VEC>
 __global__ __launch_bounds__(kRowThreads) void k_verify_rows(VerifyArgs a) {
-  __shared__ float top_s[4], sum_s[4];
+  __shared__ float top_s[4];
+  __shared__ double sum_s[4];
   __shared__ uint32_t at_s[4];
   const uint32_t row = blockIdx.x / a.n_pieces, piece = blockIdx.x % a.n_pieces, tid = threadIdx.x;
   const uint32_t base = piece * kPiece, len = min(kPiece, a.n_vocab - base);
@@ -170,16 +173,17 @@ __global__ __launch_bounds__(kRowThreads) void k_verify_rows(VerifyArgs a) {
   for (int j = kRowPer - 1; j >= 0; j--)
     if (x[j] == top) at = base + place(j);
   at = wave_min_u32(at);
-  float sum = 0.f;
+  double sum = 0;  // (of f32 terms, as every sum over the vocabulary here)
   if (temperature > 0.f && top > -INFINITY) {
     const Heat heat(temperature);
 #pragma unroll
-    for (uint32_t j = 0; j < kRowPer; j++) sum += heat.weight(x[j], top);
+    for (uint32_t j = 0; j < kRowPer; j++) sum += (double)heat.weight(x[j], top);
   }
-  sum = block_sum<kRowThreads>(sum, sum_s);
-  if (tid % 64 == 0) at_s[tid / 64] = at;
+  sum = wave_sum_f64(sum);
+  if (tid % 64 == 0) at_s[tid / 64] = at, sum_s[tid / 64] = sum;
   __syncthreads();
-  if (tid == 0) a.pieces[blockIdx.x] = {top, sum, min(min(at_s[0], at_s[1]), min(at_s[2], at_s[3])), 0};
+  if (tid == 0)
+    a.pieces[blockIdx.x] = {(sum_s[0] + sum_s[1]) + (sum_s[2] + sum_s[3]), top, min(min(at_s[0], at_s[1]), min(at_s[2], at_s[3]))};
 }
 
 // What a workgroup knows of its sequence, in LDS: of each token its row's largest
@@ -249,14 +253,14 @@ struct Walk {
         const float before = top;
 #pragma unroll
         for (uint32_t k = 0; k < 4; k++) {
-          if (j0 + 16 * k + lane >= a.n_pieces) x[k] = {-INFINITY, 0.f, ~0u, 0};
+          if (j0 + 16 * k + lane >= a.n_pieces) x[k] = {0, -INFINITY, ~0u};
           best = x[k].top > top ? x[k].at : best;  // (pieces go up, and so do the places)
           top = fmaxf(top, x[k].top);
         }
         if (before > -INFINITY) sum *= heat.weight(before, top);
 #pragma unroll
         for (uint32_t k = 0; k < 4; k++)
-          if (x[k].top > -INFINITY) sum += (double)x[k].sum * heat.weight(x[k].top, top);
+          if (x[k].top > -INFINITY) sum += x[k].sum * heat.weight(x[k].top, top);
       }
       float all = fmaxf(top, dpp<kDppXor1>(top));
       all = fmaxf(all, dpp<kDppXor2>(all));
@@ -383,11 +387,10 @@ struct Walk {
     double sum = 0;
 #pragma unroll 1
     for (uint32_t j0 = 0; j0 < kPiece / 64; j0 += 8) {
-      float x[8], all = 0.f;
+      float x[8];
       part.load<64>(heat, x, 64 * j0 + threadIdx.x % 64);
 #pragma unroll
-      for (uint32_t j = 0; j < 8; j++) all += x[j];
-      sum += (double)all;
+      for (uint32_t j = 0; j < 8; j++) sum += (double)x[j];
     }
     return wave_sum_f64(sum);
   }
@@ -404,7 +407,7 @@ struct Walk {
     auto mass = [&](uint32_t piece) {
       if (c > 0) return a.n_pieces <= 64 ? held : coherent_load(rest(latest) + piece);
       const VerifyPiece p = a.pieces[(uint64_t)(row0 + t) * a.n_pieces + piece];
-      double sum = p.top > -INFINITY ? (double)p.sum * heat.weight(p.top, m.top[t]) : 0.0;
+      double sum = p.top > -INFINITY ? p.sum * heat.weight(p.top, m.top[t]) : 0.0;
       if (without)
         for (uint32_t s = m.child[t]; s != kKvNone; s = m.sibling[s])
           if (m.token[s] / kPiece == piece) sum -= m.p[s] * m.sum[t];
@@ -528,10 +531,10 @@ __global__ __launch_bounds__(kWalkThreads, REST ? 6 : 2) void k_verify_walk(Veri
     if (open) {
       float x[kPiece / kWalkThreads];
       w.piece_of(piece).load<kWalkThreads>(w.heat, x, tid);
-      float sum = 0.f;
+      double sum = 0;
 #pragma unroll
-      for (uint32_t j = 0; j < kPiece / kWalkThreads; j++) sum += x[j];
-      const double by_wave = wave_sum_f64((double)sum);
+      for (uint32_t j = 0; j < kPiece / kWalkThreads; j++) sum += (double)x[j];
+      const double by_wave = wave_sum_f64(sum);
       if (lane == 0) sum_s[wave] = by_wave;
       __syncthreads();
       if (tid == 0) {

@@ -79,3 +79,31 @@ def test_a_draft_whose_tokens_are_all_drawn(hip, masses, vocab):
                                       True)
         assert kept == (1 if i % 2 else 2)
         assert got[0][i] == kept and got[1][i * (few + 1):][:few + 1].tolist() == path and got[2][i] == token, i
+
+
+def term_errors(logits, temperature):
+    """What the sum of a row's exponentials may be off by, relative to it: its terms are f32, the sum is f64.  A term 2^-a of
+    the largest is off by two roundings of its exponent (the difference and the product: 2·a·ln 2·2^-24 of the term) and by two
+    exponentials (to the piece's largest and from there to the row's) of at most 2^-23 each."""
+    x = (logits.astype(np.float64) - logits.max()) / np.float64(temperature)
+    p = np.exp(x)
+    return (p * (2 * -x + 4)).sum() / p.sum() * 2.0 ** -24
+
+
+@pytest.mark.parametrize("vocab", [4096, 4095, 12288, 12289])
+def test_sums_of_terms_far_apart(hip, vocab):
+    """Each piece has 256 tokens of weight 1 and else tokens of 0.98·2^-24, which an f32 sum of 1 and more loses: 14.7 of 15
+    roundings for each of the former."""
+    stride = 4 if vocab % 4 == 0 else 1  # (where rows are read four at a time, a thread's first are four apart)
+    heavy = (np.arange(vocab) % 4096 < 256 * stride) & (np.arange(vocab) % stride == 0)
+    row = np.where(heavy, 0, np.log(0.98 * 2.0 ** -24)).astype(np.float32)
+    trees, n = [[-1, 0, 0]] * 3, 9
+    logits = np.tile(row, (n, 1))
+    tokens = np.tile(np.array([0, 8, 9], np.uint32), 3)
+    got = verdict(hip, plan_of(hip, trees), trees, logits, None, tokens, np.full(n, 0.5, np.float32), np.ones(3, np.float32))
+    p = np.exp(row.astype(np.float64))
+    want = p[tokens] / p.sum()
+    bound = term_errors(row, 1.0) + 2.0 ** -24  # (and the chance's own rounding)
+    assert bound < 6 * 2.0 ** -24
+    chances = got[3].reshape(3, 3)[:, 1:]
+    assert (np.abs(chances / want.reshape(3, 3)[:, 1:] - 1) <= bound).all()
