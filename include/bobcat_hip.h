@@ -593,12 +593,17 @@ typedef struct bch_verdict {
  * more than the first token's uniform times the whole.  At a temperature not above 0
  * (or NaN) p is 1 for the first of the largest logits and `draft` is not looked at.
  * A logit that is NaN counts as -inf, +inf as the largest float; tokens from n_vocab on
- * have no probability.  If nothing is left of p (p and q agree to rounding) the
+ * have no probability.  If nothing is left of p the
  * draw is from p itself; a row without any logit above -inf gives BCH_NO_TOKEN and the
  * chance 0.  (Tokens that bch_logits_edit leaves out are not drawn, whatever the
  * draft says of them.)  Sequences without new tokens get 0 kept and BCH_NO_TOKEN.  Sums over the vocabulary are
- * f64 of f32 terms: a test or a draw within about 2^-22 of its border may go either way, always
- * the same way.  No counterpart in the reference. */
+ * f64 of f32 terms: a row's sum, and with it its probabilities, are off by E = (1.4·a + 4)·2^-24 of themselves at
+ * most, a the mean over p of log2(largest p / p), by about 2^-22 where logits differ.  A test or a draw that lies within E
+ * of its border may go either way, always the same way; after a rejection within (2·E + 2^-23) / S, S the
+ * part of p that is left, Σ max(p - q, 0), since that is a sum of differences: a draft near its target leaves little, and
+ * which token it is becomes that much less certain.  Each further rejection doubles what stands over S (without
+ * replacement that is over the draft's own rest too); for children chosen without chance it stays 2·E, and S is 1 less their p.
+ * No counterpart in the reference. */
 int bch_verify_drafts(bch_ctx *ctx, const bch_kv_plan *plan, uint32_t first, uint32_t n_seqs, uint32_t n_vocab,
                       const bch_drafts *drafts, const bch_verdict *verdict);
 

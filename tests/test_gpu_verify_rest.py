@@ -107,3 +107,39 @@ def test_sums_of_terms_far_apart(hip, vocab):
     assert bound < 6 * 2.0 ** -24
     chances = got[3].reshape(3, 3)[:, 1:]
     assert (np.abs(chances / want.reshape(3, 3)[:, 1:] - 1) <= bound).all()
+
+
+@pytest.mark.parametrize("spread", [1.0, 0.1, 0.01, 0.001, 0.0003])
+@pytest.mark.parametrize("vocab,n", [(5000, 96), (70001, 24)])
+def test_draws_from_what_a_rejection_leaves(hip, vocab, n, spread):
+    """After a rejection the draw is from (p - q)+ / S, each term the difference of two f32 numbers: p·(1 ± E' ± s), where E'
+    is a term's own error with two more roundings (of 1 / sum and of the product; term_errors has as many for the second
+    exponential that these terms do not have) and s the sum's, q·2^-24 and the difference's own rounding.  So partial sums and S
+    are off by e = 2·term_errors + 2·2^-24, and a place among them by 2·e / S: the token's range holds the uniform, taken
+    that much wider.  S goes down to about 10^-4 here, where 2^-22 of a border would not hold."""
+    rng = np.random.default_rng(vocab)
+    logits = (2 * rng.standard_normal((n, 2, vocab))).astype(np.float32)
+    heat = rng.uniform(0.6, 1.4, n).astype(np.float32)
+    x = logits[:, 0].astype(np.float64) / heat[:, None]
+    p = np.exp(x - x.max(1, keepdims=True))
+    p /= p.sum(1, keepdims=True)
+    q = p * np.exp(spread * rng.standard_normal(p.shape))
+    q = (q / q.sum(1, keepdims=True)).astype(np.float32)
+    draft = np.zeros((n, 2, vocab), np.float32)
+    draft[:, 0] = q
+    child = (q / p).argmax(1)  # rejected: q is some standard deviations above p there
+    tokens = np.stack([np.zeros(n), child], 1).astype(np.uint32).reshape(-1)
+    u = np.stack([rng.random(n, np.float32), np.full(n, BELOW_1)], 1).astype(np.float32)
+    trees = [[-1, 0]] * n
+    got = verdict(hip, plan_of(hip, trees), trees, logits.reshape(-1, vocab), draft.reshape(-1, vocab), tokens, u.reshape(-1), heat)
+    assert (got[0] == 1).all()
+    smallest = 1.0
+    for i in range(n):
+        rest = np.maximum(p[i] - q[i].astype(np.float64), 0)
+        s = rest.sum()
+        off = 2 * (2 * term_errors(logits[i, 0], heat[i]) + 2 * 2.0 ** -24) / s
+        up, t = np.cumsum(rest) / s, int(got[2][i])
+        assert t < vocab and (up[t - 1] if t else 0) - off <= u[i, 0] <= up[t] + off, (i, s, off)
+        assert abs(got[3][2 * i] - p[i, t]) <= (term_errors(logits[i, 0], heat[i]) + 2.0 ** -24) * p[i, t]
+        smallest = min(smallest, s)
+    assert smallest < spread
