@@ -4,9 +4,9 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from _drafts import verify
+from _drafts import chain, random_tree, verify
 from bobcat_amd.backend import NO_TOKEN
-from test_gpu_verify import plan_of, verdict
+from test_gpu_verify import case, plan_of, verdict
 
 pytestmark = pytest.mark.gpu
 
@@ -143,3 +143,43 @@ def test_draws_from_what_a_rejection_leaves(hip, vocab, n, spread):
         assert abs(got[3][2 * i] - p[i, t]) <= (term_errors(logits[i, 0], heat[i]) + 2.0 ** -24) * p[i, t]
         smallest = min(smallest, s)
     assert smallest < spread
+
+
+@pytest.mark.parametrize("mode", ["drawn", "distinct", "chosen"])
+@pytest.mark.parametrize("vocab", [262144, 262145, 600001])
+def test_vocabularies_of_more_pieces_than_lanes(hip, mode, vocab):
+    """64 pieces of 4,096 tokens, one more, and 147: sums in several rounds, and lanes that have several pieces each.  (Logits
+    spread so that some tens of tokens hold nearly all of p: a draw within 2^-20 of a border is a matter of one in 10^4.)"""
+    rng = np.random.default_rng(vocab)
+    trees = [random_tree(rng, 7, width=3), chain(4), [-1], random_tree(rng, 5, width=4)]
+    logits, q, tokens, u, heat = case(rng, trees, vocab, mode, spread=6.0)
+    heat[1] = 0.0 if mode == "chosen" else heat[1]
+    got, row, beyond = verdict(hip, plan_of(hip, trees), trees, logits, q, tokens, u, heat, mode == "distinct"), 0, 0
+    for i, t in enumerate(trees):
+        part = slice(row, row + len(t))
+        kept, path, token, chances = verify(t, logits[part], None if q is None else q[part], tokens[part], u[part], heat[i],
+                                            mode == "distinct")
+        assert got[0][i] == kept and got[1][part].tolist() == path and got[2][i] == token, (i, t)
+        for j, a in enumerate(t):
+            of = path[kept - 1] if j == 0 else a
+            off = term_errors(logits[row + of], heat[i]) + 2.0 ** -24 if heat[i] > 0 else 0
+            assert abs(got[3][row + j] - chances[j]) <= off * chances[j] + 1e-37, (i, j)
+        beyond += token >= 64 * 4096
+        row += len(t)
+    assert beyond > 0 or vocab < 300000
+
+
+def test_draws_in_every_piece(hip):
+    """Next tokens all over a vocabulary of 600,001: of each piece two tokens hold the same mass, a uniform for each."""
+    vocab, piece = 600001, 4096
+    places = np.array([at + d for at in range(0, vocab, piece) for d in (0, min(piece, vocab - at) - 1)])
+    row = np.full(vocab, -np.inf, np.float32)
+    row[places] = 1.5
+    n = 49  # (rows of 2.4 MB each)
+    for first in range(0, places.size, n):
+        some = np.arange(first, min(first + n, places.size))
+        u = ((some + 0.5) / places.size).astype(np.float32)
+        trees = [[-1]] * some.size
+        got = verdict(hip, plan_of(hip, trees), trees, np.tile(row, (some.size, 1)), None, np.zeros(some.size, np.uint32), u,
+                      np.ones(some.size, np.float32))
+        assert np.array_equal(got[2], places[some])
