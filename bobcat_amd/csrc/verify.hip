@@ -430,15 +430,12 @@ struct Walk {
       uint32_t from = first;
       if (per > 1) {
         double at = sum;
-        uint32_t pick = ~0u;
+        bool passed = false;
         for (uint32_t i = first; i < end; i++) {
           const double x = mass(i);
-          if (x > 0 && (pick == ~0u || !inside)) {
-            if (!inside || at + x > goal) pick = i, sum = at;
-          }
+          if (x > 0 && !passed) from = i, sum = at, passed = inside && at + x > goal;
           at += x;
         }
-        from = pick != ~0u ? pick : first;
       }
       sum = lane_f64(sum, __builtin_amdgcn_readfirstlane(owner));
       from = __builtin_amdgcn_readlane((int)from, __builtin_amdgcn_readfirstlane(owner));
