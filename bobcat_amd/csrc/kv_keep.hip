@@ -115,6 +115,8 @@ extern "C" int bch_kv_keep(bch_ctx *ctx, const bch_kv_plan *plan, uint32_t first
   uint32_t *np, *pp, row, tokens;
   BCH_TRY(kv_plan_cache(ctx, "kv_keep", plan, cache, &cp));
   BCH_TRY(kv_plan_range("kv_keep", plan, first, n_seqs, &row, &tokens));
+  // (A workgroup of 256 threads for each: a launch has fewer than 2^32.)
+  if (n_seqs >= 1u << 24) return fail(BCH_ERR_ARGUMENT, "kv_keep: %u sequences", n_seqs);
   const bch_kv_shape &s = plan->shape;
   const uint64_t cache_bytes = bch_kv_page_bytes(&s) * s.n_pages;
   if (n_layers > 1) {

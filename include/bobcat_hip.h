@@ -478,7 +478,7 @@ int bch_rope_paged(bch_ctx *ctx, const bch_rope *rope, const bch_kv_plan *plan, 
  * one for each new token of these sequences, sequence after sequence.  The next
  * batch then has n_past + kept[s] positions.  A path goes up (path[j + 1] > path[j]);
  * entries that do not, or are not below n_new, and counts above n_new move nothing
- * outside the sequence's new tokens.  One launch for the caches of n_layers (at most 128) layers, layer l's
+ * outside the sequence's new tokens.  Fewer than 2^24 sequences in a call.  One launch for the caches of n_layers (at most 128) layers, layer l's
  * layer_bytes·l bytes behind `cache` (a multiple of 16, at least a cache's bytes where
  * there are several). */
 int bch_kv_keep(bch_ctx *ctx, const bch_kv_plan *plan, uint32_t first, uint32_t n_seqs, bch_view cache,
