@@ -143,8 +143,8 @@ __device__ __forceinline__ void put_row(const AttnOut &o, uint32_t part, uint32_
   }
 }
 
-// Workgroups of a CU that the registers let run at once.  (Up to 17 registers of
-// the wide tiles and four of the narrow ones are spilled for it, where an item
+// Workgroups of a CU that the registers let run at once.  (Up to 18 registers of
+// the wide tiles, 39 with TREE, and four of the narrow ones are spilled for it, where an item
 // begins and in the staging; no block with matrix instructions reloads one.)
 constexpr uint32_t token_groups(uint32_t format, uint32_t hd) {
   return format == BCH_KV_F16 ? (hd == 64 ? 4 : hd == 128 ? 2 : 1) : (hd == 64 ? 4 : hd == 128 ? 3 : 2);

@@ -245,18 +245,23 @@ static void deal(KvSchedule &w, KvWork &work, const std::vector<Tile> &tiles, ui
 // Which tiles a batch with trees takes: wide ones, or narrow ones of up to `blocks` times 16
 // rows.  Narrow tiles cost about the same for every block and step of 32 keys once
 // there is work for all waves; a wide one as much as 6.3 blocks in the 8-bit formats,
-// where a narrow tile widens the keys for itself, and 5 in f16, or 3 where the
-// keys are more than the last cache holds and the narrow tiles bring them from memory one after
-// the other.  (32 sequences of up to 6,000 keys, eight KV heads of 128, up to 48, 64, 128
+// where a narrow tile widens the keys for itself, and 5 in f16, or 3 from 128 MB of keys
+// and values on, which the narrow tiles of a tree bring one after the other.  (32 sequences of up to 6,000 keys, eight KV heads of 128, up to 48, 64, 128
 // and 192 rows: int8 82, 106, 177, 213 us narrow and 132, 142, 174, 216 wide; f16 109, 147, 256,
 // 359 and 151, 136, 184, 272.)  Below 16 steps of a block for each wave the time is latency, and tiles of
 // one block share it among more waves (one sequence of 600 keys and 32 rows, heads of 64: 8.2
-// us, in tiles of two 11.3, wide 20.6; twelve of up to 2,500 keys and 96 rows 21, 24 and 36).  Not so in f16 where
-// each tile brings more keys than the caches hold, from 96 MB of them on: five sequences of up to 12,868 keys and 48
+// us, in tiles of two 11.3, wide 20.6; twelve of up to 2,500 keys and 96 rows 21, 24 and 36).  Not so in f16 from 96 MB
+// on: five sequences of up to 12,868 keys and 48
 // rows, heads of 128, 70 us in tiles of one block and 54 by the rule for large batches; eight of up to 6,000 and 64
 // rows 55 and 48; but three of up to 16,000, 90 MB, 32 and 46, and in int8 20 of up to 6,000 43 and 50.  Three
 // blocks beat two only where there is much more (12 of 256 rows: 52 us and 45; 32 of 96 rows and 6,000 keys 73
-// and 75).
+// and 75).  Both edges are measured ones, not a cache's size (the last one has 256 MB): over 81 f16 batches of 47 to 283 MB
+// the rule is within 12% of the best choice but for four, 17 to 25% (profiles/tree_tiles_choice.txt).
+// A prompt in the batch counts with the trees.  It needs the wide kernel in any case, and trees in narrow tiles are
+// a launch more: beside 1,024 or 2,048 tokens the rule takes wide tiles for them, which cost up to 5% more than narrow
+// ones (16 trees of 8 tokens, int8, 86.8 us and 82.6) and up to 17% less; beside 256 tokens it mostly takes narrow ones,
+// up to 38% more than wide ones (16 of 8, f16, heads of 64, 42 us and 30.5).  In none of 90 such batches is one plan
+// more than 5% behind two, the prompt's and the trees'.
 struct TreeTiles {
   bool wide;
   uint32_t blocks;
@@ -273,8 +278,8 @@ static TreeTiles tree_tiles(const std::vector<KvSeq> &seqs, uint32_t group, uint
   }
   const uint64_t waves = 4ull * n_cus * tree_tile_groups(format, head_dim, 1), work = block_steps * n_kv;
   const uint64_t bytes = keys * n_kv * kv_block_bytes(format, head_dim) / kKvBlock;
-  const bool cached = format != BCH_KV_F16 || bytes <= (96ull << 20);
-  if (most == 1 || (work <= 16 * waves && cached)) return {false, 1};
+  const bool shared = format != BCH_KV_F16 || bytes <= (96ull << 20);
+  if (most == 1 || (work <= 16 * waves && shared)) return {false, 1};
   const double ratio = format != BCH_KV_F16 ? 6.3 : bytes <= (128ull << 20) ? 5.0 : 3.0;
   if (ratio * wide_steps < block_steps) return {true, 1};
   return {false, std::min(work <= 32 * waves ? 2u : 3u, tree_tile_rows(format, head_dim) / 16)};

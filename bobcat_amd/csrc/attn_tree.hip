@@ -28,7 +28,8 @@ namespace bch {
 // one block 104; of 256, two KV heads: 70, two blocks 76.  f16, heads of 128, 32 rows of 32
 // sequences of up to 6,000: two blocks with one workgroup a CU 99, one block with two 120;
 // but 12 of up to 2,500, 48 rows, 39 and 30: so there is a kernel for each.  f16, heads of 256, 64 rows,
-// one workgroup a CU 76, two 108 (it spills).
+// one workgroup a CU 76, two 108 (it spills).  (In 8 bits 7 to 14 registers are spilled with heads of 128, 14 to 17 with
+// heads of 256, where an item begins; the loop of whole steps reloads none, that of masked ones 7 of heads of 256.)
 constexpr uint32_t tree_blocks(uint32_t format, uint32_t hd) {
   return hd == 64 ? (format == BCH_KV_F16 ? 2 : 3) : hd == 128 ? 2 : 1;
 }

@@ -40,7 +40,7 @@ constexpr uint32_t kWalkThreads = 256;
 // Rejections of trees that all workgroups sum, a launch each (of chains there is one at most).  Passes with
 // 0, 1, 2, 3, 4, 5 and 6 of them: 16 trees of 16 to 32 drawn drafts, 65,536 logits, 101, 82, 74, 66, 62, 65 and
 // 71 us; 8 of 8 to 16, without replacement, 151,936 logits, 153, 100, 77, 59, 47, 53 and 58; one of 16 drawn ones
-// 51, 42, 33, 32, 34, 39 and 45.
+// 51, 42, 33, 32, 34, 39 and 45.  (With f32 sums within a piece; f64 ones take about 1 us more of each pass.)
 constexpr uint32_t kRounds = 4;
 constexpr float kLargest = 3.402823466e38f;
 

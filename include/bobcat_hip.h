@@ -582,7 +582,8 @@ typedef struct bch_verdict {
  * stay, and the token after them, so that it and they are distributed as if the target had
  * drawn each (speculative sampling on a tree).  A sequence's first new token is the step's
  * own (no draft), and all others descend from it: BCH_ERR_ARGUMENT for a tree with another
- * root, or for more than BCH_MAX_TREE tokens.  From the first token on: with p = softmax(logits /
+ * root, or for more than BCH_MAX_TREE tokens, for rows of more than 2^30 logits, or where tokens (or sequences)
+ * times pieces of 4,096 logits reach 2^23.  From the first token on: with p = softmax(logits /
  * temperature) after the current token and q its draft row, the first child x in order
  * with u·q(x) < p(x) stays and becomes the current token; for each child that does not,
  *   p <- max(p - q, 0), normalised,
